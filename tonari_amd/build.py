@@ -19,12 +19,13 @@ import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
-SOURCES = [os.path.join(HERE, "csrc", "tonari_hip.hip")]
+SOURCES = [os.path.join(HERE, "csrc", name) for name in ("tonari_hip.hip", "tonari_operators.hip")]
 HEADERS = [os.path.join(HERE, "csrc", "nl_device.h"), os.path.join(ROOT, "include", "tonari_hip.h")]
 OUTPUT = os.path.join(HERE, "_lib", "libtonari_hip.so")
 CPU_SOURCES = [os.path.join(HERE, "csrc", "cpu", "nl_cpu.cpp")]
 CPU_OUTPUT = os.path.join(HERE, "_lib", "libtonari_cpu.so")
-TORCH_SOURCES = [os.path.join(HERE, "csrc", "torch", "frontend.cpp")]
+TORCH_SOURCES = [os.path.join(HERE, "csrc", "torch", name)
+                 for name in ("frontend.cpp", "operators.cpp")]
 TORCH_OUTPUT = os.path.join(HERE, "_lib", "_tonari_torch.so")
 ARCH = "gfx950"
 

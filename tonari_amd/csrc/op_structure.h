@@ -1,0 +1,576 @@
+// Attention within the structures of a batch.  For a query i and a key j of
+// one structure at distance r, with x = scale q.k, u = c tanh(x / c) (u = x
+// without a cap) and a slope m of the head:
+//   s = u - m r,  p = softmax_j(s),  o = sum_j p v_j
+// and back, with dp = do.v_j and delta = sum_j p dp:
+//   ds = p (dp - delta),  dx = scale ds (1 - (u / c)^2),
+//   dq = sum_j dx k_j,  dk_j = sum_i dx q_i,  dv_j = sum_i p do_i,
+//   dr = -m ds (to both atoms along their line),  dm = -sum ds r.
+//
+// One pass over the keys with the running maximum and sum of the softmax
+// (scores never leave the registers), in tiles of 32 x 32 on the matrix
+// cores.  The forward and the queries' gradients hold the tile transposed,
+// keys x queries: a lane then has 16 keys of ONE query, so that the row's
+// maximum, sum and rescaling are the lane's own but for one exchange with the
+// lane 32 away, and the weights of the tile are, as they stand in the
+// registers, the right operand of the next product (out^T = v^T p^T); the
+// rows of v^T are read in the order that the weights happen to have.  The
+// keys' gradients hold queries x keys for the same reason.
+//
+// The query heads that share a key head are rows of one tile (row = query *
+// group + head in the group): keys and values are read once for all of them,
+// and one moved atom with 4 query heads to a key head fills 4 rows.
+//
+// The distance is computed in the tile from the positions, 32 bits.  Scores,
+// statistics and sums are 32 bits; the weights p and dx are rounded to the
+// inputs' 16-bit type for the second products.
+#pragma once
+
+#include "op_common.h"
+
+namespace tnr {
+namespace op {
+
+constexpr int kTile = 32;  // keys (or query rows) staged at a time, and rows of a wave
+
+// A workgroup's part of a structure: its rows (or keys) from `first` on.
+// n_q < 0: the batch's pointers are not valid (every result is NaN).
+struct StructureTile {
+    int q_lo, n_q, k_lo, n_k;
+    int first, pad0, pad1, pad2;
+};
+
+struct StructureArgs {
+    const StructureTile* q_tiles;
+    const StructureTile* k_tiles;
+    const void *q, *k, *v;
+    int64_t q_stride[2], k_stride[2], v_stride[2];
+    const float *x_q, *x_k, *slopes;
+    ScoreRule rule;
+    int heads, kv_heads, group, dim;
+    int n_queries, n_keys;
+    int splits;
+    void* out;
+    float* lse;   // [heads][n_queries], base 2
+    float* part;  // forward splits: [split][heads][n_queries][dim + 2]
+    const void* grad_out;
+    void *grad_q, *grad_k, *grad_v;
+    float* row;     // [heads][n_queries][2]: delta, largest |grad_out|
+    float* push_q;  // [heads][n_queries][3], NULL: not wanted
+    float* push_k;  // [kv_heads][n_keys][3]
+    float* turn;    // [heads][n_queries]: the slope's gradient by rows, NULL: not wanted
+};
+
+// ------------------------------------------------------------ the batch's tiles
+
+// Structure b's tiles start at floor(ptr[b] * mult / rows) + b: room for all of
+// them, at a place that no other structure's count is needed for.
+__host__ __device__ inline int64_t tile_start(int64_t at, int64_t mult, int64_t rows, int64_t b) {
+    return at * mult / rows + b;
+}
+
+// Tiles of `q_rows` query rows and of `k_rows` keys.  Every workgroup looks
+// at all pointers, so that no tile of a batch whose pointers are wrong is left
+// valid.
+__global__ __launch_bounds__(256) void k_structure_tiles(const int64_t* q_ptr, const int64_t* k_ptr,
+                                                         int64_t n_structures, int64_t n_queries,
+                                                         int64_t n_keys, int group, int q_rows,
+                                                         int k_rows, StructureTile* q_tiles,
+                                                         StructureTile* k_tiles) {
+    int bad = 0;
+    for (int64_t b = threadIdx.x; b < n_structures; b += 256)
+        bad |= q_ptr[b + 1] < q_ptr[b] || k_ptr[b + 1] < k_ptr[b];
+    if (threadIdx.x == 0)
+        bad |= q_ptr[0] != 0 || k_ptr[0] != 0 || q_ptr[n_structures] != n_queries ||
+               k_ptr[n_structures] != n_keys;
+    bad = __syncthreads_or(bad);
+    const int lane = lane_of();
+    const int64_t waves = (int64_t)gridDim.x * 4;
+    if (bad) {
+        const int64_t nq = tile_start(n_queries, group, q_rows, n_structures);
+        const int64_t nk = tile_start(n_keys, 1, k_rows, n_structures);
+        const StructureTile none{0, -1, 0, -1, 0, 0, 0, 0};
+        for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < nq; i += waves * kWave)
+            q_tiles[i] = none;
+        if (k_tiles)
+            for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < nk; i += waves * kWave)
+                k_tiles[i] = none;
+        return;
+    }
+    for (int64_t b = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave; b < n_structures; b += waves) {
+        const int64_t q0 = q_ptr[b], q1 = q_ptr[b + 1], k0 = k_ptr[b], k1 = k_ptr[b + 1];
+        StructureTile t{(int)q0, (int)(q1 - q0), (int)k0, (int)(k1 - k0), 0, 0, 0, 0};
+        const int64_t from = tile_start(q0, group, q_rows, b);
+        const int64_t to = tile_start(q1, group, q_rows, b + 1);
+        for (int64_t i = from + lane; i < to; i += kWave) {
+            t.first = (int)((i - from) * q_rows);
+            q_tiles[i] = t;
+        }
+        if (!k_tiles) continue;
+        const int64_t kfrom = tile_start(k0, 1, k_rows, b);
+        const int64_t kto = tile_start(k1, 1, k_rows, b + 1);
+        for (int64_t i = kfrom + lane; i < kto; i += kWave) {
+            t.first = (int)((i - kfrom) * k_rows);
+            k_tiles[i] = t;
+        }
+    }
+}
+
+// ---------------------------------------------------------- matrix products
+
+// One staged tile of 32 rows of DP channels in LDS, and the two products with
+// it.  `row` operands contract over channels, `col` operands over the tile's
+// rows, whose order is that in which a lane's 16 results of a product lie:
+// row_of(i, half).
+__device__ __forceinline__ int row_of(int i, int half) { return 8 * (i / 4) + 4 * half + i % 4; }
+
+template <typename T>
+struct Mat;
+
+template <typename T, typename F>
+struct Mat16 {
+    using Frag = Vec<T, 8>;
+    // Rows are 16 bytes longer than their channels, columns 8 bytes longer
+    // than their rows: both then spread over the LDS banks.
+    static constexpr int kRows(int dp) { return kTile * (dp + 8); }
+    static constexpr int kCols(int dp) { return dp * (kTile + 4); }
+
+    // A lane's own row: channels 16 s + 8 half + 0..7.
+    template <int DP>
+    struct Row {
+        Frag x[DP / 16];
+        __device__ __forceinline__ void load(const T* p, int dim) {
+            const int half = lane_of() / 32;
+#pragma unroll
+            for (int s = 0; s < DP / 16; ++s) {
+                const int c = 16 * s + 8 * half;
+                x[s] = Frag{};
+                if (p && c < dim) x[s] = *(const Frag*)(p + c);
+            }
+        }
+        __device__ __forceinline__ float dot(const Row& o) const {
+            float sum = 0.f;
+#pragma unroll
+            for (int s = 0; s < DP / 16; ++s)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sum = fmaf((float)x[s][e], (float)o.x[s][e], sum);
+            return sum_halves(sum);
+        }
+        __device__ __forceinline__ float largest() const {
+            float top = 0.f;
+#pragma unroll
+            for (int s = 0; s < DP / 16; ++s)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf((float)x[s][e]));
+            return max_halves(top);
+        }
+    };
+
+    // acc += tile . row^T
+    template <int DP>
+    static __device__ __forceinline__ void rows(f32x16& acc, const T* tile, const Row<DP>& b) {
+        const int lane = lane_of();
+        const T* p = tile + (lane % 32) * (DP + 8) + 8 * (lane / 32);
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) acc = F::mma(*(const Frag*)(p + 16 * s), b.x[s], acc);
+    }
+
+    // acc[channel block] += tile^T . p
+    template <int DP>
+    static __device__ __forceinline__ void cols(f32x16 (&acc)[DP / 32], const T* tile,
+                                                const float (&p)[16]) {
+        const int lane = lane_of();
+        Frag b[2];
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) b[s][e] = rounded<T>(p[8 * s + e]);
+        const T* at = tile + (lane % 32) * (kTile + 4) + 4 * (lane / 32);
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const T* c = at + d * 32 * (kTile + 4) + 16 * s;
+                const Vec<T, 4> lo = *(const Vec<T, 4>*)c, hi = *(const Vec<T, 4>*)(c + 8);
+                const Frag a = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                acc[d] = F::mma(a, b[s], acc[d]);
+            }
+    }
+
+    // Threads stage units of 4 rows x 8 channels.
+    template <int DP>
+    struct Stage {
+        static constexpr int kUnits = (kTile / 4) * (DP / 8);
+        Frag x[4];
+        __device__ __forceinline__ void load(int unit, const T* base, int64_t stride, int rows,
+                                             int dim) {
+            const int r = 4 * (unit % (kTile / 4)), c = 8 * (unit / (kTile / 4));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[i] = Frag{};
+                if (r + i < rows && c < dim) x[i] = *(const Frag*)(base + (r + i) * stride + c);
+            }
+        }
+        __device__ __forceinline__ void store(int unit, T* row, T* col) const {
+            const int r = 4 * (unit % (kTile / 4)), c = 8 * (unit / (kTile / 4));
+            if (row)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) *(Frag*)(row + (r + i) * (DP + 8) + c) = x[i];
+            if (col)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const Vec<T, 4> t = {x[0][e], x[1][e], x[2][e], x[3][e]};
+                    *(Vec<T, 4>*)(col + (c + e) * (kTile + 4) + r) = t;
+                }
+        }
+    };
+    static constexpr bool kSeparateCols = true;
+};
+
+struct MmaBf16 {
+    static __device__ __forceinline__ f32x16 mma(Vec<bf16, 8> a, Vec<bf16, 8> b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    }
+};
+struct MmaF16 {
+    static __device__ __forceinline__ f32x16 mma(Vec<f16, 8> a, Vec<f16, 8> b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+    }
+};
+template <>
+struct Mat<bf16> : Mat16<bf16, MmaBf16> {};
+template <>
+struct Mat<f16> : Mat16<f16, MmaF16> {};
+
+// 32-bit products: two channels to an instruction, of which the lower lanes
+// take those of the row's first half and the upper lanes the second's, so that
+// a lane reads neighbouring floats.
+template <>
+struct Mat<float> {
+    static constexpr int kRows(int dp) { return kTile * (dp + 4); }
+    static constexpr int kCols(int) { return 0; }
+
+    template <int DP>
+    struct Row {
+        Vec<float, 4> x[DP / 8];
+        __device__ __forceinline__ void load(const float* p, int dim) {
+            const int half = lane_of() / 32;
+#pragma unroll
+            for (int s = 0; s < DP / 8; ++s) {
+                const int c = half * (DP / 2) + 4 * s;
+                x[s] = Vec<float, 4>{};
+                if (p && c < dim) x[s] = *(const Vec<float, 4>*)(p + c);
+            }
+        }
+        __device__ __forceinline__ float dot(const Row& o) const {
+            float sum = 0.f;
+#pragma unroll
+            for (int s = 0; s < DP / 8; ++s)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum = fmaf(x[s][e], o.x[s][e], sum);
+            return sum_halves(sum);
+        }
+        __device__ __forceinline__ float largest() const { return 1.f; }
+    };
+
+    template <int DP>
+    static __device__ __forceinline__ void rows(f32x16& acc, const float* tile, const Row<DP>& b) {
+        const int lane = lane_of();
+        const float* p = tile + (lane % 32) * (DP + 4) + (lane / 32) * (DP / 2);
+#pragma unroll
+        for (int s = 0; s < DP / 8; ++s) {
+            const Vec<float, 4> a = *(const Vec<float, 4>*)(p + 4 * s);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b.x[s][e], acc, 0, 0, 0);
+        }
+    }
+
+    template <int DP>
+    static __device__ __forceinline__ void cols(f32x16 (&acc)[DP / 32], const float* tile,
+                                                const float (&p)[16]) {
+        const int lane = lane_of();
+        const float* at = tile + lane % 32;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(
+                    at[row_of(i, lane / 32) * (DP + 4) + 32 * d], p[i], acc[d], 0, 0, 0);
+    }
+
+    // Threads stage units of 4 rows x 4 channels.
+    template <int DP>
+    struct Stage {
+        static constexpr int kUnits = (kTile / 4) * (DP / 4);
+        Vec<float, 4> x[4];
+        __device__ __forceinline__ void load(int unit, const float* base, int64_t stride, int rows,
+                                             int dim) {
+            const int r = unit / (DP / 4), c = 4 * (unit % (DP / 4));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[i] = Vec<float, 4>{};
+                if (r + 8 * i < rows && c < dim)
+                    x[i] = *(const Vec<float, 4>*)(base + (r + 8 * i) * stride + c);
+            }
+        }
+        __device__ __forceinline__ void store(int unit, float* row, float*) const {
+            const int r = unit / (DP / 4), c = 4 * (unit % (DP / 4));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) *(Vec<float, 4>*)(row + (r + 8 * i) * (DP + 4) + c) = x[i];
+        }
+    };
+    static constexpr bool kSeparateCols = false;
+};
+
+// Two staged tensors of 32 rows; the workgroup's threads share the units.
+template <typename T, int DP, int NW>
+struct StagePair {
+    using S = typename Mat<T>::template Stage<DP>;
+    static constexpr int kAll = 2 * S::kUnits, kThreads = NW * kWave;
+    static constexpr int kEach = (kAll + kThreads - 1) / kThreads;
+    S s[kEach];
+    // the rows' addresses: base + row * stride
+    __device__ __forceinline__ void load(const T* a, int64_t a_stride, const T* b, int64_t b_stride,
+                                         int rows, int dim) {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const int u = threadIdx.x + i * kThreads;
+            if (u < S::kUnits)
+                s[i].load(u, a, a_stride, rows, dim);
+            else if (u < kAll)
+                s[i].load(u - S::kUnits, b, b_stride, rows, dim);
+        }
+    }
+    __device__ __forceinline__ void store(T* a_row, T* a_col, T* b_row, T* b_col) const {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const int u = threadIdx.x + i * kThreads;
+            if (u < S::kUnits)
+                s[i].store(u, a_row, a_col);
+            else if (u < kAll)
+                s[i].store(u - S::kUnits, b_row, b_col);
+        }
+    }
+};
+
+// ------------------------------------------------------------------ forward
+
+// Channels 8 (i / 4) + 4 half + i % 4 of block d: groups of four, written whole.
+template <typename T, int DP>
+__device__ __forceinline__ void store_channels(T* row, int dim, const f32x16 (&acc)[DP / 32],
+                                               float by) {
+    const int half = lane_of() / 32;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int c = 32 * d + 8 * g + 4 * half;
+            if (c >= dim) continue;
+            const float x[4] = {acc[d][4 * g] * by, acc[d][4 * g + 1] * by, acc[d][4 * g + 2] * by,
+                                acc[d][4 * g + 3] * by};
+            store_floats<T, 4>(row + c, x);
+        }
+}
+
+// u log2(e) of 16 products; t = tanh where the gradient needs it.
+template <bool GRAD>
+__device__ __forceinline__ void capped(const f32x16& acc, const ScoreRule& rule, float (&u)[16],
+                                       float (&t)[GRAD ? 16 : 1]) {
+    if (rule.cap > 0.f) {
+        float top = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            u[i] = acc[i] * rule.inv;
+            top = fmaxf(top, fabsf(u[i]));
+        }
+        if (__builtin_amdgcn_ballot_w64(!(top <= kTanhNear)) == 0) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) u[i] = tanh_near(u[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) u[i] = tanh_of(u[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            if (GRAD) t[i] = u[i];
+            u[i] *= rule.cap2;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) u[i] = acc[i] * rule.scale2;
+    }
+}
+
+// grid: (tiles, kv_heads * splits); NW waves of 32 query rows each.
+template <typename T, int DP, int NW>
+__global__ __launch_bounds__(NW* kWave) void k_structure_forward(const StructureArgs a) {
+    using M = Mat<T>;
+    using Row = typename M::template Row<DP>;
+    __shared__ alignas(16) T k_rows[M::kRows(DP)];
+    __shared__ alignas(16) T v_tile[M::kSeparateCols ? M::kCols(DP) : M::kRows(DP)];
+    __shared__ alignas(16) float4 x_k[kTile];
+
+    const StructureTile t = a.q_tiles[blockIdx.x];
+    const int lane = lane_of(), half = lane / 32, wave = threadIdx.x / kWave;
+    const int kv = blockIdx.y % a.kv_heads, split = blockIdx.y / a.kv_heads;
+    const int g = a.group;
+    if (t.n_q < 0) {  // NaN for the rows that lie here in the batch
+        const int64_t all = (int64_t)a.n_queries * g;
+        const int64_t row = (int64_t)blockIdx.x * (NW * kTile) + wave * kTile + lane % 32;
+        if (row >= all || split > 0 || half) return;
+        const int query = (int)(row / g), head = kv * g + (int)(row % g);
+        T* out = (T*)a.out + ((int64_t)query * a.heads + head) * a.dim;
+        for (int c = 0; c < a.dim; ++c) out[c] = rounded<T>(nan_of());
+        if (a.lse) a.lse[(int64_t)head * a.n_queries + query] = nan_of();
+        if (a.splits > 1)
+            for (int s = 0; s < a.splits; ++s) {
+                float* part = a.part + (((int64_t)s * a.heads + head) * a.n_queries + query) *
+                                           (a.dim + 2);
+                for (int c = 0; c < a.dim; ++c) part[c] = nan_of();
+                part[a.dim] = 0.f;
+                part[a.dim + 1] = 1.f;
+            }
+        return;
+    }
+    const int rows = t.n_q * g;
+    if (t.first >= rows) return;
+
+    const int row = t.first + wave * kTile + lane % 32;
+    const bool valid = row < rows;
+    const int query = t.q_lo + (valid ? row / g : 0), head = kv * g + (valid ? row % g : 0);
+    Row qr;
+    qr.load(valid ? (const T*)a.q + (int64_t)query * a.q_stride[0] + head * a.q_stride[1] : nullptr,
+            a.dim);
+    float xq = 0.f, yq = 0.f, zq = 0.f, slope2 = 0.f;
+    if (valid) {
+        xq = a.x_q[3 * (int64_t)query];
+        yq = a.x_q[3 * (int64_t)query + 1];
+        zq = a.x_q[3 * (int64_t)query + 2];
+        slope2 = a.slopes[head] * kLog2e;
+    }
+    const T* kb = (const T*)a.k + (int64_t)t.k_lo * a.k_stride[0] + kv * a.k_stride[1];
+    const T* vb = (const T*)a.v + (int64_t)t.k_lo * a.v_stride[0] + kv * a.v_stride[1];
+    const float* xb = a.x_k + 3 * (int64_t)t.k_lo;
+
+    const int tiles = (t.n_k + kTile - 1) / kTile;
+    const int each = (tiles + a.splits - 1) / a.splits;
+    const int from = min(tiles, split * each), to = min(tiles, from + each);
+
+    f32x16 acc[DP / 32];
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) acc[d] = f32x16{};
+    float top = -inf_of(), sum = 0.f;
+
+    StagePair<T, DP, NW> stage;
+    float4 xs{};
+    const auto fetch = [&](int tile) {
+        const int k0 = tile * kTile, n = t.n_k - k0;
+        stage.load(kb + (int64_t)k0 * a.k_stride[0], a.k_stride[0],
+                   vb + (int64_t)k0 * a.v_stride[0], a.v_stride[0], n, a.dim);
+        if (threadIdx.x < kTile && (int)threadIdx.x < n) {
+            const float* p = xb + 3 * (int64_t)(k0 + threadIdx.x);
+            xs = float4{p[0], p[1], p[2], 0.f};
+        }
+    };
+    if (from < to) fetch(from);
+    for (int tile = from; tile < to; ++tile) {
+        __syncthreads();
+        if constexpr (M::kSeparateCols)
+            stage.store(k_rows, nullptr, nullptr, v_tile);
+        else
+            stage.store(k_rows, nullptr, v_tile, nullptr);
+        if (threadIdx.x < kTile) x_k[threadIdx.x] = xs;
+        __syncthreads();
+        if (tile + 1 < to) fetch(tile + 1);
+
+        f32x16 dot{};
+        M::template rows<DP>(dot, k_rows, qr);
+        float s[16], unused[1];
+        capped<false>(dot, a.rule, s, unused);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float4 x = x_k[row_of(i, half)];
+            const float dx = xq - x.x, dy = yq - x.y, dz = zq - x.z;
+            const float r = __builtin_amdgcn_sqrtf(fmaf(dx, dx, fmaf(dy, dy, dz * dz)));
+            s[i] = fmaf(-slope2, r, s[i]);
+        }
+        const int left = t.n_k - tile * kTile;
+        if (left < kTile)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = row_of(i, half) < left ? s[i] : -inf_of();
+        float high = s[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) high = fmaxf(high, s[i]);
+        high = fmaxf(top, max_halves(high));
+        const float ref = high == -inf_of() ? 0.f : high;  // nothing but -inf so far
+        const float fade = exp2_of(top - ref);
+        top = high;
+        float part = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            s[i] = exp2_of(s[i] - ref);
+            part += s[i];
+        }
+        sum = fmaf(sum, fade, part);
+        if (__builtin_amdgcn_ballot_w64(fade != 1.f) != 0)
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d) acc[d] *= fade;
+        M::template cols<DP>(acc, v_tile, s);
+    }
+    sum = sum_halves(sum);
+    if (!valid) return;
+    if (a.splits > 1) {
+        float* part =
+            a.part + (((int64_t)split * a.heads + head) * a.n_queries + query) * (a.dim + 2);
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int c = 32 * d + row_of(i, half);
+                if (c < a.dim) part[c] = acc[d][i];
+            }
+        if (half == 0) {
+            part[a.dim] = top;
+            part[a.dim + 1] = sum;
+        }
+        return;
+    }
+    const float by = sum == 0.f ? 0.f : 1.f / sum;
+    store_channels<T, DP>((T*)a.out + ((int64_t)query * a.heads + head) * a.dim, a.dim, acc, by);
+    if (a.lse && half == 0)
+        a.lse[(int64_t)head * a.n_queries + query] =
+            sum == 0.f ? -inf_of() : top + __builtin_amdgcn_logf(sum);
+}
+
+// Joins the splits of a row: one wave each, lanes over channels.
+template <typename T>
+__global__ __launch_bounds__(256) void k_structure_join(const StructureArgs a) {
+    const int64_t at = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
+    const int64_t rows = (int64_t)a.heads * a.n_queries;
+    if (at >= rows) return;
+    const int lane = lane_of();
+    const int64_t step = rows * (a.dim + 2);
+    const float* part = a.part + at * (a.dim + 2);
+    float top = -inf_of();
+    for (int s = 0; s < a.splits; ++s) top = fmaxf(top, part[s * step + a.dim]);
+    const float ref = top == -inf_of() ? 0.f : top;
+    float sum = 0.f, x0 = 0.f, x1 = 0.f;
+    for (int s = 0; s < a.splits; ++s) {
+        const float* p = part + s * step;
+        const float w = exp2_of(p[a.dim] - ref);
+        sum = fmaf(w, p[a.dim + 1], sum);
+        if (lane < a.dim) x0 = fmaf(w, p[lane], x0);
+        if (lane + kWave < a.dim) x1 = fmaf(w, p[lane + kWave], x1);
+    }
+    const int head = (int)(at / a.n_queries), query = (int)(at % a.n_queries);
+    const float by = sum == 0.f ? 0.f : 1.f / sum;
+    T* out = (T*)a.out + ((int64_t)query * a.heads + head) * a.dim;
+    if (lane < a.dim) out[lane] = rounded<T>(x0 * by);
+    if (lane + kWave < a.dim) out[lane + kWave] = rounded<T>(x1 * by);
+    if (a.lse && lane == 0)
+        a.lse[at] = sum == 0.f ? -inf_of() : ref + __builtin_amdgcn_logf(sum);
+}
+
+}  // namespace op
+}  // namespace tnr

@@ -1,0 +1,426 @@
+// The gradients of structure attention (op_structure.h has the formulas), in
+// two passes that both recompute a tile's weights from the forward's row
+// statistics: by queries (grad_q, and for every row delta, its own share of
+// the positions' gradient and the slope's) and by keys (grad_k, grad_v and the
+// keys' share of the positions' gradient).  Neither needs an atomic, so the
+// sums' order is fixed by the sizes.
+//
+// delta = do.o from the rounded output is good enough for grad_q, grad_k and
+// grad_v, which are rounded to the same type, but not for the gradients of
+// positions and slopes, which are 32-bit: the queries' pass also sums
+// e = sum p (dp - do.o), which is what the rounding of o left out, and
+// corrects by it: sum p (dp - delta) f = sum p (dp - do.o) f - e sum p f.
+//
+// float16: dx is scaled by a power of two that follows |do| (of the row, or the
+// largest so far of the rows that a key has met), and p by 2^12, so that
+// neither small upstream gradients nor the small weights of long rows fall out
+// of the type's range.  bfloat16 has the range of 32 bits.
+#pragma once
+
+#include "op_structure.h"
+
+namespace tnr {
+namespace op {
+
+template <typename T>
+constexpr bool kNarrow = false;
+template <>
+constexpr bool kNarrow<f16> = true;
+
+constexpr int kNoScale = -1000;
+
+// Sums of a query row besides grad_q: e, sum (ds u, p u) for the unit vectors
+// u, sum (ds r, p r).
+constexpr int kRowSums = 9;
+
+__device__ __forceinline__ float power_of(int e) { return __builtin_amdgcn_ldexpf(1.f, e); }
+__device__ __forceinline__ int exponent_of(float x) {
+    return x > 0.f && x < inf_of() ? __builtin_amdgcn_frexp_expf(x) : 0;
+}
+
+// What a row's sums make, for its own lane.
+__device__ __forceinline__ void finish_row(const StructureArgs& a, int head, int query,
+                                           float delta, float largest, float slope,
+                                           const float (&w)[kRowSums]) {
+    const int64_t at = (int64_t)head * a.n_queries + query;
+    a.row[2 * at] = delta + w[0];
+    a.row[2 * at + 1] = largest;
+    if (a.push_q)
+        for (int c = 0; c < 3; ++c) a.push_q[3 * at + c] = -slope * (w[1 + c] - w[0] * w[4 + c]);
+    if (a.turn) a.turn[at] = -(w[7] - w[0] * w[8]);
+}
+
+// grid: (query tiles, kv_heads * splits).
+template <typename T, int DP, int NW>
+__global__ __launch_bounds__(NW* kWave) void k_structure_dq(const StructureArgs a) {
+    using M = Mat<T>;
+    using Row = typename M::template Row<DP>;
+    __shared__ alignas(16) T k_rows[M::kRows(DP)];
+    __shared__ alignas(16) T k_cols[M::kSeparateCols ? M::kCols(DP) : 8];
+    __shared__ alignas(16) T v_rows[M::kRows(DP)];
+    __shared__ alignas(16) float4 x_k[kTile];
+
+    const StructureTile t = a.q_tiles[blockIdx.x];
+    const int lane = lane_of(), half = lane / 32, wave = threadIdx.x / kWave;
+    const int kv = blockIdx.y % a.kv_heads, split = blockIdx.y / a.kv_heads;
+    const int g = a.group;
+    if (t.n_q < 0) {
+        const int64_t row = (int64_t)blockIdx.x * (NW * kTile) + wave * kTile + lane % 32;
+        if (row >= (int64_t)a.n_queries * g || half) return;
+        const int query = (int)(row / g), head = kv * g + (int)(row % g);
+        const int64_t at = (int64_t)head * a.n_queries + query;
+        if (a.splits > 1) {
+            float* part = a.part + ((int64_t)split * a.heads * a.n_queries + at) * (a.dim + kRowSums);
+            for (int c = 0; c < a.dim + kRowSums; ++c) part[c] = nan_of();
+            return;
+        }
+        T* dq = (T*)a.grad_q + ((int64_t)query * a.heads + head) * a.dim;
+        for (int c = 0; c < a.dim; ++c) dq[c] = rounded<T>(nan_of());
+        const float w[kRowSums] = {nan_of()};
+        finish_row(a, head, query, 0.f, 1.f, 1.f, w);
+        return;
+    }
+    const int rows = t.n_q * g;
+    if (t.first >= rows) return;
+
+    const int row = t.first + wave * kTile + lane % 32;
+    const bool valid = row < rows;
+    const int query = t.q_lo + (valid ? row / g : 0), head = kv * g + (valid ? row % g : 0);
+    const int64_t at = (int64_t)head * a.n_queries + query;
+    const int64_t flat = ((int64_t)query * a.heads + head) * a.dim;
+    Row qr, dor;
+    qr.load(valid ? (const T*)a.q + (int64_t)query * a.q_stride[0] + head * a.q_stride[1] : nullptr,
+            a.dim);
+    dor.load(valid ? (const T*)a.grad_out + flat : nullptr, a.dim);
+    float delta, largest = 1.f;
+    {
+        Row o;
+        o.load(valid ? (const T*)a.out + flat : nullptr, a.dim);
+        delta = dor.dot(o);
+    }
+    float unit = 1.f;
+    if (kNarrow<T>) {
+        largest = dor.largest();
+        unit = power_of(-exponent_of(largest));
+    }
+    float xq = 0.f, yq = 0.f, zq = 0.f, slope = 0.f, lse = inf_of();
+    if (valid) {
+        xq = a.x_q[3 * (int64_t)query];
+        yq = a.x_q[3 * (int64_t)query + 1];
+        zq = a.x_q[3 * (int64_t)query + 2];
+        slope = a.slopes[head];
+        lse = a.lse[at];
+        if (lse == -inf_of()) lse = inf_of();  // no weight anywhere
+    }
+    const float slope2 = slope * kLog2e;
+    const bool geometry = a.push_q != nullptr || a.push_k != nullptr || a.turn != nullptr;
+    const T* kb = (const T*)a.k + (int64_t)t.k_lo * a.k_stride[0] + kv * a.k_stride[1];
+    const T* vb = (const T*)a.v + (int64_t)t.k_lo * a.v_stride[0] + kv * a.v_stride[1];
+    const float* xb = a.x_k + 3 * (int64_t)t.k_lo;
+
+    const int tiles = (t.n_k + kTile - 1) / kTile;
+    const int each = (tiles + a.splits - 1) / a.splits;
+    const int from = min(tiles, split * each), to = min(tiles, from + each);
+
+    f32x16 acc[DP / 32];
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) acc[d] = f32x16{};
+    float w[kRowSums];
+#pragma unroll
+    for (int i = 0; i < kRowSums; ++i) w[i] = 0.f;
+
+    StagePair<T, DP, NW> stage;
+    float4 xs{};
+    const auto fetch = [&](int tile) {
+        const int k0 = tile * kTile, n = t.n_k - k0;
+        stage.load(kb + (int64_t)k0 * a.k_stride[0], a.k_stride[0],
+                   vb + (int64_t)k0 * a.v_stride[0], a.v_stride[0], n, a.dim);
+        if (threadIdx.x < kTile && (int)threadIdx.x < n) {
+            const float* p = xb + 3 * (int64_t)(k0 + threadIdx.x);
+            xs = float4{p[0], p[1], p[2], 0.f};
+        }
+    };
+    if (from < to) fetch(from);
+    for (int tile = from; tile < to; ++tile) {
+        __syncthreads();
+        stage.store(k_rows, M::kSeparateCols ? k_cols : nullptr, v_rows, nullptr);
+        if (threadIdx.x < kTile) x_k[threadIdx.x] = xs;
+        __syncthreads();
+        if (tile + 1 < to) fetch(tile + 1);
+
+        f32x16 dot{}, dp{};
+        M::template rows<DP>(dot, k_rows, qr);
+        M::template rows<DP>(dp, v_rows, dor);
+        float p[16], th[16];
+        capped<true>(dot, a.rule, p, th);
+        const int left = t.n_k - tile * kTile;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float4 x = x_k[row_of(i, half)];
+            const float dx = xq - x.x, dy = yq - x.y, dz = zq - x.z;
+            const float r = __builtin_amdgcn_sqrtf(fmaf(dx, dx, fmaf(dy, dy, dz * dz)));
+            float s = exp2_of(fmaf(-slope2, r, p[i]) - lse);
+            if (left < kTile && row_of(i, half) >= left) s = 0.f;
+            const float ds = s * (dp[i] - delta);
+            if (geometry) {
+                const float over = r > 0.f ? __builtin_amdgcn_rcpf(r) : 0.f;
+                const float wd = ds * over, wp = s * over;
+                w[0] += ds;
+                w[1] = fmaf(wd, dx, w[1]);
+                w[2] = fmaf(wd, dy, w[2]);
+                w[3] = fmaf(wd, dz, w[3]);
+                w[4] = fmaf(wp, dx, w[4]);
+                w[5] = fmaf(wp, dy, w[5]);
+                w[6] = fmaf(wp, dz, w[6]);
+                w[7] = fmaf(ds, r, w[7]);
+                w[8] = fmaf(s, r, w[8]);
+            }
+            p[i] = ds * unit;
+        }
+        if (a.rule.cap > 0.f)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) p[i] *= fmaf(-th[i], th[i], 1.f);
+        M::template cols<DP>(acc, M::kSeparateCols ? k_cols : k_rows, p);
+    }
+#pragma unroll
+    for (int i = 0; i < kRowSums; ++i) w[i] = sum_halves(w[i]);
+    if (!valid) return;
+    if (a.splits > 1) {
+        float* part = a.part + ((int64_t)split * a.heads * a.n_queries + at) * (a.dim + kRowSums);
+        const float by = 1.f / unit;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int c = 32 * d + row_of(i, half);
+                if (c < a.dim) part[c] = acc[d][i] * by;
+            }
+        if (half == 0)
+#pragma unroll
+            for (int i = 0; i < kRowSums; ++i) part[a.dim + i] = w[i];
+        return;
+    }
+    store_channels<T, DP>((T*)a.grad_q + flat, a.dim, acc, a.rule.scale / unit);
+    if (half == 0) finish_row(a, head, query, delta, largest, slope, w);
+}
+
+// Joins the splits of a row of the queries' pass: one wave each.
+template <typename T>
+__global__ __launch_bounds__(256) void k_structure_join_dq(const StructureArgs a) {
+    const int64_t at = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
+    const int64_t rows = (int64_t)a.heads * a.n_queries;
+    if (at >= rows) return;
+    const int lane = lane_of();
+    const int head = (int)(at / a.n_queries), query = (int)(at % a.n_queries);
+    const int64_t flat = ((int64_t)query * a.heads + head) * a.dim;
+    const int64_t step = rows * (a.dim + kRowSums);
+    const float* part = a.part + at * (a.dim + kRowSums);
+    float x0 = 0.f, x1 = 0.f, w[kRowSums] = {};
+    for (int s = 0; s < a.splits; ++s) {
+        const float* p = part + s * step;
+        if (lane < a.dim) x0 += p[lane];
+        if (lane + kWave < a.dim) x1 += p[lane + kWave];
+        for (int i = 0; i < kRowSums; ++i) w[i] += p[a.dim + i];
+    }
+    float delta = 0.f, top = 0.f;
+    for (int c = lane; c < a.dim; c += kWave) {
+        const float go = (float)((const T*)a.grad_out)[flat + c];
+        delta = fmaf(go, (float)((const T*)a.out)[flat + c], delta);
+        top = fmaxf(top, fabsf(go));
+    }
+    for (int d = 32; d > 0; d >>= 1) {
+        delta += __shfl_xor(delta, d);
+        top = fmaxf(top, __shfl_xor(top, d));
+    }
+    T* dq = (T*)a.grad_q + flat;
+    if (lane < a.dim) dq[lane] = rounded<T>(x0 * a.rule.scale);
+    if (lane + kWave < a.dim) dq[lane + kWave] = rounded<T>(x1 * a.rule.scale);
+    if (lane == 0) finish_row(a, head, query, delta, top, a.slopes[head], w);
+}
+
+// grid: (key tiles, kv_heads); NW waves of 32 keys each.
+template <typename T, int DP, int NW>
+__global__ __launch_bounds__(NW* kWave) void k_structure_dkv(const StructureArgs a) {
+    using M = Mat<T>;
+    using Row = typename M::template Row<DP>;
+    constexpr float kLift = kNarrow<T> ? 12.f : 0.f;
+    constexpr float kLower = kNarrow<T> ? 1.f / 4096.f : 1.f;
+    __shared__ alignas(16) T q_rows[M::kRows(DP)];
+    __shared__ alignas(16) T o_rows[M::kRows(DP)];
+    __shared__ alignas(16) T q_cols[M::kSeparateCols ? M::kCols(DP) : 8];
+    __shared__ alignas(16) T o_cols[M::kSeparateCols ? M::kCols(DP) : 8];
+    __shared__ alignas(16) float4 x_q[kTile];   // position, largest |grad_out|
+    __shared__ alignas(16) float2 stat[kTile];  // log-sum, delta
+
+    const StructureTile t = a.k_tiles[blockIdx.x];
+    const int lane = lane_of(), half = lane / 32, wave = threadIdx.x / kWave;
+    const int kv = blockIdx.y;
+    if (t.n_q < 0) {
+        const int64_t key = (int64_t)blockIdx.x * (NW * kTile) + wave * kTile + lane % 32;
+        if (key >= a.n_keys || half) return;
+        for (int c = 0; c < a.dim; ++c) {
+            ((T*)a.grad_k)[(key * a.kv_heads + kv) * a.dim + c] = rounded<T>(nan_of());
+            ((T*)a.grad_v)[(key * a.kv_heads + kv) * a.dim + c] = rounded<T>(nan_of());
+        }
+        if (a.push_k)
+            for (int c = 0; c < 3; ++c)
+                a.push_k[3 * ((int64_t)kv * a.n_keys + key) + c] = nan_of();
+        return;
+    }
+    if (t.first >= t.n_k) return;
+    const int place = t.first + wave * kTile + lane % 32;
+    const bool valid = place < t.n_k;
+    const int64_t key = t.k_lo + (valid ? place : 0);
+    Row kr, vr;
+    kr.load(valid ? (const T*)a.k + key * a.k_stride[0] + kv * a.k_stride[1] : nullptr, a.dim);
+    vr.load(valid ? (const T*)a.v + key * a.v_stride[0] + kv * a.v_stride[1] : nullptr, a.dim);
+    const float xk = valid ? a.x_k[3 * key] : 0.f, yk = valid ? a.x_k[3 * key + 1] : 0.f,
+                zk = valid ? a.x_k[3 * key + 2] : 0.f;
+
+    f32x16 dk[DP / 32], dv[DP / 32];
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) dk[d] = dv[d] = f32x16{};
+    float px = 0.f, py = 0.f, pz = 0.f;
+    int scale_e = kNoScale;  // exponent of what dk is held in
+
+    const int per_head = (t.n_q + kTile - 1) / kTile, tiles = per_head * a.group;
+    StagePair<T, DP, NW> stage;
+    float4 xs{};
+    float2 ss{};
+    const auto fetch = [&](int tile) {
+        const int head = kv * a.group + tile / per_head;
+        const int q0 = (tile % per_head) * kTile, n = t.n_q - q0;
+        const int64_t first = t.q_lo + q0;
+        stage.load((const T*)a.q + first * a.q_stride[0] + head * a.q_stride[1], a.q_stride[0],
+                   (const T*)a.grad_out + (first * a.heads + head) * a.dim,
+                   (int64_t)a.heads * a.dim, n, a.dim);
+        if (threadIdx.x < kTile) {
+            xs = float4{0.f, 0.f, 0.f, 0.f};
+            ss = float2{inf_of(), 0.f};
+            if ((int)threadIdx.x < n) {
+                const int64_t query = first + threadIdx.x;
+                const int64_t at = (int64_t)head * a.n_queries + query;
+                xs = float4{a.x_q[3 * query], a.x_q[3 * query + 1], a.x_q[3 * query + 2],
+                            a.row[2 * at + 1]};
+                ss = float2{a.lse[at], a.row[2 * at]};
+                if (ss.x == -inf_of()) ss.x = inf_of();
+            }
+        }
+    };
+    if (tiles > 0) fetch(0);
+    for (int tile = 0; tile < tiles; ++tile) {
+        __syncthreads();
+        stage.store(q_rows, M::kSeparateCols ? q_cols : nullptr, o_rows,
+                    M::kSeparateCols ? o_cols : nullptr);
+        if (threadIdx.x < kTile) {
+            x_q[threadIdx.x] = xs;
+            stat[threadIdx.x] = ss;
+        }
+        __syncthreads();
+        const float slope = a.slopes[kv * a.group + tile / per_head], slope2 = slope * kLog2e;
+        if (tile + 1 < tiles) fetch(tile + 1);
+
+        f32x16 dot{}, dp{};
+        M::template rows<DP>(dot, q_rows, kr);
+        M::template rows<DP>(dp, o_rows, vr);
+        float p[16], th[16], dx[16];
+        capped<true>(dot, a.rule, p, th);
+        float tile_top = 0.f, ux = 0.f, uy = 0.f, uz = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float4 x = x_q[row_of(i, half)];
+            const float2 st = stat[row_of(i, half)];
+            const float ex = x.x - xk, ey = x.y - yk, ez = x.z - zk;
+            const float r = __builtin_amdgcn_sqrtf(fmaf(ex, ex, fmaf(ey, ey, ez * ez)));
+            p[i] = exp2_of(fmaf(-slope2, r, p[i]) - st.x + kLift);
+            const float ds = p[i] * kLower * (dp[i] - st.y);
+            if (a.push_k) {
+                const float wd = ds * (r > 0.f ? __builtin_amdgcn_rcpf(r) : 0.f);
+                ux = fmaf(wd, ex, ux);
+                uy = fmaf(wd, ey, uy);
+                uz = fmaf(wd, ez, uz);
+            }
+            if (kNarrow<T>) tile_top = fmaxf(tile_top, x.w);
+            dx[i] = ds;
+        }
+        px = fmaf(slope, ux, px);
+        py = fmaf(slope, uy, py);
+        pz = fmaf(slope, uz, pz);
+        if (a.rule.cap > 0.f)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) dx[i] *= fmaf(-th[i], th[i], 1.f);
+        if (kNarrow<T>) {
+            tile_top = max_halves(tile_top);
+            const int e = exponent_of(tile_top);
+            if (tile_top > 0.f && e > scale_e) {  // (all zeros: dx is zero whatever the scale)
+                const float by = scale_e == kNoScale ? 1.f : power_of(scale_e - e);
+#pragma unroll
+                for (int d = 0; d < DP / 32; ++d) dk[d] *= by;
+                scale_e = e;
+            }
+            const float unit = scale_e == kNoScale ? 1.f : power_of(-scale_e);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) dx[i] *= unit;
+        }
+        M::template cols<DP>(dv, M::kSeparateCols ? o_cols : o_rows, p);
+        M::template cols<DP>(dk, M::kSeparateCols ? q_cols : q_rows, dx);
+    }
+    px = sum_halves(px);
+    py = sum_halves(py);
+    pz = sum_halves(pz);
+    if (!valid) return;
+    const int64_t flat = (key * a.kv_heads + kv) * a.dim;
+    const float back = kNarrow<T> && scale_e != kNoScale ? power_of(scale_e) : 1.f;
+    store_channels<T, DP>((T*)a.grad_k + flat, a.dim, dk, a.rule.scale * back);
+    store_channels<T, DP>((T*)a.grad_v + flat, a.dim, dv, kLower);
+    if (a.push_k && half == 0) {
+        float* push = a.push_k + 3 * ((int64_t)kv * a.n_keys + key);
+        push[0] = px;
+        push[1] = py;
+        push[2] = pz;
+    }
+}
+
+// Sums over the heads: positions' gradients (threads over atoms and axes), and
+// over all rows: a slope's (one workgroup each, the first `heads` of the grid
+// where slopes are wanted).
+__global__ __launch_bounds__(256) void k_structure_finish(const StructureArgs a, float* grad_x_q,
+                                                          float* grad_x_k, float* grad_slopes,
+                                                          int shared) {
+    int64_t block = blockIdx.x;
+    if (grad_slopes) {
+        if (block < a.heads) {
+            __shared__ float waves[4];
+            const float* from = a.turn + block * a.n_queries;
+            float sum = 0.f;
+            for (int64_t i = threadIdx.x; i < a.n_queries; i += 256) sum += from[i];
+            for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
+            if (lane_of() == 0) waves[threadIdx.x / kWave] = sum;
+            __syncthreads();
+            if (threadIdx.x == 0) grad_slopes[block] = waves[0] + waves[1] + waves[2] + waves[3];
+            return;
+        }
+        block -= a.heads;
+    }
+    const int64_t nk = 3 * (int64_t)a.n_keys, nq = 3 * (int64_t)a.n_queries;
+    int64_t i = block * 256 + threadIdx.x;
+    if (grad_x_k) {
+        if (i < nk) {
+            float sum = 0.f;
+            for (int h = 0; h < a.kv_heads; ++h) sum += a.push_k[h * nk + i];
+            if (shared)
+                for (int h = 0; h < a.heads; ++h) sum += a.push_q[h * nq + i];
+            grad_x_k[i] = sum;
+            return;
+        }
+        i -= nk;
+    }
+    if (grad_x_q && i < nq) {
+        float sum = 0.f;
+        for (int h = 0; h < a.heads; ++h) sum += a.push_q[h * nq + i];
+        grad_x_q[i] = sum;
+    }
+}
+
+}  // namespace op
+}  // namespace tnr

@@ -1,0 +1,755 @@
+// C ABI of the operators (include/tonari_operators.h): checks of requests,
+// workspaces and launches.  Every call returns a code; no exception crosses it.
+#include "op_embedding.h"
+#include "op_neighbor.h"
+#include "op_structure_backward.h"
+
+#include <cstdio>
+
+using namespace tnr::op;
+
+namespace {
+
+int refuse(char* err, size_t len, const char* message) {
+    if (err && len) std::snprintf(err, len, "%s", message);
+    return TNR_INPUT_ERROR;
+}
+
+int launched(char* err, size_t len) {
+    const hipError_t e = hipGetLastError();
+    if (e == hipSuccess) return TNR_OK;
+    if (err && len) std::snprintf(err, len, "HIP error: %s", hipGetErrorString(e));
+    return TNR_DEVICE_ERROR;
+}
+
+bool is_type(int32_t dtype) {
+    return dtype == TNR_FLOAT32 || dtype == TNR_BFLOAT16 || dtype == TNR_FLOAT16;
+}
+size_t size_of(int32_t dtype) { return dtype == TNR_FLOAT32 ? 4 : 2; }
+size_t padded(size_t bytes) { return (bytes + 255) / 256 * 256; }
+
+template <typename F>
+void with_type(int32_t dtype, F&& f) {
+    if (dtype == TNR_FLOAT32)
+        f(float{});
+    else if (dtype == TNR_BFLOAT16)
+        f(bf16{});
+    else
+        f(f16{});
+}
+template <int N>
+struct Int {
+    static constexpr int value = N;
+};
+
+// A launch of more than 2^32 threads is not possible.
+constexpr int64_t kMostThreads = (int64_t(1) << 32) - 1;
+
+void zero(void* p, size_t bytes, hipStream_t stream) {
+    const int64_t words = (int64_t)(bytes / 4);
+    if (words == 0) return;
+    const int64_t blocks = (words + 1023) / 1024;
+    k_op_zero<<<(unsigned)(blocks < 1024 ? blocks : 1024), 256, 0, stream>>>((int32_t*)p, words);
+}
+
+// ------------------------------------------------------------------ embedding
+
+int check_embedding(const tnr_embedding* r, bool backward, char* err, size_t len) {
+    if (!r) return refuse(err, len, "request is null");
+    if (!is_type(r->dtype)) return refuse(err, len, "dtype must be float32, bfloat16 or float16");
+    if (r->index_bytes != 4 && r->index_bytes != 8)
+        return refuse(err, len, "species must be int32 or int64");
+    if (r->n_atoms < 0 || r->n_species < 0 || r->channels < 1 || r->n_atoms >= INT32_MAX ||
+        r->n_species >= INT32_MAX || r->channels > (1 << 20))
+        return refuse(err, len, "invalid sizes");
+    const bool rows = r->n_atoms > 0, table = r->n_species > 0;
+    if ((rows && (!r->species || !(backward ? r->grad_out : r->out))) ||
+        (table && !(backward ? r->grad_weight : r->weight)))
+        return refuse(err, len, "required pointers are null");
+    return TNR_OK;
+}
+
+// Channels that one thread takes: the most, up to 16 bytes, that divide a row
+// and keep every row's address a multiple of them.
+int vector_of(const tnr_embedding& r, const void* a, const void* b) {
+    const int64_t size = (int64_t)size_of(r.dtype);
+    for (int64_t n = 16 / size; n > 1; n /= 2)
+        if (r.channels % n == 0 && (uintptr_t)a % (n * size) == 0 && (uintptr_t)b % (n * size) == 0)
+            return (int)n;
+    return 1;
+}
+
+template <typename F>
+void with_vector(int vec, F&& f) {
+    if (vec == 8)
+        f(Int<8>{});
+    else if (vec == 4)
+        f(Int<4>{});
+    else if (vec == 2)
+        f(Int<2>{});
+    else
+        f(Int<1>{});
+}
+
+EmbeddingArgs embedding_args(const tnr_embedding& r) {
+    return {r.species, r.weight, r.grad_out, r.out,  r.grad_weight,
+            r.n_atoms, r.n_species, r.channels, r.scale};
+}
+
+// Sorted atoms of a group: enough groups for the device, and no more than 256
+// atoms, whose partial rows are few beside them.
+int64_t embedding_each(int64_t n) {
+    const int64_t e = n / 4096;
+    return e < 16 ? 16 : e > 256 ? 256 : e;
+}
+
+struct EmbeddingSpace {
+    int32_t *counts, *totals, *key[2], *atom[2];
+    int2* runs;
+    float* partial;
+    size_t bytes;
+};
+EmbeddingSpace embedding_space(const tnr_embedding& r, void* base) {
+    size_t at = 0;
+    const auto part = [&](size_t bytes) {
+        char* p = (char*)base + at;
+        at += padded(bytes);
+        return p;
+    };
+    const int64_t tiles = sort_tiles(r.n_atoms), each = embedding_each(r.n_atoms);
+    EmbeddingSpace s{};
+    s.counts = (int32_t*)part((size_t)kSortRadix * tiles * 4);
+    s.totals = (int32_t*)part((size_t)kSortRadix * 4);
+    for (int i = 0; i < 2; ++i) {
+        s.key[i] = (int32_t*)part((size_t)r.n_atoms * 4);
+        s.atom[i] = (int32_t*)part((size_t)r.n_atoms * 4);
+    }
+    s.runs = (int2*)part((size_t)r.n_species * 8);
+    s.partial = (float*)part((size_t)((r.n_atoms + each - 1) / each) * 2 * r.channels * 4);
+    s.bytes = at;
+    return s;
+}
+
+// A pass over `keys`, whose items `put` writes.
+template <typename Keys, typename Put>
+void sort_pass(Keys keys, int64_t n, SortPass pass, int32_t* counts, int32_t* totals, Put put,
+               hipStream_t stream) {
+    const unsigned tiles = (unsigned)sort_tiles(n);
+    const int radix = 1 << pass.bits;
+    k_sort_count<<<tiles, kSortThreads, 0, stream>>>(keys, n, pass, counts);
+    k_sort_scan<<<(radix + kSortWaves - 1) / kSortWaves, kSortThreads, 0, stream>>>(
+        counts, tiles, radix, totals);
+    k_sort_move<<<tiles, kSortThreads, 0, stream>>>(keys, n, pass, counts, totals, put);
+}
+
+template <typename I>
+void sort_species(const tnr_embedding& r, const EmbeddingSpace& s, RunArgs& runs,
+                  hipStream_t stream) {
+    const SortPlan plan = sort_plan(r.n_species + 1);
+    int from = 0;
+    for (int p = 0; p < plan.passes; ++p) {
+        if (p == 0)
+            sort_pass(SpeciesOf<I>{(const I*)r.species, r.n_species}, r.n_atoms, plan.pass[p],
+                      s.counts, s.totals, PutAtom{s.key[0], s.atom[0]}, stream);
+        else {
+            sort_pass(SortKeys{s.key[from]}, r.n_atoms, plan.pass[p], s.counts, s.totals,
+                      MoveAtom{s.atom[from], s.key[1 - from], s.atom[1 - from]}, stream);
+            from = 1 - from;
+        }
+    }
+    runs.key = s.key[from];
+    runs.atom = s.atom[from];
+}
+
+// ------------------------------------------------------------------ attention
+
+int check_heads(int32_t dtype, int32_t heads, int32_t kv_heads, int32_t dim, float scale,
+                float softcap, char* err, size_t len) {
+    if (!is_type(dtype)) return refuse(err, len, "dtype must be float32, bfloat16 or float16");
+    if (heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || heads > 1024)
+        return refuse(err, len, "heads must be a multiple of the key and value heads, at most 1024");
+    if (dim < 8 || dim > 128 || dim % 8 != 0)
+        return refuse(err, len, "the head dimension must be a multiple of 8, from 8 to 128");
+    if (!std::isfinite(scale)) return refuse(err, len, "scale must be finite");
+    if (!std::isfinite(softcap) || softcap < 0.f)
+        return refuse(err, len, "softcap must be finite and positive");
+    return TNR_OK;
+}
+
+bool aligned(const void* p, const int64_t (&stride)[2], int32_t dtype) {
+    const int64_t unit = 16 / (int64_t)size_of(dtype);
+    return (uintptr_t)p % 16 == 0 && stride[0] % unit == 0 && stride[1] % unit == 0;
+}
+
+// ------------------------------------------------------- structure attention
+
+// Waves of 32 rows in a workgroup: as many as the batch's structures fill.
+// They share the staged keys; a wave without rows only helps to stage.
+int waves_for(int64_t rows, int64_t structures) {
+    const int64_t mean = structures > 0 ? rows / structures : 0;
+    return mean <= 32 ? 1 : mean <= 64 ? 2 : 4;
+}
+
+struct StructurePlan {
+    int group, q_waves, k_waves, splits;
+    int64_t q_tiles, k_tiles;
+};
+
+StructurePlan structure_plan(const tnr_structure_attention& r) {
+    StructurePlan p{};
+    p.group = r.heads / r.kv_heads;
+    p.q_waves = waves_for(r.n_queries * p.group, r.n_structures);
+    p.k_waves = waves_for(r.n_keys, r.n_structures);
+    p.q_tiles = tile_start(r.n_queries, p.group, p.q_waves * kTile, r.n_structures);
+    p.k_tiles = tile_start(r.n_keys, 1, p.k_waves * kTile, r.n_structures);
+    // Few rows: keys are split over workgroups, at least 8 tiles each, until
+    // there are waves enough for the device.
+    const int64_t waves = (r.n_queries * p.group / kTile + r.n_structures) * r.kv_heads;
+    const int64_t mean = r.n_structures > 0 ? r.n_keys / r.n_structures / (8 * kTile) : 0;
+    int64_t splits = waves > 0 ? 2048 / waves : 1;
+    if (splits > mean) splits = mean;
+    if (splits > 64) splits = 64;
+    p.splits = splits < 2 ? 1 : (int)splits;
+    return p;
+}
+
+int check_structure(const tnr_structure_attention* r, bool backward, char* err, size_t len) {
+    if (!r) return refuse(err, len, "request is null");
+    const int code = check_heads(r->dtype, r->heads, r->kv_heads, r->dim, r->scale, r->softcap, err,
+                                 len);
+    if (code != TNR_OK) return code;
+    if (r->n_structures < 0 || r->n_queries < 0 || r->n_keys < 0 ||
+        (r->n_structures == 0 && (r->n_queries > 0 || r->n_keys > 0)))
+        return refuse(err, len, "invalid sizes");
+    if (r->n_queries >= INT32_MAX / r->heads || r->n_keys >= INT32_MAX / r->kv_heads ||
+        r->n_structures >= INT32_MAX)
+        return refuse(err, len, "too many atoms");
+    const StructurePlan p = structure_plan(*r);
+    if (p.q_tiles * p.q_waves * kWave > kMostThreads || p.k_tiles * p.k_waves * kWave > kMostThreads ||
+        (int64_t)r->kv_heads * p.splits > 65535)
+        return refuse(err, len, "too many atoms");
+    if (r->n_structures > 0 && (!r->query_ptr || !r->key_ptr))
+        return refuse(err, len, "required pointers are null");
+    if (!r->slopes || (r->n_queries > 0 && (!r->q || !r->query_positions || !r->out)) ||
+        (r->n_keys > 0 && (!r->k || !r->v || !r->positions)))
+        return refuse(err, len, "required pointers are null");
+    if (!aligned(r->q, r->q_stride, r->dtype) || !aligned(r->k, r->k_stride, r->dtype) ||
+        !aligned(r->v, r->v_stride, r->dtype) || (uintptr_t)r->out % 16 != 0)
+        return refuse(err, len, "q, k, v and out must be aligned to 16 bytes");
+    if (backward) {
+        if ((r->n_queries > 0 && (!r->grad_out || !r->grad_q || !r->lse)) ||
+            (r->n_keys > 0 && (!r->grad_k || !r->grad_v)))
+            return refuse(err, len, "required pointers are null");
+        if ((uintptr_t)r->grad_out % 16 != 0 || (uintptr_t)r->grad_q % 16 != 0 ||
+            (uintptr_t)r->grad_k % 16 != 0 || (uintptr_t)r->grad_v % 16 != 0)
+            return refuse(err, len, "gradients must be aligned to 16 bytes");
+    }
+    return TNR_OK;
+}
+
+StructureArgs structure_args(const tnr_structure_attention& r, const StructurePlan& p) {
+    StructureArgs a{};
+    a.q = r.q;
+    a.k = r.k;
+    a.v = r.v;
+    for (int i = 0; i < 2; ++i) {
+        a.q_stride[i] = r.q_stride[i];
+        a.k_stride[i] = r.k_stride[i];
+        a.v_stride[i] = r.v_stride[i];
+    }
+    a.x_q = r.query_positions;
+    a.x_k = r.positions;
+    a.slopes = r.slopes;
+    a.rule = ScoreRule::of(r.scale, r.softcap);
+    a.heads = r.heads;
+    a.kv_heads = r.kv_heads;
+    a.group = p.group;
+    a.dim = r.dim;
+    a.n_queries = (int)r.n_queries;
+    a.n_keys = (int)r.n_keys;
+    a.splits = p.splits;
+    a.out = r.out;
+    a.lse = r.lse;
+    a.grad_out = r.grad_out;
+    a.grad_q = r.grad_q;
+    a.grad_k = r.grad_k;
+    a.grad_v = r.grad_v;
+    return a;
+}
+
+// Where the batch has no tile table of its own size, the pointers into it.
+struct StructureSpace {
+    StructureTile *q_tiles, *k_tiles;
+    float *part, *row, *push_q, *push_k, *turn;
+    size_t bytes;
+};
+StructureSpace structure_space(const tnr_structure_attention& r, const StructurePlan& p,
+                               bool backward, void* base) {
+    size_t at = 0;
+    const auto part = [&](size_t bytes) {
+        char* q = (char*)base + at;
+        at += padded(bytes);
+        return q;
+    };
+    const size_t rows = (size_t)r.heads * r.n_queries;
+    StructureSpace s{};
+    s.q_tiles = (StructureTile*)part((size_t)p.q_tiles * sizeof(StructureTile));
+    if (p.splits > 1)
+        s.part = (float*)part(rows * p.splits * (r.dim + (backward ? kRowSums : 2)) * 4);
+    if (backward) {
+        s.k_tiles = (StructureTile*)part((size_t)p.k_tiles * sizeof(StructureTile));
+        s.row = (float*)part(rows * 8);
+        if (r.grad_positions || r.grad_query_positions) {
+            s.push_q = (float*)part(rows * 12);
+            s.push_k = (float*)part((size_t)r.kv_heads * r.n_keys * 12);
+        }
+        if (r.grad_slopes) s.turn = (float*)part(rows * 4);
+    }
+    s.bytes = at;
+    return s;
+}
+
+void lay_tiles(const tnr_structure_attention& r, const StructurePlan& p, const StructureSpace& s,
+               hipStream_t stream) {
+    const int64_t blocks = (r.n_structures + 3) / 4;
+    k_structure_tiles<<<(unsigned)(blocks < 64 ? blocks : 64), 256, 0, stream>>>(
+        r.query_ptr, r.key_ptr, r.n_structures, r.n_queries, r.n_keys, p.group, p.q_waves * kTile,
+        p.k_waves * kTile, s.q_tiles, s.k_tiles);
+}
+
+template <typename F>
+void with_dim(int32_t dim, F&& f) {
+    if (dim <= 32)
+        f(Int<32>{});
+    else if (dim <= 64)
+        f(Int<64>{});
+    else if (dim <= 96)
+        f(Int<96>{});
+    else
+        f(Int<128>{});
+}
+template <typename F>
+void with_waves(int waves, F&& f) {
+    if (waves == 1)
+        f(Int<1>{});
+    else if (waves == 2)
+        f(Int<2>{});
+    else
+        f(Int<4>{});
+}
+
+// -------------------------------------------------------- neighbor attention
+
+constexpr int64_t kMostAtoms = int64_t(1) << 26;  // a wave each
+
+int check_list(const tnr_neighbor_list* l, char* err, size_t len) {
+    if (!l) return refuse(err, len, "list is null");
+    if (l->n_pairs < 0 || l->n_sources < 0 || l->n_targets < 0)
+        return refuse(err, len, "invalid sizes");
+    if (l->n_pairs >= INT32_MAX || l->n_sources >= kMostAtoms || l->n_targets >= kMostAtoms)
+        return refuse(err, len, "too many pairs or atoms");
+    if (l->n_pairs > 0 && (l->n_sources == 0 || l->n_targets == 0))
+        return refuse(err, len, "a list with pairs needs sources and targets");
+    if (!l->rows || (uintptr_t)l->rows % 256 != 0)
+        return refuse(err, len, "rows must be given and aligned to 256 bytes");
+    return TNR_OK;
+}
+
+struct RowsSpace {
+    int32_t *counts, *totals, *key[2];
+    int2* order;
+    size_t bytes;
+};
+RowsSpace rows_space(const tnr_neighbor_list& l, void* base) {
+    size_t at = 0;
+    const auto part = [&](size_t bytes) {
+        char* q = (char*)base + at;
+        at += padded(bytes);
+        return q;
+    };
+    RowsSpace s{};
+    if (!l.transpose || l.n_pairs == 0) return s;
+    s.counts = (int32_t*)part((size_t)kSortRadix * sort_tiles(l.n_pairs) * 4);
+    s.totals = (int32_t*)part((size_t)kSortRadix * 4);
+    s.key[0] = (int32_t*)part((size_t)l.n_pairs * 4);
+    if (sort_plan(l.n_targets).passes > 1) {
+        s.key[1] = (int32_t*)part((size_t)l.n_pairs * 4);
+        s.order = (int2*)part((size_t)l.n_pairs * 8);
+    }
+    s.bytes = at;
+    return s;
+}
+
+NeighborRows rows_of(const tnr_neighbor_list& l) {
+    return neighbor_rows(l.rows, l.n_pairs, l.n_sources, l.n_targets, l.transpose != 0);
+}
+
+int check_neighbor(const tnr_neighbor_attention* r, bool backward, char* err, size_t len) {
+    if (!r) return refuse(err, len, "request is null");
+    int code = check_heads(r->dtype, r->heads, r->kv_heads, r->dim, r->scale, r->softcap, err, len);
+    if (code == TNR_OK) code = check_list(&r->list, err, len);
+    if (code != TNR_OK) return code;
+    if (r->list.n_sources >= INT32_MAX / r->heads || r->list.n_targets >= INT32_MAX / r->kv_heads)
+        return refuse(err, len, "too many pairs or atoms");
+    if (!r->slopes || (r->list.n_sources > 0 && (!r->q || !r->out)) ||
+        (r->list.n_targets > 0 && (!r->k || !r->v)) || (r->list.n_pairs > 0 && !r->distances))
+        return refuse(err, len, "required pointers are null");
+    if (!aligned(r->q, r->q_stride, r->dtype) || !aligned(r->k, r->k_stride, r->dtype) ||
+        !aligned(r->v, r->v_stride, r->dtype) || (uintptr_t)r->out % 16 != 0)
+        return refuse(err, len, "q, k, v and out must be aligned to 16 bytes");
+    if (backward) {
+        if (!r->list.transpose) return refuse(err, len, "the backward needs the rows by target too");
+        if ((r->list.n_sources > 0 && (!r->grad_out || !r->grad_q || !r->lse ||
+                                       (r->dtype != TNR_FLOAT32 && !r->out32))) ||
+            (r->list.n_targets > 0 && (!r->grad_k || !r->grad_v)) || !r->grad_slopes ||
+            (r->list.n_pairs > 0 && !r->grad_distances))
+            return refuse(err, len, "required pointers are null");
+        if ((uintptr_t)r->grad_out % 16 != 0 || (uintptr_t)r->grad_q % 16 != 0 ||
+            (uintptr_t)r->grad_k % 16 != 0 || (uintptr_t)r->grad_v % 16 != 0)
+            return refuse(err, len, "gradients must be aligned to 16 bytes");
+    }
+    return TNR_OK;
+}
+
+NeighborArgs neighbor_args(const tnr_neighbor_attention& r) {
+    NeighborArgs a{};
+    a.rows = rows_of(r.list);
+    a.n_pairs = (int)r.list.n_pairs;
+    a.n_sources = (int)r.list.n_sources;
+    a.n_targets = (int)r.list.n_targets;
+    a.q = r.q;
+    a.k = r.k;
+    a.v = r.v;
+    for (int i = 0; i < 2; ++i) {
+        a.q_stride[i] = r.q_stride[i];
+        a.k_stride[i] = r.k_stride[i];
+        a.v_stride[i] = r.v_stride[i];
+    }
+    a.distances = r.distances;
+    a.slopes = r.slopes;
+    a.rule = ScoreRule::of(r.scale, r.softcap);
+    a.heads = r.heads;
+    a.kv_heads = r.kv_heads;
+    a.group = r.heads / r.kv_heads;
+    a.dim = r.dim;
+    a.out = r.out;
+    a.out32 = r.out32;
+    a.lse = r.lse;
+    a.grad_out = r.grad_out;
+    a.out_full = r.dtype == TNR_FLOAT32 ? (const float*)r.out : r.out32;
+    a.grad_q = r.grad_q;
+    a.grad_k = r.grad_k;
+    a.grad_v = r.grad_v;
+    a.grad_distances = r.grad_distances;
+    return a;
+}
+
+// Lanes of 16 bytes that make a head: a power of two.
+template <typename F>
+void with_lanes(int32_t dtype, int32_t dim, F&& f) {
+    const int units = (int)(dim * size_of(dtype) / 16);
+    if (units <= 1)
+        f(Int<1>{});
+    else if (units <= 2)
+        f(Int<2>{});
+    else if (units <= 4)
+        f(Int<4>{});
+    else if (units <= 8)
+        f(Int<8>{});
+    else if (units <= 16)
+        f(Int<16>{});
+    else
+        f(Int<32>{});
+}
+
+// Lanes of a slot: the heads' lanes, a power of two, at most a wave.
+int slot_of(int lanes, int heads) {
+    int slot = lanes;
+    while (slot < kWave && slot < lanes * heads) slot *= 2;
+    return slot;
+}
+
+}  // namespace
+
+extern "C" {
+
+int tnr_operators_version(void) { return TNR_OPERATORS_VERSION; }
+
+int tnr_embedding_forward(const tnr_embedding* req, void* stream, char* err, size_t err_len) {
+    const int code = check_embedding(req, false, err, err_len);
+    if (code != TNR_OK) return code;
+    const tnr_embedding& r = *req;
+    if (r.n_atoms == 0) return TNR_OK;
+    const EmbeddingArgs a = embedding_args(r);
+    with_type(r.dtype, [&](auto t) {
+        using T = decltype(t);
+        with_vector(vector_of(r, r.weight, r.out), [&](auto v) {
+            constexpr int VEC = decltype(v)::value;
+            if constexpr (VEC * sizeof(T) <= 16) {
+                const int64_t blocks = (r.n_atoms * (r.channels / VEC) + 255) / 256;
+                const unsigned grid = (unsigned)(blocks < 16384 ? blocks : 16384);
+                if (r.index_bytes == 4)
+                    k_embedding_forward<T, int32_t, VEC><<<grid, 256, 0, (hipStream_t)stream>>>(a);
+                else
+                    k_embedding_forward<T, int64_t, VEC><<<grid, 256, 0, (hipStream_t)stream>>>(a);
+            }
+        });
+    });
+    return launched(err, err_len);
+}
+
+size_t tnr_embedding_workspace_size(const tnr_embedding* req) {
+    if (!req || req->n_atoms < 0 || req->n_species < 0 || req->channels < 1) return 0;
+    return embedding_space(*req, nullptr).bytes;
+}
+
+int tnr_embedding_backward(const tnr_embedding* req, void* workspace, size_t workspace_bytes,
+                           void* stream, char* err, size_t err_len) {
+    const int code = check_embedding(req, true, err, err_len);
+    if (code != TNR_OK) return code;
+    const tnr_embedding& r = *req;
+    if (r.n_species == 0) return TNR_OK;
+    const EmbeddingSpace s = embedding_space(r, workspace);
+    if (!workspace || (uintptr_t)workspace % 256 != 0 || workspace_bytes < s.bytes)
+        return refuse(err, err_len, "workspace is too small or not aligned to 256 bytes");
+    const hipStream_t st = (hipStream_t)stream;
+    const EmbeddingArgs a = embedding_args(r);
+    RunArgs runs{};
+    runs.runs = s.runs;
+    runs.partial = s.partial;
+    runs.each = embedding_each(r.n_atoms);
+    zero(s.runs, (size_t)r.n_species * 8, st);
+    if (r.n_atoms > 0) {
+        if (r.index_bytes == 4)
+            sort_species<int32_t>(r, s, runs, st);
+        else
+            sort_species<int64_t>(r, s, runs, st);
+    }
+    with_type(r.dtype, [&](auto t) {
+        using T = decltype(t);
+        with_vector(vector_of(r, r.grad_out, r.grad_weight), [&](auto v) {
+            constexpr int VEC = decltype(v)::value;
+            if constexpr (VEC * sizeof(T) <= 16) {
+                int lanes = 1;
+                while (lanes < 64 && lanes * VEC < r.channels) lanes *= 2;
+                const unsigned y = (unsigned)((r.channels + lanes * VEC - 1) / (lanes * VEC));
+                const int64_t groups = (r.n_atoms + runs.each - 1) / runs.each;
+                const int64_t in_block = 256 / lanes;
+                if (groups > 0)
+                    k_embedding_runs<T, VEC>
+                        <<<dim3((unsigned)((groups + in_block - 1) / in_block), y), 256, 0, st>>>(
+                            a, runs, lanes);
+                k_embedding_join<T, VEC>
+                    <<<dim3((unsigned)r.n_species, y), 256, 0, st>>>(a, runs, lanes);
+            }
+        });
+    });
+    return launched(err, err_len);
+}
+
+size_t tnr_structure_forward_workspace_size(const tnr_structure_attention* req) {
+    if (check_structure(req, false, nullptr, 0) != TNR_OK) return 0;
+    return structure_space(*req, structure_plan(*req), false, nullptr).bytes;
+}
+
+int tnr_structure_forward(const tnr_structure_attention* req, void* workspace,
+                          size_t workspace_bytes, void* stream, char* err, size_t err_len) {
+    const int code = check_structure(req, false, err, err_len);
+    if (code != TNR_OK) return code;
+    const tnr_structure_attention& r = *req;
+    if (r.n_queries == 0) return TNR_OK;
+    const StructurePlan p = structure_plan(r);
+    const StructureSpace s = structure_space(r, p, false, workspace);
+    if (!workspace || (uintptr_t)workspace % 256 != 0 || workspace_bytes < s.bytes)
+        return refuse(err, err_len, "workspace is too small or not aligned to 256 bytes");
+    const hipStream_t st = (hipStream_t)stream;
+    StructureArgs a = structure_args(r, p);
+    a.q_tiles = s.q_tiles;
+    a.part = s.part;
+    lay_tiles(r, p, s, st);
+    with_type(r.dtype, [&](auto t) {
+        using T = decltype(t);
+        with_dim(r.dim, [&](auto d) {
+            constexpr int DP = decltype(d)::value;
+            with_waves(p.q_waves, [&](auto w) {
+                constexpr int NW = decltype(w)::value;
+                k_structure_forward<T, DP, NW>
+                    <<<dim3((unsigned)p.q_tiles, r.kv_heads * p.splits), NW * kWave, 0, st>>>(a);
+            });
+        });
+        if (p.splits > 1)
+            k_structure_join<T>
+                <<<(unsigned)((r.n_queries * r.heads + 3) / 4), 256, 0, st>>>(a);
+    });
+    return launched(err, err_len);
+}
+
+size_t tnr_structure_backward_workspace_size(const tnr_structure_attention* req) {
+    if (check_structure(req, false, nullptr, 0) != TNR_OK) return 0;
+    return structure_space(*req, structure_plan(*req), true, nullptr).bytes;
+}
+
+int tnr_structure_backward(const tnr_structure_attention* req, void* workspace,
+                           size_t workspace_bytes, void* stream, char* err, size_t err_len) {
+    const int code = check_structure(req, true, err, err_len);
+    if (code != TNR_OK) return code;
+    const tnr_structure_attention& r = *req;
+    const StructurePlan p = structure_plan(r);
+    const StructureSpace s = structure_space(r, p, true, workspace);
+    if (!workspace || (uintptr_t)workspace % 256 != 0 || workspace_bytes < s.bytes)
+        return refuse(err, err_len, "workspace is too small or not aligned to 256 bytes");
+    const hipStream_t st = (hipStream_t)stream;
+    StructureArgs a = structure_args(r, p);
+    a.q_tiles = s.q_tiles;
+    a.k_tiles = s.k_tiles;
+    a.part = s.part;
+    a.row = s.row;
+    a.push_q = s.push_q;
+    a.push_k = s.push_k;
+    a.turn = s.turn;
+    if (r.n_structures > 0) lay_tiles(r, p, s, st);
+    with_type(r.dtype, [&](auto t) {
+        using T = decltype(t);
+        with_dim(r.dim, [&](auto d) {
+            constexpr int DP = decltype(d)::value;
+            if (r.n_queries > 0)
+                with_waves(p.q_waves, [&](auto w) {
+                    constexpr int NW = decltype(w)::value;
+                    k_structure_dq<T, DP, NW>
+                        <<<dim3((unsigned)p.q_tiles, r.kv_heads * p.splits), NW * kWave, 0, st>>>(
+                            a);
+                });
+            if (r.n_queries > 0 && p.splits > 1)
+                k_structure_join_dq<T>
+                    <<<(unsigned)((r.n_queries * r.heads + 3) / 4), 256, 0, st>>>(a);
+            if (r.n_keys > 0)
+                with_waves(p.k_waves, [&](auto w) {
+                    constexpr int NW = decltype(w)::value;
+                    k_structure_dkv<T, DP, NW>
+                        <<<dim3((unsigned)p.k_tiles, r.kv_heads), NW * kWave, 0, st>>>(a);
+                });
+        });
+    });
+    const int shared = r.grad_positions && !r.grad_query_positions &&
+                       r.query_positions == r.positions && r.n_queries == r.n_keys;
+    int64_t items = (r.grad_positions ? 3 * r.n_keys : 0) +
+                    (r.grad_query_positions ? 3 * r.n_queries : 0);
+    const int64_t blocks = (items + 255) / 256 + (r.grad_slopes ? r.heads : 0);
+    if (blocks > 0)
+        k_structure_finish<<<(unsigned)blocks, 256, 0, st>>>(a, r.grad_query_positions,
+                                                             r.grad_positions, r.grad_slopes, shared);
+    return launched(err, err_len);
+}
+
+size_t tnr_neighbor_rows_size(const tnr_neighbor_list* list) {
+    if (!list || list->n_pairs < 0 || list->n_sources < 0 || list->n_targets < 0) return 0;
+    return neighbor_rows(nullptr, list->n_pairs, list->n_sources, list->n_targets,
+                         list->transpose != 0)
+        .bytes;
+}
+
+size_t tnr_neighbor_rows_workspace_size(const tnr_neighbor_list* list) {
+    if (!list || list->n_pairs < 0 || list->n_sources < 0 || list->n_targets < 0) return 0;
+    return rows_space(*list, nullptr).bytes;
+}
+
+int tnr_neighbor_rows(const tnr_neighbor_list* list, void* workspace, size_t workspace_bytes,
+                      void* stream, char* err, size_t err_len) {
+    const int code = check_list(list, err, err_len);
+    if (code != TNR_OK) return code;
+    const tnr_neighbor_list& l = *list;
+    if (l.n_pairs > 0 && (!l.sources || !l.targets))
+        return refuse(err, err_len, "required pointers are null");
+    const RowsSpace s = rows_space(l, workspace);
+    if (s.bytes > 0 && (!workspace || (uintptr_t)workspace % 256 != 0 || workspace_bytes < s.bytes))
+        return refuse(err, err_len, "workspace is too small or not aligned to 256 bytes");
+    const hipStream_t st = (hipStream_t)stream;
+    const NeighborRows rows = rows_of(l);
+    // status and the runs, which lie at the front
+    zero(rows.status, (char*)rows.target - (char*)rows.status, st);
+    if (l.n_pairs > 0) {
+        const int64_t blocks = (l.n_pairs + 1023) / 1024;
+        k_neighbor_rows<<<(unsigned)(blocks < 8192 ? blocks : 8192), 256, 0, st>>>(
+            l.sources, l.targets, l.n_pairs, l.n_sources, l.n_targets, rows);
+        if (l.transpose) {
+            const SortPlan plan = sort_plan(l.n_targets);
+            const int32_t* key = nullptr;
+            for (int p = 0; p < plan.passes; ++p) {
+                // the last pass writes the rows' own order
+                const bool own = (plan.passes - 1 - p) % 2 == 0;
+                int32_t* to = s.key[own ? 0 : 1];
+                int2* order = own ? rows.order : s.order;
+                if (p == 0)
+                    sort_pass(PairKeys{rows.target}, l.n_pairs, plan.pass[p], s.counts, s.totals,
+                              PutPair{l.sources, to, order}, st);
+                else
+                    sort_pass(SortKeys{key}, l.n_pairs, plan.pass[p], s.counts, s.totals,
+                              MovePair{own ? s.order : rows.order, to, order}, st);
+                key = to;
+            }
+            k_neighbor_targets<<<(unsigned)((l.n_pairs + 255) / 256), 256, 0, st>>>(
+                key, l.n_pairs, rows.targets);
+        }
+    }
+    return launched(err, err_len);
+}
+
+int tnr_neighbor_forward(const tnr_neighbor_attention* req, void* stream, char* err,
+                         size_t err_len) {
+    const int code = check_neighbor(req, false, err, err_len);
+    if (code != TNR_OK) return code;
+    const tnr_neighbor_attention& r = *req;
+    if (r.list.n_sources == 0) return TNR_OK;
+    NeighborArgs a = neighbor_args(r);
+    with_type(r.dtype, [&](auto t) {
+        using T = decltype(t);
+        with_lanes(r.dtype, r.dim, [&](auto l) {
+            constexpr int LPH = decltype(l)::value;
+            a.slot = slot_of(LPH, r.heads);
+            const int block = a.slot / LPH;
+            k_neighbor_forward<T, LPH>
+                <<<dim3((unsigned)((r.list.n_sources + 3) / 4), (r.heads + block - 1) / block), 256,
+                   0, (hipStream_t)stream>>>(a);
+        });
+    });
+    return launched(err, err_len);
+}
+
+size_t tnr_neighbor_backward_workspace_size(const tnr_neighbor_attention* req) {
+    if (!req || req->heads < 1 || req->list.n_sources < 0) return 0;
+    return 2 * padded((size_t)req->list.n_sources * req->heads * 4);
+}
+
+int tnr_neighbor_backward(const tnr_neighbor_attention* req, void* workspace,
+                          size_t workspace_bytes, void* stream, char* err, size_t err_len) {
+    const int code = check_neighbor(req, true, err, err_len);
+    if (code != TNR_OK) return code;
+    const tnr_neighbor_attention& r = *req;
+    const size_t need = tnr_neighbor_backward_workspace_size(req);
+    if (need > 0 && (!workspace || (uintptr_t)workspace % 256 != 0 || workspace_bytes < need))
+        return refuse(err, err_len, "workspace is too small or not aligned to 256 bytes");
+    const hipStream_t st = (hipStream_t)stream;
+    NeighborArgs a = neighbor_args(r);
+    a.delta = (float*)workspace;
+    a.turn = (float*)((char*)workspace + need / 2);
+    with_type(r.dtype, [&](auto t) {
+        using T = decltype(t);
+        with_lanes(r.dtype, r.dim, [&](auto l) {
+            constexpr int LPH = decltype(l)::value;
+            a.slot = slot_of(LPH, r.heads);
+            if (r.list.n_sources > 0)
+                k_neighbor_dq<T, LPH>
+                    <<<(unsigned)((r.list.n_sources + 3) / 4), 256, 0, st>>>(a);
+            a.slot = slot_of(LPH, r.kv_heads);
+            const int block = a.slot / LPH;
+            if (r.list.n_targets > 0)
+                k_neighbor_dkv<T, LPH><<<dim3((unsigned)((r.list.n_targets + 3) / 4),
+                                              (r.kv_heads + block - 1) / block),
+                                         256, 0, st>>>(a);
+        });
+    });
+    k_neighbor_slopes<<<r.heads, 256, 0, st>>>(a.turn, r.list.n_sources, r.grad_slopes);
+    return launched(err, err_len);
+}
+
+}  // extern "C"

@@ -355,6 +355,8 @@ Answer search(const std::string& quantities, const Tensor& positions, const Tens
 
 }  // namespace
 
+void bind_operators(pybind11::module& m);  // operators.cpp
+
 // Both run without the GIL, as torch's own functions do: an allocation that
 // waits for the device, a full launch queue or the wait for the count leaves
 // the other Python threads running.  (Saved-tensor hooks take it themselves.)
@@ -384,4 +386,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
                                     runs);
               END_HANDLE_TH_ERRORS_PYBIND
           });
+    bind_operators(m);
 }
