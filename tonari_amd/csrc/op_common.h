@@ -9,6 +9,7 @@
 
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 
 namespace tnr {
 namespace op {
@@ -46,6 +47,34 @@ __device__ __forceinline__ float sum_halves(float x) {
 __device__ __forceinline__ float max_halves(float x) {
     const Halves h = halves_of(x);
     return fmaxf(h.low, h.high);
+}
+
+template <int CTRL>
+__device__ __forceinline__ float dpp_of(float x) {
+    return __int_as_float(
+        __builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, false));
+}
+__device__ __forceinline__ float sum_of(float a, float b) { return a + b; }
+__device__ __forceinline__ float max_of(float a, float b) { return fmaxf(a, b); }
+
+// f over the lanes whose numbers differ in the bits from `from` (a power of two)
+// up, in all of them: rotations within 16 lanes, then swaps of rows.
+template <float (*F)(float, float)>
+__device__ __forceinline__ float join_lanes(float x, int from) {
+    if (from <= 1) x = F(x, dpp_of<0xb1>(x));
+    if (from <= 2) x = F(x, dpp_of<0x4e>(x));
+    if (from <= 4) x = F(x, dpp_of<0x124>(x));
+    if (from <= 8) x = F(x, dpp_of<0x128>(x));
+    if (from <= 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x),
+                                                        false, false);
+        x = F(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    }
+    if (from <= 32) {
+        const Halves h = halves_of(x);
+        x = F(h.low, h.high);
+    }
+    return x;
 }
 
 // ------------------------------------------------------------------ scores
@@ -99,6 +128,33 @@ __device__ __forceinline__ void store_floats(T* p, const float (&x)[N]) {
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = rounded<T>(x[i]);
     *(Vec<T, N>*)p = v;
+}
+
+// Sum of n floats by a workgroup of 1,024, in its first thread.
+__device__ __forceinline__ float block_sum(const float* x, int64_t n) {
+    __shared__ float waves[16];
+    float part[8] = {};
+    int64_t i = threadIdx.x;
+    for (; i + 7 * 1024 < n; i += 8 * 1024)
+#pragma unroll
+        for (int u = 0; u < 8; ++u) part[u] += x[i + u * 1024];
+    for (; i < n; i += 1024) part[0] += x[i];
+    float sum = join_lanes<sum_of>(((part[0] + part[1]) + (part[2] + part[3])) +
+                                       ((part[4] + part[5]) + (part[6] + part[7])),
+                                   1);
+    if (lane_of() == 0) waves[threadIdx.x / kWave] = sum;
+    __syncthreads();
+    sum = 0.f;
+    if (threadIdx.x == 0)
+        for (int w = 0; w < 16; ++w) sum += waves[w];
+    return sum;
+}
+
+// A head's slope: the sum of its rows, one workgroup each.
+__global__ __launch_bounds__(1024) inline void k_slopes(const float* turn, int64_t rows,
+                                                        float* grad_slopes) {
+    const float sum = block_sum(turn + (int64_t)blockIdx.x * rows, rows);
+    if (threadIdx.x == 0) grad_slopes[blockIdx.x] = sum;
 }
 
 }  // namespace op

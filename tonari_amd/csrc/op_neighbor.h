@@ -126,22 +126,45 @@ struct NeighborArgs {
     float* turn;   // [heads][n_sources]
 };
 
+// 16 bytes of a row, as they are loaded: products of 16-bit values go two at a
+// time into a 32-bit sum.
 template <typename T>
-constexpr int kVec = 16 / sizeof(T);
-
-template <int CTRL>
-__device__ __forceinline__ float dpp_of(float x) {
-    return __int_as_float(
-        __builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, false));
-}
+struct Raw {
+    static constexpr int kVec = 16 / sizeof(T);
+    Vec<T, kVec> x;
+    __device__ __forceinline__ static Raw at(const char* p) {
+        return {*(const Vec<T, kVec>*)p};
+    }
+    __device__ __forceinline__ float dot(const Raw& o, float sum) const {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) sum = fmaf(x[i], o.x[i], sum);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kVec; i += 2) {
+                const Vec<T, 2> a = {x[i], x[i + 1]}, b = {o.x[i], o.x[i + 1]};
+                if constexpr (std::is_same_v<T, bf16>)
+                    sum = __builtin_amdgcn_fdot2_f32_bf16(a, b, sum, false);
+                else
+                    sum = __builtin_amdgcn_fdot2(a, b, sum, false);
+            }
+        }
+        return sum;
+    }
+    // acc += p x
+    __device__ __forceinline__ void add(float p, float (&acc)[kVec]) const {
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) acc[i] = fmaf(p, (float)x[i], acc[i]);
+    }
+};
 
 // Sum over the LPH lanes of a head, in all of them.
 template <int LPH>
 __device__ __forceinline__ float head_sum(float x) {
-    if constexpr (LPH >= 2) x += dpp_of<0xb1>(x);   // lane ^ 1
-    if constexpr (LPH >= 4) x += dpp_of<0x4e>(x);   // lane ^ 2
-    if constexpr (LPH >= 8) x += dpp_of<0x141>(x);  // mirrored in 8
-    if constexpr (LPH >= 16) x += dpp_of<0x140>(x); // mirrored in 16
+    if constexpr (LPH >= 2) x += dpp_of<0xb1>(x);    // lane ^ 1
+    if constexpr (LPH >= 4) x += dpp_of<0x4e>(x);    // lane ^ 2
+    if constexpr (LPH >= 8) x += dpp_of<0x141>(x);   // mirrored in 8
+    if constexpr (LPH >= 16) x += dpp_of<0x140>(x);  // mirrored in 16
     if constexpr (LPH >= 32) x += __shfl_xor(x, 16);
     return x;
 }
@@ -161,90 +184,6 @@ __device__ __forceinline__ void fill_nan(T* p, int64_t n, int64_t from, int64_t 
     for (int64_t i = from; i < n; i += step) p[i] = rounded<T>(nan_of());
 }
 
-// grid: (sources / 4, head blocks).
-template <typename T, int LPH>
-__global__ __launch_bounds__(256) void k_neighbor_forward(const NeighborArgs a) {
-    constexpr int VEC = kVec<T>, kAhead = 4;
-    const int64_t i = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
-    if (i >= a.n_sources) return;
-    const int lane = lane_of(), slot = lane / a.slot, in_slot = lane % a.slot;
-    const int head = blockIdx.y * (a.slot / LPH) + in_slot / LPH;
-    const int c = (in_slot % LPH) * VEC;
-    const bool mine = head < a.heads && c < a.dim;
-    const int slots = kWave / a.slot;
-    T* out = (T*)a.out + (i * a.heads + head) * a.dim + c;
-    const int64_t row = i * a.heads + head;
-    float acc[VEC];
-#pragma unroll
-    for (int x = 0; x < VEC; ++x) acc[x] = 0.f;
-    float top = -inf_of(), sum = 0.f;
-    const bool valid = *a.rows.status == 0;
-    if (valid) {
-        float q[VEC] = {};
-        if (mine)
-            load_floats<T, VEC>((const T*)a.q + i * a.q_stride[0] + head * a.q_stride[1] + c, q);
-        const float slope2 = mine ? a.slopes[head] * kLog2e : 0.f;
-        const int kv = mine ? head / a.group : 0;
-        const T* k = (const T*)a.k + kv * a.k_stride[1] + (mine ? c : 0);
-        const T* v = (const T*)a.v + kv * a.v_stride[1] + (mine ? c : 0);
-        const int2 run = run_of(a.rows.sources, i);
-        for (int e0 = run.x; e0 < run.y; e0 += slots * kAhead) {
-            float kx[kAhead][VEC], vx[kAhead][VEC], d[kAhead], s[kAhead];
-#pragma unroll
-            for (int u = 0; u < kAhead; ++u) {
-                const int e = min(e0 + u * slots + slot, run.y - 1);
-                const int64_t j = a.rows.target[e];
-                d[u] = a.distances[e];
-                load_floats<T, VEC>(k + j * a.k_stride[0], kx[u]);
-                load_floats<T, VEC>(v + j * a.v_stride[0], vx[u]);
-            }
-            float high = top;
-#pragma unroll
-            for (int u = 0; u < kAhead; ++u) {
-                float dot = 0.f, t;
-#pragma unroll
-                for (int x = 0; x < VEC; ++x) dot = fmaf(q[x], kx[u][x], dot);
-                dot = head_sum<LPH>(mine ? dot : 0.f);
-                s[u] = fmaf(-slope2, d[u], capped_one(dot, a.rule, t));
-                if (e0 + u * slots + slot >= run.y) s[u] = -inf_of();
-                high = fmaxf(high, s[u]);
-            }
-            const float ref = high == -inf_of() ? 0.f : high;
-            const float fade = exp2_of(top - ref);
-            top = high;
-            sum *= fade;
-#pragma unroll
-            for (int x = 0; x < VEC; ++x) acc[x] *= fade;
-#pragma unroll
-            for (int u = 0; u < kAhead; ++u) {
-                // a pair beyond the run's end repeats its last one, with weight 0
-                const bool in = e0 + u * slots + slot < run.y;
-                const float p = in ? exp2_of(s[u] - ref) : 0.f;
-                sum += p;
-#pragma unroll
-                for (int x = 0; x < VEC; ++x) acc[x] = fmaf(p, in ? vx[u][x] : 0.f, acc[x]);
-            }
-        }
-        for (int d = a.slot; d < kWave; d <<= 1) {
-            const float other = __shfl_xor(top, d), high = fmaxf(top, other);
-            const float ref = high == -inf_of() ? 0.f : high;
-            const float w = exp2_of(top - ref), z = exp2_of(other - ref);
-            sum = sum * w + __shfl_xor(sum, d) * z;
-#pragma unroll
-            for (int x = 0; x < VEC; ++x) acc[x] = acc[x] * w + __shfl_xor(acc[x], d) * z;
-            top = high;
-        }
-    }
-    if (!mine || slot != 0) return;
-    const float by = !valid ? nan_of() : sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll
-    for (int x = 0; x < VEC; ++x) acc[x] = valid ? acc[x] * by : nan_of();
-    store_floats<T, VEC>(out, acc);
-    if (a.out32) store_floats<float, VEC>(a.out32 + row * a.dim + c, acc);
-    if (a.lse && c == 0)
-        a.lse[row] = !valid ? nan_of() : sum == 0.f ? -inf_of() : top + __builtin_amdgcn_logf(sum);
-}
-
 // Floats of any count, 16 bytes at a time.
 template <int N>
 __device__ __forceinline__ void load_wide(const float* p, float (&x)[N]) {
@@ -256,187 +195,332 @@ __device__ __forceinline__ void load_wide(const float* p, float (&x)[N]) {
     }
 }
 
-// By sources: grad_q, grad_d, delta and the slopes' gradient by rows.  Blocks of
-// heads that do not fit a wave follow one another in it, so that a pair's
-// grad_d is summed by one lane.
-template <typename T, int LPH>
-__global__ __launch_bounds__(256) void k_neighbor_dq(const NeighborArgs a) {
-    constexpr int VEC = kVec<T>, kAhead = 4;
+// What a lane of a wave takes: 16 bytes of a key head's channels, for GH query
+// heads that share it (`head` is the first).  A slot holds `block` such units.
+// Lanes whose head or channels do not exist read those of others and add
+// nothing.
+template <typename T, int LPH, int GH>
+struct Lane {
+    static constexpr int VEC = Raw<T>::kVec;
+    int lane, slot, in_slot, slots, head, kv, c;
+    bool there, mine;  // the head exists; the channels too
+    __device__ __forceinline__ Lane(const NeighborArgs& a, int first) {
+        lane = lane_of();
+        slot = lane / a.slot;
+        in_slot = lane % a.slot;
+        slots = kWave / a.slot;
+        head = (first + in_slot / LPH) * GH;
+        there = head < a.heads;
+        c = (in_slot % LPH) * VEC;
+        mine = there && c < a.dim;
+        if (!there) head = 0;
+        kv = head / a.group;
+        if (!mine) c = 0;
+    }
+};
+template <typename T>
+__device__ __forceinline__ const char* row_at(const char* base, int row, uint32_t bytes) {
+    return base + (uint64_t)(uint32_t)row * bytes;
+}
+
+// grid: (sources / 4, blocks of units).
+template <typename T, int LPH, int GH>
+__global__ __launch_bounds__(256) void k_neighbor_forward(const NeighborArgs a) {
+    constexpr int VEC = Raw<T>::kVec, kAhead = 4;
     const int64_t i = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
     if (i >= a.n_sources) return;
-    const int lane = lane_of(), slot = lane / a.slot, in_slot = lane % a.slot;
-    const int slots = kWave / a.slot, block = a.slot / LPH;
-    const int c = (in_slot % LPH) * VEC;
+    const Lane<T, LPH, GH> l(a, blockIdx.y * (a.slot / LPH));
+    const int64_t row = i * a.heads + l.head;
+    float acc[GH][VEC], top[GH], sum[GH];
+#pragma unroll
+    for (int g = 0; g < GH; ++g) {
+        top[g] = -inf_of();
+        sum[g] = 0.f;
+#pragma unroll
+        for (int x = 0; x < VEC; ++x) acc[g][x] = 0.f;
+    }
+    const bool valid = *a.rows.status == 0;
+    if (valid) {
+        Raw<T> q[GH];
+        float slope2[GH];
+#pragma unroll
+        for (int g = 0; g < GH; ++g) {
+            q[g] = Raw<T>{};
+            if (l.mine)
+                q[g] = Raw<T>::at((const char*)((const T*)a.q + i * a.q_stride[0] +
+                                                (l.head + g) * a.q_stride[1] + l.c));
+            slope2[g] = a.slopes[l.head + g] * kLog2e;
+        }
+        const char* k = (const char*)((const T*)a.k + l.kv * a.k_stride[1] + l.c);
+        const char* v = (const char*)((const T*)a.v + l.kv * a.v_stride[1] + l.c);
+        const uint32_t k_row = (uint32_t)(a.k_stride[0] * sizeof(T));
+        const uint32_t v_row = (uint32_t)(a.v_stride[0] * sizeof(T));
+        const int2 run = run_of(a.rows.sources, i);
+        // a pair beyond the run's end repeats its last one, with weight 0
+        const auto step = [&](int e0, auto whole) {
+            Raw<T> kx[kAhead], vx[kAhead];
+            float d[kAhead];
+            bool in[kAhead];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                int e = e0 + u * l.slots + l.slot;
+                in[u] = whole || e < run.y;
+                if (!whole) e = min(e, run.y - 1);
+                const int j = a.rows.target[e];
+                d[u] = a.distances[e];
+                kx[u] = Raw<T>::at(row_at<T>(k, j, k_row));
+                vx[u] = Raw<T>::at(row_at<T>(v, j, v_row));
+            }
+            if (!whole)
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u)
+                    if (!in[u]) vx[u] = Raw<T>{};
+#pragma unroll
+            for (int g = 0; g < GH; ++g) {
+                float s[kAhead], high = top[g], t;
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u) {
+                    const float dot = head_sum<LPH>(q[g].dot(kx[u], 0.f));
+                    s[u] = fmaf(-slope2[g], d[u], capped_one(dot, a.rule, t));
+                    if (!whole && !in[u]) s[u] = -inf_of();
+                    high = fmaxf(high, s[u]);
+                }
+                const float ref = high == -inf_of() ? 0.f : high;
+                const float fade = exp2_of(top[g] - ref);
+                top[g] = high;
+                sum[g] *= fade;
+#pragma unroll
+                for (int x = 0; x < VEC; ++x) acc[g][x] *= fade;
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u) {
+                    const float p = exp2_of(s[u] - ref);
+                    sum[g] += p;
+                    vx[u].add(p, acc[g]);
+                }
+            }
+        };
+        int e0 = run.x;
+        for (; e0 + l.slots * kAhead <= run.y; e0 += l.slots * kAhead)
+            step(e0, std::true_type{});
+        if (e0 < run.y) step(e0, std::false_type{});
+        // the slots' sums, in the largest maximum's terms
+#pragma unroll
+        for (int g = 0; g < GH; ++g) {
+            const float high = join_lanes<max_of>(top[g], a.slot);
+            const float w = exp2_of(top[g] - (high == -inf_of() ? 0.f : high));
+            top[g] = high;
+            sum[g] = join_lanes<sum_of>(sum[g] * w, a.slot);
+#pragma unroll
+            for (int x = 0; x < VEC; ++x) acc[g][x] = join_lanes<sum_of>(acc[g][x] * w, a.slot);
+        }
+    }
+    if (!l.mine || l.slot != 0) return;
+#pragma unroll
+    for (int g = 0; g < GH; ++g) {
+        const float by = sum[g] == 0.f ? 0.f : 1.f / sum[g];
+        const int64_t at = (row + g) * a.dim + l.c;
+#pragma unroll
+        for (int x = 0; x < VEC; ++x) acc[g][x] = valid ? acc[g][x] * by : nan_of();
+        store_floats<T, VEC>((T*)a.out + at, acc[g]);
+        if (a.out32) store_floats<float, VEC>(a.out32 + at, acc[g]);
+        if (a.lse && l.c == 0)
+            a.lse[row + g] = !valid        ? nan_of()
+                             : sum[g] == 0.f ? -inf_of()
+                                             : top[g] + __builtin_amdgcn_logf(sum[g]);
+    }
+}
+
+// By sources: grad_q, grad_d, delta and the slopes' gradient by rows.  Blocks of
+// units that do not fit a wave follow one another in it, so that a pair's
+// grad_d is summed by one lane.
+template <typename T, int LPH, int GH>
+__global__ __launch_bounds__(256) void k_neighbor_dq(const NeighborArgs a) {
+    constexpr int VEC = Raw<T>::kVec, kAhead = GH == 4 ? 2 : 4;
+    const int64_t i = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
+    if (i >= a.n_sources) return;
     if (*a.rows.status != 0) {
+        const int lane = lane_of();
         fill_nan((T*)a.grad_q + i * a.heads * a.dim, (int64_t)a.heads * a.dim, lane, kWave);
         fill_nan(a.grad_distances, a.n_pairs, i * kWave + lane, (int64_t)a.n_sources * kWave);
         for (int h = lane; h < a.heads; h += kWave) a.turn[(int64_t)h * a.n_sources + i] = nan_of();
         return;
     }
     const int2 run = run_of(a.rows.sources, i);
-    for (int h0 = 0; h0 < a.heads; h0 += block) {
-        const int head = h0 + in_slot / LPH;
-        const bool mine = head < a.heads && c < a.dim;
-        const int64_t row = i * a.heads + head;
-        float q[VEC] = {}, go[VEC] = {}, acc[VEC];
-        float delta = 0.f, turn = 0.f, lse = inf_of(), slope = 0.f;
-        if (mine) {
-            float o[VEC];
-            load_floats<T, VEC>((const T*)a.q + i * a.q_stride[0] + head * a.q_stride[1] + c, q);
-            load_floats<T, VEC>((const T*)a.grad_out + row * a.dim + c, go);
-            load_wide<VEC>(a.out_full + row * a.dim + c, o);
+    const uint32_t k_row = (uint32_t)(a.k_stride[0] * sizeof(T));
+    const uint32_t v_row = (uint32_t)(a.v_stride[0] * sizeof(T));
+    for (int first = 0; first * GH < a.heads; first += a.slot / LPH) {
+        const Lane<T, LPH, GH> l(a, first);
+        const int64_t row = i * a.heads + l.head;
+        Raw<T> q[GH], go[GH];
+        float acc[GH][VEC], delta[GH], turn[GH], lse[GH], slope[GH];
 #pragma unroll
-            for (int x = 0; x < VEC; ++x) delta = fmaf(go[x], o[x], delta);
-            lse = a.lse[row];
-            if (lse == -inf_of()) lse = inf_of();
-            slope = a.slopes[head];
+        for (int g = 0; g < GH; ++g) {
+            q[g] = go[g] = Raw<T>{};
+            delta[g] = turn[g] = slope[g] = 0.f;
+            lse[g] = inf_of();  // a lane without channels weighs nothing
+            if (l.mine) {
+                const int64_t at = (row + g) * a.dim + l.c;
+                float o[VEC];
+                q[g] = Raw<T>::at((const char*)((const T*)a.q + i * a.q_stride[0] +
+                                                (l.head + g) * a.q_stride[1] + l.c));
+                go[g] = Raw<T>::at((const char*)((const T*)a.grad_out + at));
+                load_wide<VEC>(a.out_full + at, o);
+#pragma unroll
+                for (int x = 0; x < VEC; ++x) delta[g] = fmaf((float)go[g].x[x], o[x], delta[g]);
+                lse[g] = a.lse[row + g];
+                if (lse[g] == -inf_of()) lse[g] = inf_of();
+                slope[g] = a.slopes[l.head + g];
+            }
+            delta[g] = head_sum<LPH>(delta[g]);
+            if (l.mine && l.c == 0 && l.slot == 0) a.delta[row + g] = delta[g];
+#pragma unroll
+            for (int x = 0; x < VEC; ++x) acc[g][x] = 0.f;
         }
-        delta = head_sum<LPH>(delta);
-        // every lane of a head that is there holds its lse and slope
-        const float slope2 = slope * kLog2e;
-        if (mine && c == 0 && slot == 0) a.delta[row] = delta;
-#pragma unroll
-        for (int x = 0; x < VEC; ++x) acc[x] = 0.f;
-        const int kv = mine ? head / a.group : 0;
-        const T* k = (const T*)a.k + kv * a.k_stride[1] + (mine ? c : 0);
-        const T* v = (const T*)a.v + kv * a.v_stride[1] + (mine ? c : 0);
-        for (int e0 = run.x; e0 < run.y; e0 += slots * kAhead) {
-            float kx[kAhead][VEC], vx[kAhead][VEC], d[kAhead];
+        const char* k = (const char*)((const T*)a.k + l.kv * a.k_stride[1] + l.c);
+        const char* v = (const char*)((const T*)a.v + l.kv * a.v_stride[1] + l.c);
+        const auto step = [&](int e0, auto whole) {
+            Raw<T> kx[kAhead], vx[kAhead];
+            float d[kAhead];
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
-                const int e = min(e0 + u * slots + slot, run.y - 1);
-                const int64_t j = a.rows.target[e];
+                int e = e0 + u * l.slots + l.slot;
+                if (!whole) e = min(e, run.y - 1);
+                const int j = a.rows.target[e];
                 d[u] = a.distances[e];
-                load_floats<T, VEC>(k + j * a.k_stride[0], kx[u]);
-                load_floats<T, VEC>(v + j * a.v_stride[0], vx[u]);
+                kx[u] = Raw<T>::at(row_at<T>(k, j, k_row));
+                vx[u] = Raw<T>::at(row_at<T>(v, j, v_row));
             }
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
-                const int e = e0 + u * slots + slot;
-                const bool in = e < run.y;
-                float dot = 0.f, dp = 0.f, t;
+                const int e = e0 + u * l.slots + l.slot;
+                const bool in = whole || e < run.y;
+                if (!whole && !in) kx[u] = Raw<T>{};
+                float push = 0.f;
 #pragma unroll
-                for (int x = 0; x < VEC; ++x) {
-                    dot = fmaf(q[x], kx[u][x], dot);
-                    dp = fmaf(go[x], vx[u][x], dp);
+                for (int g = 0; g < GH; ++g) {
+                    float t;
+                    const float dot = head_sum<LPH>(q[g].dot(kx[u], 0.f));
+                    const float dp = head_sum<LPH>(go[g].dot(vx[u], 0.f));
+                    const float s =
+                        fmaf(-slope[g] * kLog2e, d[u], capped_one(dot, a.rule, t));
+                    float ds = exp2_of(s - lse[g]) * (dp - delta[g]);
+                    if (!l.mine || (!whole && !in)) ds = 0.f;
+                    kx[u].add(a.rule.cap > 0.f ? ds * fmaf(-t, t, 1.f) : ds, acc[g]);
+                    turn[g] = fmaf(-ds, d[u], turn[g]);
+                    push = fmaf(-slope[g], ds, push);
                 }
-                dot = head_sum<LPH>(mine ? dot : 0.f);
-                dp = head_sum<LPH>(mine ? dp : 0.f);
-                const float s = fmaf(-slope2, d[u], capped_one(dot, a.rule, t));
-                // (only lanes of the head's channels know its lse)
-                const float ds = in && mine ? exp2_of(s - lse) * (dp - delta) : 0.f;
-                const float dx = ds * fmaf(-t, t, 1.f);
-#pragma unroll
-                for (int x = 0; x < VEC; ++x) acc[x] = fmaf(dx, in ? kx[u][x] : 0.f, acc[x]);
-                turn = fmaf(-ds, in ? d[u] : 0.f, turn);
-                float push = -slope * ds;
                 for (int w = LPH; w < a.slot; w <<= 1) push += __shfl_xor(push, w);
-                if (in && in_slot == 0)
-                    a.grad_distances[e] = h0 == 0 ? push : a.grad_distances[e] + push;
+                if (in && l.in_slot == 0)
+                    a.grad_distances[e] = first == 0 ? push : a.grad_distances[e] + push;
             }
-        }
-        for (int d = a.slot; d < kWave; d <<= 1) {
-            turn += __shfl_xor(turn, d);
+        };
+        int e0 = run.x;
+        for (; e0 + l.slots * kAhead <= run.y; e0 += l.slots * kAhead)
+            step(e0, std::true_type{});
+        if (e0 < run.y) step(e0, std::false_type{});
 #pragma unroll
-            for (int x = 0; x < VEC; ++x) acc[x] += __shfl_xor(acc[x], d);
-        }
-        if (mine && slot == 0) {
+        for (int g = 0; g < GH; ++g) {
+            turn[g] = join_lanes<sum_of>(turn[g], a.slot);
 #pragma unroll
-            for (int x = 0; x < VEC; ++x) acc[x] *= a.rule.scale;
-            store_floats<T, VEC>((T*)a.grad_q + row * a.dim + c, acc);
-            if (c == 0) a.turn[(int64_t)head * a.n_sources + i] = turn;
+            for (int x = 0; x < VEC; ++x)
+                acc[g][x] = join_lanes<sum_of>(acc[g][x], a.slot) * a.rule.scale;
+            if (l.mine && l.slot == 0) {
+                store_floats<T, VEC>((T*)a.grad_q + (row + g) * a.dim + l.c, acc[g]);
+                if (l.c == 0) a.turn[(int64_t)(l.head + g) * a.n_sources + i] = turn[g];
+            }
         }
     }
 }
 
-// By targets: grad_k and grad_v.  grid: (targets / 4, blocks of key heads).
-template <typename T, int LPH>
+// By targets: grad_k and grad_v.  grid: (targets / 4, blocks of key heads).  A
+// unit here is a key head; its query heads are taken GH at a time.
+template <typename T, int LPH, int GH>
 __global__ __launch_bounds__(256) void k_neighbor_dkv(const NeighborArgs a) {
-    constexpr int VEC = kVec<T>, kAhead = 2;
+    constexpr int VEC = Raw<T>::kVec, kAhead = GH == 4 ? 1 : GH == 2 ? 2 : 4;
     const int64_t j = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
     if (j >= a.n_targets) return;
     const int lane = lane_of(), slot = lane / a.slot, in_slot = lane % a.slot;
-    const int kv = blockIdx.y * (a.slot / LPH) + in_slot / LPH;
-    const int c = (in_slot % LPH) * VEC;
-    const bool mine = kv < a.kv_heads && c < a.dim;
     const int slots = kWave / a.slot;
+    int kv = blockIdx.y * (a.slot / LPH) + in_slot / LPH, c = (in_slot % LPH) * VEC;
+    const bool mine = kv < a.kv_heads && c < a.dim;
+    if (kv >= a.kv_heads) kv = 0;
+    if (!mine) c = 0;
     const int64_t flat = (j * a.kv_heads + kv) * a.dim + c;
     float dk[VEC], dv[VEC];
     const bool valid = *a.rows.status == 0;
 #pragma unroll
     for (int x = 0; x < VEC; ++x) dk[x] = dv[x] = valid ? 0.f : nan_of();
     if (valid) {
-        float k[VEC] = {}, v[VEC] = {};
+        Raw<T> k{}, v{};
         if (mine) {
-            load_floats<T, VEC>((const T*)a.k + j * a.k_stride[0] + kv * a.k_stride[1] + c, k);
-            load_floats<T, VEC>((const T*)a.v + j * a.v_stride[0] + kv * a.v_stride[1] + c, v);
+            k = Raw<T>::at((const char*)((const T*)a.k + j * a.k_stride[0] + kv * a.k_stride[1] + c));
+            v = Raw<T>::at((const char*)((const T*)a.v + j * a.v_stride[0] + kv * a.v_stride[1] + c));
         }
         const int2 run = run_of(a.rows.targets, j);
-        for (int g = 0; g < a.group; ++g) {
-            const int head = mine ? kv * a.group + g : 0;
-            const float slope2 = a.slopes[head] * kLog2e;
-            const T* q = (const T*)a.q + head * a.q_stride[1] + (mine ? c : 0);
-            const T* go = (const T*)a.grad_out + (int64_t)head * a.dim + (mine ? c : 0);
-            for (int p0 = run.x; p0 < run.y; p0 += slots * kAhead) {
-                float qx[kAhead][VEC], ox[kAhead][VEC], d[kAhead], lse[kAhead], delta[kAhead];
+        const uint32_t q_row = (uint32_t)(a.q_stride[0] * sizeof(T));
+        const uint32_t q_head = (uint32_t)(a.q_stride[1] * sizeof(T));
+        const uint32_t o_head = (uint32_t)(a.dim * sizeof(T)), o_row = a.heads * o_head;
+        for (int g0 = 0; g0 < a.group; g0 += GH) {
+            const int head = kv * a.group + g0;
+            float slope2[GH];
+#pragma unroll
+            for (int g = 0; g < GH; ++g) slope2[g] = a.slopes[head + g] * kLog2e;
+            const char* q = (const char*)((const T*)a.q + head * a.q_stride[1] + c);
+            const char* go = (const char*)((const T*)a.grad_out + (int64_t)head * a.dim + c);
+            const auto step = [&](int p0, auto whole) {
+                Raw<T> qx[kAhead][GH], ox[kAhead][GH];
+                float d[kAhead], lse[kAhead][GH], delta[kAhead][GH];
 #pragma unroll
                 for (int u = 0; u < kAhead; ++u) {
-                    const int2 at = a.rows.order[min(p0 + u * slots + slot, run.y - 1)];
-                    const int64_t i = at.y;
-                    d[u] = a.distances[at.x];
-                    load_floats<T, VEC>(q + i * a.q_stride[0], qx[u]);
-                    load_floats<T, VEC>(go + i * a.heads * a.dim, ox[u]);
-                    lse[u] = a.lse[i * a.heads + head];
-                    delta[u] = a.delta[i * a.heads + head];
+                    int at = p0 + u * slots + slot;
+                    if (!whole) at = min(at, run.y - 1);
+                    const int2 pair = a.rows.order[at];
+                    const char* qi = row_at<T>(q, pair.y, q_row);
+                    const char* oi = row_at<T>(go, pair.y, o_row);
+                    const int64_t row = (int64_t)pair.y * a.heads + head;
+                    d[u] = a.distances[pair.x];
+#pragma unroll
+                    for (int g = 0; g < GH; ++g) {
+                        qx[u][g] = Raw<T>::at(qi + g * q_head);
+                        ox[u][g] = Raw<T>::at(oi + g * o_head);
+                        lse[u][g] = a.lse[row + g];
+                        delta[u][g] = a.delta[row + g];
+                    }
                 }
 #pragma unroll
                 for (int u = 0; u < kAhead; ++u) {
-                    const bool in = p0 + u * slots + slot < run.y;
-                    float dot = 0.f, dp = 0.f, t;
+                    const bool in = whole || p0 + u * slots + slot < run.y;
 #pragma unroll
-                    for (int x = 0; x < VEC; ++x) {
-                        dot = fmaf(qx[u][x], k[x], dot);
-                        dp = fmaf(ox[u][x], v[x], dp);
-                    }
-                    dot = head_sum<LPH>(mine ? dot : 0.f);
-                    dp = head_sum<LPH>(mine ? dp : 0.f);
-                    const float s = fmaf(-slope2, d[u], capped_one(dot, a.rule, t));
-                    const bool any = in && lse[u] != -inf_of();
-                    const float p = any ? exp2_of(s - lse[u]) : 0.f;
-                    const float dx = any ? p * (dp - delta[u]) * fmaf(-t, t, 1.f) : 0.f;
-#pragma unroll
-                    for (int x = 0; x < VEC; ++x) {
-                        dk[x] = fmaf(dx, in ? qx[u][x] : 0.f, dk[x]);
-                        dv[x] = fmaf(p, in ? ox[u][x] : 0.f, dv[x]);
+                    for (int g = 0; g < GH; ++g) {
+                        float t;
+                        if (!whole && !in) qx[u][g] = ox[u][g] = Raw<T>{};
+                        const float dot = head_sum<LPH>(qx[u][g].dot(k, 0.f));
+                        const float dp = head_sum<LPH>(ox[u][g].dot(v, 0.f));
+                        const float s = fmaf(-slope2[g], d[u], capped_one(dot, a.rule, t));
+                        const bool any = in && lse[u][g] != -inf_of();
+                        const float p = any ? exp2_of(s - lse[u][g]) : 0.f;
+                        float dx = any ? p * (dp - delta[u][g]) : 0.f;
+                        if (a.rule.cap > 0.f) dx *= fmaf(-t, t, 1.f);
+                        qx[u][g].add(dx, dk);
+                        ox[u][g].add(p, dv);
                     }
                 }
-            }
+            };
+            int p0 = run.x;
+            for (; p0 + slots * kAhead <= run.y; p0 += slots * kAhead) step(p0, std::true_type{});
+            if (p0 < run.y) step(p0, std::false_type{});
         }
-        for (int d = a.slot; d < kWave; d <<= 1)
 #pragma unroll
-            for (int x = 0; x < VEC; ++x) {
-                dk[x] += __shfl_xor(dk[x], d);
-                dv[x] += __shfl_xor(dv[x], d);
-            }
+        for (int x = 0; x < VEC; ++x) {
+            dk[x] = join_lanes<sum_of>(dk[x], a.slot);
+            dv[x] = join_lanes<sum_of>(dv[x], a.slot);
+        }
     }
     if (!mine || slot != 0) return;
 #pragma unroll
     for (int x = 0; x < VEC; ++x) dk[x] *= a.rule.scale;
     store_floats<T, VEC>((T*)a.grad_k + flat, dk);
     store_floats<T, VEC>((T*)a.grad_v + flat, dv);
-}
-
-// A head's slope: the sum of its rows, one workgroup each.
-__global__ __launch_bounds__(256) void k_neighbor_slopes(const float* turn, int64_t rows,
-                                                         float* grad_slopes) {
-    __shared__ float waves[4];
-    const float* from = turn + (int64_t)blockIdx.x * rows;
-    float sum = 0.f;
-    for (int64_t i = threadIdx.x; i < rows; i += 256) sum += from[i];
-    for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
-    if (lane_of() == 0) waves[threadIdx.x / kWave] = sum;
-    __syncthreads();
-    if (threadIdx.x == 0) grad_slopes[blockIdx.x] = waves[0] + waves[1] + waves[2] + waves[3];
 }
 
 }  // namespace op

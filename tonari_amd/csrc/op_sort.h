@@ -15,7 +15,7 @@ namespace op {
 
 constexpr int kSortThreads = 256;
 constexpr int kSortWaves = kSortThreads / kWave;
-constexpr int kSortRounds = 16;                           // items of a lane
+constexpr int kSortRounds = 8;                            // items of a lane
 constexpr int kSortTile = kSortThreads * kSortRounds;     // items of a workgroup
 constexpr int kSortBits = 10;
 constexpr int kSortRadix = 1 << kSortBits;

@@ -49,10 +49,11 @@ struct StructureArgs {
     ScoreRule rule;
     int heads, kv_heads, group, dim;
     int n_queries, n_keys;
-    int splits;
+    int splits, k_splits;
     void* out;
     float* lse;   // [heads][n_queries], base 2
-    float* part;  // forward splits: [split][heads][n_queries][dim + 2]
+    float* part;    // splits of a row: [split][heads][n_queries][dim + 2], or dim + kRowSums
+    float* part_k;  // splits of a key: [split][kv_heads][n_keys][2 dim + 3]
     const void* grad_out;
     void *grad_q, *grad_k, *grad_v;
     float* row;     // [heads][n_queries][2]: delta, largest |grad_out|

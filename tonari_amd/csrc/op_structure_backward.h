@@ -238,7 +238,7 @@ __global__ __launch_bounds__(256) void k_structure_join_dq(const StructureArgs a
     if (lane == 0) finish_row(a, head, query, delta, top, a.slopes[head], w);
 }
 
-// grid: (key tiles, kv_heads); NW waves of 32 keys each.
+// grid: (key tiles, kv_heads * k_splits); NW waves of 32 keys each.
 template <typename T, int DP, int NW>
 __global__ __launch_bounds__(NW* kWave) void k_structure_dkv(const StructureArgs a) {
     using M = Mat<T>;
@@ -254,10 +254,16 @@ __global__ __launch_bounds__(NW* kWave) void k_structure_dkv(const StructureArgs
 
     const StructureTile t = a.k_tiles[blockIdx.x];
     const int lane = lane_of(), half = lane / 32, wave = threadIdx.x / kWave;
-    const int kv = blockIdx.y;
+    const int kv = blockIdx.y % a.kv_heads, split = blockIdx.y / a.kv_heads;
     if (t.n_q < 0) {
         const int64_t key = (int64_t)blockIdx.x * (NW * kTile) + wave * kTile + lane % 32;
         if (key >= a.n_keys || half) return;
+        if (a.k_splits > 1) {
+            float* part = a.part_k + (((int64_t)split * a.kv_heads + kv) * a.n_keys + key) *
+                                         (2 * a.dim + 3);
+            for (int c = 0; c < 2 * a.dim + 3; ++c) part[c] = nan_of();
+            return;
+        }
         for (int c = 0; c < a.dim; ++c) {
             ((T*)a.grad_k)[(key * a.kv_heads + kv) * a.dim + c] = rounded<T>(nan_of());
             ((T*)a.grad_v)[(key * a.kv_heads + kv) * a.dim + c] = rounded<T>(nan_of());
@@ -307,8 +313,10 @@ __global__ __launch_bounds__(NW* kWave) void k_structure_dkv(const StructureArgs
             }
         }
     };
-    if (tiles > 0) fetch(0);
-    for (int tile = 0; tile < tiles; ++tile) {
+    const int each = (tiles + a.k_splits - 1) / a.k_splits;
+    const int from = min(tiles, split * each), to = min(tiles, from + each);
+    if (from < to) fetch(from);
+    for (int tile = from; tile < to; ++tile) {
         __syncthreads();
         stage.store(q_rows, M::kSeparateCols ? q_cols : nullptr, o_rows,
                     M::kSeparateCols ? o_cols : nullptr);
@@ -318,7 +326,7 @@ __global__ __launch_bounds__(NW* kWave) void k_structure_dkv(const StructureArgs
         }
         __syncthreads();
         const float slope = a.slopes[kv * a.group + tile / per_head], slope2 = slope * kLog2e;
-        if (tile + 1 < tiles) fetch(tile + 1);
+        if (tile + 1 < to) fetch(tile + 1);
 
         f32x16 dot{}, dp{};
         M::template rows<DP>(dot, q_rows, kr);
@@ -371,6 +379,25 @@ __global__ __launch_bounds__(NW* kWave) void k_structure_dkv(const StructureArgs
     if (!valid) return;
     const int64_t flat = (key * a.kv_heads + kv) * a.dim;
     const float back = kNarrow<T> && scale_e != kNoScale ? power_of(scale_e) : 1.f;
+    if (a.k_splits > 1) {
+        float* part =
+            a.part_k + (((int64_t)split * a.kv_heads + kv) * a.n_keys + key) * (2 * a.dim + 3);
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int c = 32 * d + row_of(i, half);
+                if (c >= a.dim) continue;
+                part[c] = dk[d][i] * back;
+                part[a.dim + c] = dv[d][i] * kLower;
+            }
+        if (half == 0) {
+            part[2 * a.dim] = px;
+            part[2 * a.dim + 1] = py;
+            part[2 * a.dim + 2] = pz;
+        }
+        return;
+    }
     store_channels<T, DP>((T*)a.grad_k + flat, a.dim, dk, a.rule.scale * back);
     store_channels<T, DP>((T*)a.grad_v + flat, a.dim, dv, kLower);
     if (a.push_k && half == 0) {
@@ -381,29 +408,32 @@ __global__ __launch_bounds__(NW* kWave) void k_structure_dkv(const StructureArgs
     }
 }
 
-// Sums over the heads: positions' gradients (threads over atoms and axes), and
-// over all rows: a slope's (one workgroup each, the first `heads` of the grid
-// where slopes are wanted).
+// Joins the splits of a key: threads over its 2 dim + 3 sums.
+template <typename T>
+__global__ __launch_bounds__(256) void k_structure_join_dkv(const StructureArgs a) {
+    const int64_t width = 2 * a.dim + 3, keys = (int64_t)a.kv_heads * a.n_keys;
+    const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (u >= keys * width) return;
+    const int64_t at = u / width;
+    const int c = (int)(u - at * width);
+    float sum = 0.f;
+#pragma unroll 4
+    for (int s = 0; s < a.k_splits; ++s) sum += a.part_k[s * keys * width + u];
+    const int64_t kv = at / a.n_keys, key = at - kv * a.n_keys;
+    const int64_t flat = (key * a.kv_heads + kv) * a.dim;
+    if (c < a.dim)
+        ((T*)a.grad_k)[flat + c] = rounded<T>(sum * a.rule.scale);
+    else if (c < 2 * a.dim)
+        ((T*)a.grad_v)[flat + c - a.dim] = rounded<T>(sum);
+    else if (a.push_k)
+        a.push_k[3 * at + c - 2 * a.dim] = sum;
+}
+
+// Sums over the heads of the positions' gradients, threads over atoms and axes.
 __global__ __launch_bounds__(256) void k_structure_finish(const StructureArgs a, float* grad_x_q,
-                                                          float* grad_x_k, float* grad_slopes,
-                                                          int shared) {
-    int64_t block = blockIdx.x;
-    if (grad_slopes) {
-        if (block < a.heads) {
-            __shared__ float waves[4];
-            const float* from = a.turn + block * a.n_queries;
-            float sum = 0.f;
-            for (int64_t i = threadIdx.x; i < a.n_queries; i += 256) sum += from[i];
-            for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
-            if (lane_of() == 0) waves[threadIdx.x / kWave] = sum;
-            __syncthreads();
-            if (threadIdx.x == 0) grad_slopes[block] = waves[0] + waves[1] + waves[2] + waves[3];
-            return;
-        }
-        block -= a.heads;
-    }
+                                                          float* grad_x_k, int shared) {
     const int64_t nk = 3 * (int64_t)a.n_keys, nq = 3 * (int64_t)a.n_queries;
-    int64_t i = block * 256 + threadIdx.x;
+    int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (grad_x_k) {
         if (i < nk) {
             float sum = 0.f;

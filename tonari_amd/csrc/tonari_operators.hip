@@ -176,9 +176,12 @@ int check_heads(int32_t dtype, int32_t heads, int32_t kv_heads, int32_t dim, flo
     return TNR_OK;
 }
 
+// Rows are found by 32-bit strides in bytes.
 bool aligned(const void* p, const int64_t (&stride)[2], int32_t dtype) {
     const int64_t unit = 16 / (int64_t)size_of(dtype);
-    return (uintptr_t)p % 16 == 0 && stride[0] % unit == 0 && stride[1] % unit == 0;
+    for (const int64_t s : stride)
+        if (s % unit != 0 || s < 0 || s >= (int64_t(1) << 29)) return false;
+    return (uintptr_t)p % 16 == 0;
 }
 
 // ------------------------------------------------------- structure attention
@@ -191,9 +194,11 @@ int waves_for(int64_t rows, int64_t structures) {
 }
 
 struct StructurePlan {
-    int group, q_waves, k_waves, splits;
+    int group, q_waves, k_waves, splits, k_splits;
     int64_t q_tiles, k_tiles;
 };
+
+constexpr int64_t kSplitWaves = 4096;
 
 StructurePlan structure_plan(const tnr_structure_attention& r) {
     StructurePlan p{};
@@ -202,14 +207,19 @@ StructurePlan structure_plan(const tnr_structure_attention& r) {
     p.k_waves = waves_for(r.n_keys, r.n_structures);
     p.q_tiles = tile_start(r.n_queries, p.group, p.q_waves * kTile, r.n_structures);
     p.k_tiles = tile_start(r.n_keys, 1, p.k_waves * kTile, r.n_structures);
-    // Few rows: keys are split over workgroups, at least 8 tiles each, until
-    // there are waves enough for the device.
-    const int64_t waves = (r.n_queries * p.group / kTile + r.n_structures) * r.kv_heads;
-    const int64_t mean = r.n_structures > 0 ? r.n_keys / r.n_structures / (8 * kTile) : 0;
-    int64_t splits = waves > 0 ? 2048 / waves : 1;
-    if (splits > mean) splits = mean;
-    if (splits > 64) splits = 64;
-    p.splits = splits < 2 ? 1 : (int)splits;
+    // Few rows: the keys (or, for the keys' gradients, the rows) are split over
+    // workgroups, at least 8 tiles each, until there are waves enough for the
+    // device.
+    const auto split = [&](int64_t rows, int64_t others) {
+        const int64_t waves = (rows / kTile + r.n_structures) * r.kv_heads;
+        const int64_t most = r.n_structures > 0 ? others / r.n_structures / (8 * kTile) : 0;
+        int64_t n = waves > 0 ? kSplitWaves / waves : 1;
+        if (n > most) n = most;
+        if (n > 64) n = 64;
+        return n < 2 ? 1 : (int)n;
+    };
+    p.splits = split(r.n_queries * p.group, r.n_keys);
+    p.k_splits = split(r.n_keys, r.n_queries * p.group);
     return p;
 }
 
@@ -235,7 +245,7 @@ int check_structure(const tnr_structure_attention* r, bool backward, char* err, 
         return refuse(err, len, "required pointers are null");
     if (!aligned(r->q, r->q_stride, r->dtype) || !aligned(r->k, r->k_stride, r->dtype) ||
         !aligned(r->v, r->v_stride, r->dtype) || (uintptr_t)r->out % 16 != 0)
-        return refuse(err, len, "q, k, v and out must be aligned to 16 bytes");
+        return refuse(err, len, "q, k, v and out must be aligned to 16 bytes, with strides below 2^29");
     if (backward) {
         if ((r->n_queries > 0 && (!r->grad_out || !r->grad_q || !r->lse)) ||
             (r->n_keys > 0 && (!r->grad_k || !r->grad_v)))
@@ -268,6 +278,7 @@ StructureArgs structure_args(const tnr_structure_attention& r, const StructurePl
     a.n_queries = (int)r.n_queries;
     a.n_keys = (int)r.n_keys;
     a.splits = p.splits;
+    a.k_splits = p.k_splits;
     a.out = r.out;
     a.lse = r.lse;
     a.grad_out = r.grad_out;
@@ -280,7 +291,7 @@ StructureArgs structure_args(const tnr_structure_attention& r, const StructurePl
 // Where the batch has no tile table of its own size, the pointers into it.
 struct StructureSpace {
     StructureTile *q_tiles, *k_tiles;
-    float *part, *row, *push_q, *push_k, *turn;
+    float *part, *part_k, *row, *push_q, *push_k, *turn;
     size_t bytes;
 };
 StructureSpace structure_space(const tnr_structure_attention& r, const StructurePlan& p,
@@ -298,6 +309,9 @@ StructureSpace structure_space(const tnr_structure_attention& r, const Structure
         s.part = (float*)part(rows * p.splits * (r.dim + (backward ? kRowSums : 2)) * 4);
     if (backward) {
         s.k_tiles = (StructureTile*)part((size_t)p.k_tiles * sizeof(StructureTile));
+        if (p.k_splits > 1)
+            s.part_k = (float*)part((size_t)r.kv_heads * r.n_keys * p.k_splits *
+                                    (2 * r.dim + 3) * 4);
         s.row = (float*)part(rows * 8);
         if (r.grad_positions || r.grad_query_positions) {
             s.push_q = (float*)part(rows * 12);
@@ -396,7 +410,7 @@ int check_neighbor(const tnr_neighbor_attention* r, bool backward, char* err, si
         return refuse(err, len, "required pointers are null");
     if (!aligned(r->q, r->q_stride, r->dtype) || !aligned(r->k, r->k_stride, r->dtype) ||
         !aligned(r->v, r->v_stride, r->dtype) || (uintptr_t)r->out % 16 != 0)
-        return refuse(err, len, "q, k, v and out must be aligned to 16 bytes");
+        return refuse(err, len, "q, k, v and out must be aligned to 16 bytes, with strides below 2^29");
     if (backward) {
         if (!r->list.transpose) return refuse(err, len, "the backward needs the rows by target too");
         if ((r->list.n_sources > 0 && (!r->grad_out || !r->grad_q || !r->lse ||
@@ -444,28 +458,37 @@ NeighborArgs neighbor_args(const tnr_neighbor_attention& r) {
     return a;
 }
 
-// Lanes of 16 bytes that make a head: a power of two.
-template <typename F>
-void with_lanes(int32_t dtype, int32_t dim, F&& f) {
-    const int units = (int)(dim * size_of(dtype) / 16);
+// Lanes of 16 bytes that make a head, a power of two (types of 16 bits fill 16 at
+// most), and the query heads that one lane takes.
+template <typename T, typename F>
+void with_lanes(int32_t dim, int group, F&& f) {
+    const int units = (int)(dim * sizeof(T) / 16);
+    const auto heads = [&](auto lanes) {
+        if (group % 4 == 0)
+            f(lanes, Int<4>{});
+        else if (group % 2 == 0)
+            f(lanes, Int<2>{});
+        else
+            f(lanes, Int<1>{});
+    };
     if (units <= 1)
-        f(Int<1>{});
+        heads(Int<1>{});
     else if (units <= 2)
-        f(Int<2>{});
+        heads(Int<2>{});
     else if (units <= 4)
-        f(Int<4>{});
+        heads(Int<4>{});
     else if (units <= 8)
-        f(Int<8>{});
+        heads(Int<8>{});
     else if (units <= 16)
-        f(Int<16>{});
-    else
-        f(Int<32>{});
+        heads(Int<16>{});
+    else if constexpr (sizeof(T) == 4)
+        heads(Int<32>{});
 }
 
-// Lanes of a slot: the heads' lanes, a power of two, at most a wave.
-int slot_of(int lanes, int heads) {
+// Lanes of a slot: those of its units, a power of two, at most a wave.
+int slot_of(int lanes, int units) {
     int slot = lanes;
-    while (slot < kWave && slot < lanes * heads) slot *= 2;
+    while (slot < kWave && slot < lanes * units) slot *= 2;
     return slot;
 }
 
@@ -603,6 +626,7 @@ int tnr_structure_backward(const tnr_structure_attention* req, void* workspace,
     a.q_tiles = s.q_tiles;
     a.k_tiles = s.k_tiles;
     a.part = s.part;
+    a.part_k = s.part_k;
     a.row = s.row;
     a.push_q = s.push_q;
     a.push_k = s.push_k;
@@ -626,18 +650,23 @@ int tnr_structure_backward(const tnr_structure_attention* req, void* workspace,
                 with_waves(p.k_waves, [&](auto w) {
                     constexpr int NW = decltype(w)::value;
                     k_structure_dkv<T, DP, NW>
-                        <<<dim3((unsigned)p.k_tiles, r.kv_heads), NW * kWave, 0, st>>>(a);
+                        <<<dim3((unsigned)p.k_tiles, r.kv_heads * p.k_splits), NW * kWave, 0,
+                           st>>>(a);
                 });
+            if (r.n_keys > 0 && p.k_splits > 1)
+                k_structure_join_dkv<T>
+                    <<<(unsigned)((r.kv_heads * r.n_keys * (2 * r.dim + 3) + 255) / 256), 256, 0,
+                       st>>>(a);
         });
     });
     const int shared = r.grad_positions && !r.grad_query_positions &&
                        r.query_positions == r.positions && r.n_queries == r.n_keys;
-    int64_t items = (r.grad_positions ? 3 * r.n_keys : 0) +
+    const int64_t items = (r.grad_positions ? 3 * r.n_keys : 0) +
                     (r.grad_query_positions ? 3 * r.n_queries : 0);
-    const int64_t blocks = (items + 255) / 256 + (r.grad_slopes ? r.heads : 0);
-    if (blocks > 0)
-        k_structure_finish<<<(unsigned)blocks, 256, 0, st>>>(a, r.grad_query_positions,
-                                                             r.grad_positions, r.grad_slopes, shared);
+    if (items > 0)
+        k_structure_finish<<<(unsigned)((items + 255) / 256), 256, 0, st>>>(
+            a, r.grad_query_positions, r.grad_positions, shared);
+    if (r.grad_slopes) k_slopes<<<r.heads, 1024, 0, st>>>(a.turn, r.n_queries, r.grad_slopes);
     return launched(err, err_len);
 }
 
@@ -703,13 +732,14 @@ int tnr_neighbor_forward(const tnr_neighbor_attention* req, void* stream, char* 
     NeighborArgs a = neighbor_args(r);
     with_type(r.dtype, [&](auto t) {
         using T = decltype(t);
-        with_lanes(r.dtype, r.dim, [&](auto l) {
-            constexpr int LPH = decltype(l)::value;
-            a.slot = slot_of(LPH, r.heads);
+        with_lanes<T>(r.dim, a.group, [&](auto l, auto g) {
+            constexpr int LPH = decltype(l)::value, GH = decltype(g)::value;
+            const int units = r.heads / GH;
+            a.slot = slot_of(LPH, units);
             const int block = a.slot / LPH;
-            k_neighbor_forward<T, LPH>
-                <<<dim3((unsigned)((r.list.n_sources + 3) / 4), (r.heads + block - 1) / block), 256,
-                   0, (hipStream_t)stream>>>(a);
+            k_neighbor_forward<T, LPH, GH>
+                <<<dim3((unsigned)((r.list.n_sources + 3) / 4), (units + block - 1) / block), 256, 0,
+                   (hipStream_t)stream>>>(a);
         });
     });
     return launched(err, err_len);
@@ -734,21 +764,21 @@ int tnr_neighbor_backward(const tnr_neighbor_attention* req, void* workspace,
     a.turn = (float*)((char*)workspace + need / 2);
     with_type(r.dtype, [&](auto t) {
         using T = decltype(t);
-        with_lanes(r.dtype, r.dim, [&](auto l) {
-            constexpr int LPH = decltype(l)::value;
-            a.slot = slot_of(LPH, r.heads);
+        with_lanes<T>(r.dim, a.group, [&](auto l, auto g) {
+            constexpr int LPH = decltype(l)::value, GH = decltype(g)::value;
+            a.slot = slot_of(LPH, r.heads / GH);
             if (r.list.n_sources > 0)
-                k_neighbor_dq<T, LPH>
+                k_neighbor_dq<T, LPH, GH>
                     <<<(unsigned)((r.list.n_sources + 3) / 4), 256, 0, st>>>(a);
             a.slot = slot_of(LPH, r.kv_heads);
             const int block = a.slot / LPH;
             if (r.list.n_targets > 0)
-                k_neighbor_dkv<T, LPH><<<dim3((unsigned)((r.list.n_targets + 3) / 4),
-                                              (r.kv_heads + block - 1) / block),
-                                         256, 0, st>>>(a);
+                k_neighbor_dkv<T, LPH, GH><<<dim3((unsigned)((r.list.n_targets + 3) / 4),
+                                                  (r.kv_heads + block - 1) / block),
+                                             256, 0, st>>>(a);
         });
     });
-    k_neighbor_slopes<<<r.heads, 256, 0, st>>>(a.turn, r.list.n_sources, r.grad_slopes);
+    k_slopes<<<r.heads, 1024, 0, st>>>(a.turn, r.list.n_sources, r.grad_slopes);
     return launched(err, err_len);
 }
 
