@@ -8,6 +8,9 @@ Flags that matter for parity and safety:
   -fno-gpu-flush-denormals-to-zero       IEEE denormals, like the CPU path
   -Xclang -target-feature -Xclang -packed-fp32-ops
                                          no packed FP32 instructions
+  -mllvm -amdgpu-mfma-vgpr-form=1        matrix products accumulate in vector
+                                         registers: sums that are rescaled
+                                         would move to and from the others
 """
 
 from __future__ import annotations
@@ -48,6 +51,7 @@ def command(output: str = OUTPUT, extra: list[str] | None = None) -> list[str]:
         "-ffp-contract=off",
         "-fno-gpu-flush-denormals-to-zero",
         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
+        "-mllvm", "-amdgpu-mfma-vgpr-form=1",
         "-I", os.path.join(ROOT, "include"),
         f'-DTNR_OFFLOAD_ARCH="{ARCH}"',
         *(extra or []),

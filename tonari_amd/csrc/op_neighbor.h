@@ -122,7 +122,7 @@ struct NeighborArgs {
     const float* out_full;  // the forward's output in 32 bits
     void *grad_q, *grad_k, *grad_v;
     float* grad_distances;
-    float* delta;  // [n_sources][heads]
+    float2* stat;  // [n_sources][heads]: log-sum (inf: no weight) and delta
     float* turn;   // [heads][n_sources]
 };
 
@@ -223,6 +223,33 @@ __device__ __forceinline__ const char* row_at(const char* base, int row, uint32_
     return base + (uint64_t)(uint32_t)row * bytes;
 }
 
+// 64 pairs of a source, one to a lane, and the next 64 on their way.  A lane
+// beyond the run holds its last pair.
+struct PairChunk {
+    int first, left;  // of the run's pairs; those from `first` on
+    int target, next_target;
+    float distance, next_distance;
+    __device__ __forceinline__ PairChunk(const NeighborArgs& a, int2 run)
+        : first(run.x - kWave), left(run.y - run.x + kWave), target(0), next_target(0),
+          distance(0.f), next_distance(0.f) {
+        fetch(a, run, run.x);
+        next(a, run);
+    }
+    __device__ __forceinline__ void fetch(const NeighborArgs& a, int2 run, int from) {
+        if (from >= run.y) return;
+        const int e = min(from + lane_of(), run.y - 1);
+        next_target = a.rows.target[e];
+        next_distance = a.distances[e];
+    }
+    __device__ __forceinline__ void next(const NeighborArgs& a, int2 run) {
+        first += kWave;
+        left -= kWave;
+        target = next_target;
+        distance = next_distance;
+        fetch(a, run, first + kWave);
+    }
+};
+
 // grid: (sources / 4, blocks of units).
 template <typename T, int LPH, int GH>
 __global__ __launch_bounds__(256) void k_neighbor_forward(const NeighborArgs a) {
@@ -256,18 +283,20 @@ __global__ __launch_bounds__(256) void k_neighbor_forward(const NeighborArgs a) 
         const uint32_t k_row = (uint32_t)(a.k_stride[0] * sizeof(T));
         const uint32_t v_row = (uint32_t)(a.v_stride[0] * sizeof(T));
         const int2 run = run_of(a.rows.sources, i);
-        // a pair beyond the run's end repeats its last one, with weight 0
-        const auto step = [&](int e0, auto whole) {
+        // The targets and distances of 64 pairs are loaded together, one to a lane,
+        // 64 pairs ahead.  A pair beyond the run's end repeats its last one, with
+        // weight 0.
+        PairChunk chunk(a, run);
+        const auto step = [&](int p0, auto whole) {
             Raw<T> kx[kAhead], vx[kAhead];
             float d[kAhead];
             bool in[kAhead];
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
-                int e = e0 + u * l.slots + l.slot;
-                in[u] = whole || e < run.y;
-                if (!whole) e = min(e, run.y - 1);
-                const int j = a.rows.target[e];
-                d[u] = a.distances[e];
+                const int p = p0 + u * l.slots + l.slot;
+                in[u] = whole || p < chunk.left;
+                const int j = __shfl(chunk.target, p);
+                d[u] = __shfl(chunk.distance, p);
                 kx[u] = Raw<T>::at(row_at<T>(k, j, k_row));
                 vx[u] = Raw<T>::at(row_at<T>(v, j, v_row));
             }
@@ -299,10 +328,12 @@ __global__ __launch_bounds__(256) void k_neighbor_forward(const NeighborArgs a) 
                 }
             }
         };
-        int e0 = run.x;
-        for (; e0 + l.slots * kAhead <= run.y; e0 += l.slots * kAhead)
-            step(e0, std::true_type{});
-        if (e0 < run.y) step(e0, std::false_type{});
+        for (; chunk.left > 0; chunk.next(a, run)) {
+            const int n = min(chunk.left, kWave), stride = l.slots * kAhead;
+            int p0 = 0;
+            for (; p0 + stride <= n; p0 += stride) step(p0, std::true_type{});
+            if (p0 < n) step(p0, std::false_type{});
+        }
         // the slots' sums, in the largest maximum's terms
 #pragma unroll
         for (int g = 0; g < GH; ++g) {
@@ -372,28 +403,29 @@ __global__ __launch_bounds__(256) void k_neighbor_dq(const NeighborArgs a) {
                 slope[g] = a.slopes[l.head + g];
             }
             delta[g] = head_sum<LPH>(delta[g]);
-            if (l.mine && l.c == 0 && l.slot == 0) a.delta[row + g] = delta[g];
+            if (l.mine && l.c == 0 && l.slot == 0) a.stat[row + g] = float2{lse[g], delta[g]};
 #pragma unroll
             for (int x = 0; x < VEC; ++x) acc[g][x] = 0.f;
         }
         const char* k = (const char*)((const T*)a.k + l.kv * a.k_stride[1] + l.c);
         const char* v = (const char*)((const T*)a.v + l.kv * a.v_stride[1] + l.c);
-        const auto step = [&](int e0, auto whole) {
+        PairChunk chunk(a, run);
+        const auto step = [&](int p0, auto whole) {
             Raw<T> kx[kAhead], vx[kAhead];
             float d[kAhead];
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
-                int e = e0 + u * l.slots + l.slot;
-                if (!whole) e = min(e, run.y - 1);
-                const int j = a.rows.target[e];
-                d[u] = a.distances[e];
+                const int p = p0 + u * l.slots + l.slot;
+                const int j = __shfl(chunk.target, p);
+                d[u] = __shfl(chunk.distance, p);
                 kx[u] = Raw<T>::at(row_at<T>(k, j, k_row));
                 vx[u] = Raw<T>::at(row_at<T>(v, j, v_row));
             }
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
-                const int e = e0 + u * l.slots + l.slot;
-                const bool in = whole || e < run.y;
+                const int p = p0 + u * l.slots + l.slot;
+                const bool in = whole || p < chunk.left;
+                const int e = chunk.first + p;
                 if (!whole && !in) kx[u] = Raw<T>{};
                 float push = 0.f;
 #pragma unroll
@@ -414,10 +446,12 @@ __global__ __launch_bounds__(256) void k_neighbor_dq(const NeighborArgs a) {
                     a.grad_distances[e] = first == 0 ? push : a.grad_distances[e] + push;
             }
         };
-        int e0 = run.x;
-        for (; e0 + l.slots * kAhead <= run.y; e0 += l.slots * kAhead)
-            step(e0, std::true_type{});
-        if (e0 < run.y) step(e0, std::false_type{});
+        for (; chunk.left > 0; chunk.next(a, run)) {
+            const int n = min(chunk.left, kWave), stride = l.slots * kAhead;
+            int p0 = 0;
+            for (; p0 + stride <= n; p0 += stride) step(p0, std::true_type{});
+            if (p0 < n) step(p0, std::false_type{});
+        }
 #pragma unroll
         for (int g = 0; g < GH; ++g) {
             turn[g] = join_lanes<sum_of>(turn[g], a.slot);
@@ -436,7 +470,7 @@ __global__ __launch_bounds__(256) void k_neighbor_dq(const NeighborArgs a) {
 // unit here is a key head; its query heads are taken GH at a time.
 template <typename T, int LPH, int GH>
 __global__ __launch_bounds__(256) void k_neighbor_dkv(const NeighborArgs a) {
-    constexpr int VEC = Raw<T>::kVec, kAhead = GH == 4 ? 1 : GH == 2 ? 2 : 4;
+    constexpr int VEC = Raw<T>::kVec, kAhead = GH == 1 ? 4 : 2;
     const int64_t j = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
     if (j >= a.n_targets) return;
     const int lane = lane_of(), slot = lane / a.slot, in_slot = lane % a.slot;
@@ -467,48 +501,65 @@ __global__ __launch_bounds__(256) void k_neighbor_dkv(const NeighborArgs a) {
             for (int g = 0; g < GH; ++g) slope2[g] = a.slopes[head + g] * kLog2e;
             const char* q = (const char*)((const T*)a.q + head * a.q_stride[1] + c);
             const char* go = (const char*)((const T*)a.grad_out + (int64_t)head * a.dim + c);
-            const auto step = [&](int p0, auto whole) {
-                Raw<T> qx[kAhead][GH], ox[kAhead][GH];
-                float d[kAhead], lse[kAhead][GH], delta[kAhead][GH];
-#pragma unroll
-                for (int u = 0; u < kAhead; ++u) {
-                    int at = p0 + u * slots + slot;
-                    if (!whole) at = min(at, run.y - 1);
-                    const int2 pair = a.rows.order[at];
-                    const char* qi = row_at<T>(q, pair.y, q_row);
-                    const char* oi = row_at<T>(go, pair.y, o_row);
-                    const int64_t row = (int64_t)pair.y * a.heads + head;
-                    d[u] = a.distances[pair.x];
-#pragma unroll
-                    for (int g = 0; g < GH; ++g) {
-                        qx[u][g] = Raw<T>::at(qi + g * q_head);
-                        ox[u][g] = Raw<T>::at(oi + g * o_head);
-                        lse[u][g] = a.lse[row + g];
-                        delta[u][g] = a.delta[row + g];
-                    }
-                }
-#pragma unroll
-                for (int u = 0; u < kAhead; ++u) {
-                    const bool in = whole || p0 + u * slots + slot < run.y;
-#pragma unroll
-                    for (int g = 0; g < GH; ++g) {
-                        float t;
-                        if (!whole && !in) qx[u][g] = ox[u][g] = Raw<T>{};
-                        const float dot = head_sum<LPH>(qx[u][g].dot(k, 0.f));
-                        const float dp = head_sum<LPH>(ox[u][g].dot(v, 0.f));
-                        const float s = fmaf(-slope2[g], d[u], capped_one(dot, a.rule, t));
-                        const bool any = in && lse[u][g] != -inf_of();
-                        const float p = any ? exp2_of(s - lse[u][g]) : 0.f;
-                        float dx = any ? p * (dp - delta[u][g]) : 0.f;
-                        if (a.rule.cap > 0.f) dx *= fmaf(-t, t, 1.f);
-                        qx[u][g].add(dx, dk);
-                        ox[u][g].add(p, dv);
-                    }
-                }
+            const char* stat = (const char*)(a.stat + head);
+            const uint32_t stat_row = a.heads * sizeof(float2);
+            // 64 pairs of the target, one to a lane, and the next 64 on their way
+            int2 pair{}, next_pair{};
+            float distance = 0.f, next_distance = 0.f;
+            const auto fetch = [&](int from) {
+                if (from >= run.y) return;
+                next_pair = a.rows.order[min(from + lane, run.y - 1)];
+                next_distance = a.distances[next_pair.x];
             };
-            int p0 = run.x;
-            for (; p0 + slots * kAhead <= run.y; p0 += slots * kAhead) step(p0, std::true_type{});
-            if (p0 < run.y) step(p0, std::false_type{});
+            fetch(run.x);
+            for (int from = run.x; from < run.y; from += kWave) {
+                pair = next_pair;
+                distance = next_distance;
+                fetch(from + kWave);
+                const int n = min(run.y - from, kWave);
+                const auto step = [&](int p0, auto whole) {
+                    Raw<T> qx[kAhead][GH], ox[kAhead][GH];
+                    float d[kAhead];
+                    float2 st[kAhead][GH];
+#pragma unroll
+                    for (int u = 0; u < kAhead; ++u) {
+                        const int p = p0 + u * slots + slot;
+                        const int i = __shfl(pair.y, p);
+                        d[u] = __shfl(distance, p);
+                        const char* qi = row_at<T>(q, i, q_row);
+                        const char* oi = row_at<T>(go, i, o_row);
+                        const float2* si = (const float2*)row_at<T>(stat, i, stat_row);
+#pragma unroll
+                        for (int g = 0; g < GH; ++g) {
+                            qx[u][g] = Raw<T>::at(qi + g * q_head);
+                            ox[u][g] = Raw<T>::at(oi + g * o_head);
+                            st[u][g] = si[g];
+                        }
+                    }
+#pragma unroll
+                    for (int u = 0; u < kAhead; ++u) {
+                        const bool in = whole || p0 + u * slots + slot < n;
+#pragma unroll
+                        for (int g = 0; g < GH; ++g) {
+                            float t;
+                            if (!whole && !in) qx[u][g] = ox[u][g] = Raw<T>{};
+                            const float dot = head_sum<LPH>(qx[u][g].dot(k, 0.f));
+                            const float dp = head_sum<LPH>(ox[u][g].dot(v, 0.f));
+                            const float s = fmaf(-slope2[g], d[u], capped_one(dot, a.rule, t));
+                            float p = exp2_of(s - st[u][g].x);
+                            if (!whole && !in) p = 0.f;
+                            float dx = p * (dp - st[u][g].y);
+                            if (a.rule.cap > 0.f) dx *= fmaf(-t, t, 1.f);
+                            qx[u][g].add(dx, dk);
+                            ox[u][g].add(p, dv);
+                        }
+                    }
+                };
+                const int stride = slots * kAhead;
+                int p0 = 0;
+                for (; p0 + stride <= n; p0 += stride) step(p0, std::true_type{});
+                if (p0 < n) step(p0, std::false_type{});
+            }
         }
 #pragma unroll
         for (int x = 0; x < VEC; ++x) {

@@ -203,13 +203,14 @@ struct Mat16 {
     struct Stage {
         static constexpr int kUnits = (kTile / 4) * (DP / 8);
         Frag x[4];
-        __device__ __forceinline__ void load(int unit, const T* base, int64_t stride, int rows,
+        __device__ __forceinline__ void load(int unit, const T* base, int stride, int rows,
                                              int dim) {
             const int r = 4 * (unit % (kTile / 4)), c = 8 * (unit / (kTile / 4));
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 x[i] = Frag{};
-                if (r + i < rows && c < dim) x[i] = *(const Frag*)(base + (r + i) * stride + c);
+                if (r + i < rows && c < dim)
+                    x[i] = *(const Frag*)(base + (uint32_t)((r + i) * stride + c));
             }
         }
         __device__ __forceinline__ void store(int unit, T* row, T* col) const {
@@ -305,14 +306,14 @@ struct Mat<float> {
     struct Stage {
         static constexpr int kUnits = (kTile / 4) * (DP / 4);
         Vec<float, 4> x[4];
-        __device__ __forceinline__ void load(int unit, const float* base, int64_t stride, int rows,
+        __device__ __forceinline__ void load(int unit, const float* base, int stride, int rows,
                                              int dim) {
             const int r = unit / (DP / 4), c = 4 * (unit % (DP / 4));
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 x[i] = Vec<float, 4>{};
                 if (r + 8 * i < rows && c < dim)
-                    x[i] = *(const Vec<float, 4>*)(base + (r + 8 * i) * stride + c);
+                    x[i] = *(const Vec<float, 4>*)(base + (uint32_t)((r + 8 * i) * stride + c));
             }
         }
         __device__ __forceinline__ void store(int unit, float* row, float*) const {
@@ -324,33 +325,52 @@ struct Mat<float> {
     static constexpr bool kSeparateCols = false;
 };
 
-// Two staged tensors of 32 rows; the workgroup's threads share the units.
+// Two staged tensors of 32 rows; the workgroup's threads share the units.  With
+// one unit each they are loaded a tile ahead, with more (few waves, wide heads)
+// when their tile is placed: their registers are worth more than the wait.
 template <typename T, int DP, int NW>
 struct StagePair {
     using S = typename Mat<T>::template Stage<DP>;
     static constexpr int kAll = 2 * S::kUnits, kThreads = NW * kWave;
     static constexpr int kEach = (kAll + kThreads - 1) / kThreads;
-    S s[kEach];
-    // the rows' addresses: base + row * stride
-    __device__ __forceinline__ void load(const T* a, int64_t a_stride, const T* b, int64_t b_stride,
-                                         int rows, int dim) {
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            const int u = threadIdx.x + i * kThreads;
-            if (u < S::kUnits)
-                s[i].load(u, a, a_stride, rows, dim);
-            else if (u < kAll)
-                s[i].load(u - S::kUnits, b, b_stride, rows, dim);
-        }
+    static constexpr bool kAhead = kEach == 1;
+    const T *a, *b;
+    int a_stride, b_stride, rows, dim;
+    S ahead;
+
+    __device__ __forceinline__ void load(S& s, int u) const {
+        if (u < S::kUnits)
+            s.load(u, a, a_stride, rows, dim);
+        else if (u < kAll)
+            s.load(u - S::kUnits, b, b_stride, rows, dim);
     }
-    __device__ __forceinline__ void store(T* a_row, T* a_col, T* b_row, T* b_col) const {
-#pragma unroll
+    static __device__ __forceinline__ void put(const S& s, int u, T* a_row, T* a_col, T* b_row,
+                                               T* b_col) {
+        if (u < S::kUnits)
+            s.store(u, a_row, a_col);
+        else if (u < kAll)
+            s.store(u - S::kUnits, b_row, b_col);
+    }
+    __device__ __forceinline__ void fetch(const T* a_, int a_stride_, const T* b_, int b_stride_,
+                                          int rows_, int dim_) {
+        a = a_;
+        b = b_;
+        a_stride = a_stride_;
+        b_stride = b_stride_;
+        rows = rows_;
+        dim = dim_;
+        if (kAhead) load(ahead, threadIdx.x);
+    }
+    __device__ __forceinline__ void place(T* a_row, T* a_col, T* b_row, T* b_col) const {
+        if (kAhead) {
+            put(ahead, threadIdx.x, a_row, a_col, b_row, b_col);
+            return;
+        }
+#pragma unroll 2
         for (int i = 0; i < kEach; ++i) {
-            const int u = threadIdx.x + i * kThreads;
-            if (u < S::kUnits)
-                s[i].store(u, a_row, a_col);
-            else if (u < kAll)
-                s[i].store(u - S::kUnits, b_row, b_col);
+            S s;
+            load(s, threadIdx.x + i * kThreads);
+            put(s, threadIdx.x + i * kThreads, a_row, a_col, b_row, b_col);
         }
     }
 };
@@ -374,43 +394,66 @@ __device__ __forceinline__ void store_channels(T* row, int dim, const f32x16 (&a
         }
 }
 
-// u log2(e) of 16 products; t = tanh where the gradient needs it.
-template <bool GRAD>
-__device__ __forceinline__ void capped(const f32x16& acc, const ScoreRule& rule, float (&u)[16],
-                                       float (&t)[GRAD ? 16 : 1]) {
-    if (rule.cap > 0.f) {
-        float top = 0.f;
+// Whether the tile's 16 products all lie where tanh needs no exp.
+template <bool CAP>
+__device__ __forceinline__ bool all_near(const f32x16& dot, const ScoreRule& rule) {
+    if (!CAP) return true;
+    float top = 0.f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            u[i] = acc[i] * rule.inv;
-            top = fmaxf(top, fabsf(u[i]));
-        }
-        if (__builtin_amdgcn_ballot_w64(!(top <= kTanhNear)) == 0) {
+    for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(dot[i]));
+    return __builtin_amdgcn_ballot_w64(!(top * rule.inv <= kTanhNear)) == 0;
+}
+// u log2(e) + shift of the products of run `run`, and what their gradients are
+// multiplied by.
+template <bool CAP>
+__device__ __forceinline__ void capped(const f32x16& dot, int run, const ScoreRule& rule, bool near,
+                                       float shift, float (&u)[4], float (&bend)[4]) {
+    if (!CAP) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) u[i] = tanh_near(u[i]);
-        } else {
+        for (int e = 0; e < 4; ++e) u[e] = fmaf(dot[4 * run + e], rule.scale2, shift);
+        return;
+    }
+    // (the empty asm keeps this a branch of the wave: one side only is computed)
+    if (near) {
+        asm volatile("");
 #pragma unroll
-            for (int i = 0; i < 16; ++i) u[i] = tanh_of(u[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            if (GRAD) t[i] = u[i];
-            u[i] *= rule.cap2;
-        }
+        for (int e = 0; e < 4; ++e) u[e] = tanh_near(dot[4 * run + e] * rule.inv);
     } else {
+        asm volatile("");
 #pragma unroll
-        for (int i = 0; i < 16; ++i) u[i] = acc[i] * rule.scale2;
+        for (int e = 0; e < 4; ++e) u[e] = tanh_of(dot[4 * run + e] * rule.inv);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        bend[e] = fmaf(-u[e], u[e], 1.f);
+        u[e] = fmaf(u[e], rule.cap2, shift);
     }
 }
 
+// Positions of a staged tile, by axes: a lane's 16 rows are 4 runs of 4.
+struct TilePositions {
+    alignas(16) float x[3][kTile];
+};
+__device__ __forceinline__ Vec<float, 4> four_of(const float* x, int run, int half) {
+    return *(const Vec<float, 4>*)(x + 8 * run + 4 * half);
+}
+
+// Waves that a SIMD is to hold, of 512 registers: the accumulators and rows of
+// one wave grow with the head dimension.
+template <typename T>
+constexpr int waves_held(int dp) {
+    return sizeof(T) == 4 ? (dp <= 32 ? 3 : dp <= 64 ? 2 : 1) : (dp <= 32 ? 4 : dp <= 64 ? 3 : 2);
+}
+
 // grid: (tiles, kv_heads * splits); NW waves of 32 query rows each.
-template <typename T, int DP, int NW>
-__global__ __launch_bounds__(NW* kWave) void k_structure_forward(const StructureArgs a) {
+template <typename T, int DP, int NW, bool CAP>
+__global__ __launch_bounds__(NW* kWave, waves_held<T>(DP)) void k_structure_forward(
+    const StructureArgs a) {
     using M = Mat<T>;
     using Row = typename M::template Row<DP>;
     __shared__ alignas(16) T k_rows[M::kRows(DP)];
     __shared__ alignas(16) T v_tile[M::kSeparateCols ? M::kCols(DP) : M::kRows(DP)];
-    __shared__ alignas(16) float4 x_k[kTile];
+    __shared__ TilePositions x_k;
 
     const StructureTile t = a.q_tiles[blockIdx.x];
     const int lane = lane_of(), half = lane / 32, wave = threadIdx.x / kWave;
@@ -439,6 +482,7 @@ __global__ __launch_bounds__(NW* kWave) void k_structure_forward(const Structure
 
     const int row = t.first + wave * kTile + lane % 32;
     const bool valid = row < rows;
+    const bool busy = t.first + wave * kTile < rows;  // a wave without rows only helps to stage
     const int query = t.q_lo + (valid ? row / g : 0), head = kv * g + (valid ? row % g : 0);
     Row qr;
     qr.load(valid ? (const T*)a.q + (int64_t)query * a.q_stride[0] + head * a.q_stride[1] : nullptr,
@@ -464,60 +508,86 @@ __global__ __launch_bounds__(NW* kWave) void k_structure_forward(const Structure
     float top = -inf_of(), sum = 0.f;
 
     StagePair<T, DP, NW> stage;
-    float4 xs{};
+    float xs[3];
     const auto fetch = [&](int tile) {
         const int k0 = tile * kTile, n = t.n_k - k0;
-        stage.load(kb + (int64_t)k0 * a.k_stride[0], a.k_stride[0],
-                   vb + (int64_t)k0 * a.v_stride[0], a.v_stride[0], n, a.dim);
-        if (threadIdx.x < kTile && (int)threadIdx.x < n) {
-            const float* p = xb + 3 * (int64_t)(k0 + threadIdx.x);
-            xs = float4{p[0], p[1], p[2], 0.f};
+        stage.fetch(kb + (int64_t)k0 * a.k_stride[0], (int)a.k_stride[0],
+                   vb + (int64_t)k0 * a.v_stride[0], (int)a.v_stride[0], n, a.dim);
+        if (threadIdx.x < kTile) {
+            const float* p = xb + 3 * (int64_t)(k0 + min((int)threadIdx.x, n - 1));
+#pragma unroll
+            for (int c = 0; c < 3; ++c) xs[c] = p[c];
         }
+    };
+    const auto place = [&] {
+        __syncthreads();
+        if constexpr (M::kSeparateCols)
+            stage.place(k_rows, nullptr, nullptr, v_tile);
+        else
+            stage.place(k_rows, nullptr, v_tile, nullptr);
+        if (threadIdx.x < kTile)
+#pragma unroll
+            for (int c = 0; c < 3; ++c) x_k.x[c][threadIdx.x] = xs[c];
+        __syncthreads();
+    };
+    // Weights are taken relative to `top`, the maximum when it was last set: it
+    // is set anew only where a score passes it by more than 2^8 (the row's sums
+    // then change their unit), so that most tiles neither subtract nor rescale.
+    const auto weigh = [&](int left) {
+        f32x16 dot{};
+        M::template rows<DP>(dot, k_rows, qr);
+        float s[16], unused[4];
+        const float ref = top == -inf_of() ? 0.f : top;
+        const bool near = all_near<CAP>(dot, a.rule);
+        float high = -inf_of();
+#pragma unroll
+        for (int run = 0; run < 4; ++run) {
+            const Vec<float, 4> x = four_of(x_k.x[0], run, half), y = four_of(x_k.x[1], run, half),
+                                z = four_of(x_k.x[2], run, half);
+            float u[4];
+            capped<CAP>(dot, run, a.rule, near, -ref, u, unused);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float dx = xq - x[e], dy = yq - y[e], dz = zq - z[e];
+                const float r = __builtin_amdgcn_sqrtf(fmaf(dx, dx, fmaf(dy, dy, dz * dz)));
+                s[4 * run + e] = fmaf(-slope2, r, u[e]);
+            }
+            if (left < kTile) {
+                asm volatile("");  // a branch: only a structure's last tile pays for the selects
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (8 * run + e >= left - 4 * half) s[4 * run + e] = -inf_of();
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) high = fmaxf(high, s[4 * run + e]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        high = max_halves(high);
+        const bool anew = high > 8.f || (top == -inf_of() && high > -inf_of());
+        if (__builtin_amdgcn_ballot_w64(anew) != 0) {
+            const float up = anew ? high : 0.f;
+            const float fade = exp2_of(-up);
+            top = anew ? ref + high : top;
+            sum *= fade;
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d) acc[d] *= fade;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] -= up;
+        }
+        float part[4] = {};
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            s[i] = exp2_of(s[i]);
+            part[i % 4] += s[i];
+        }
+        sum += (part[0] + part[1]) + (part[2] + part[3]);
+        M::template cols<DP>(acc, v_tile, s);
     };
     if (from < to) fetch(from);
     for (int tile = from; tile < to; ++tile) {
-        __syncthreads();
-        if constexpr (M::kSeparateCols)
-            stage.store(k_rows, nullptr, nullptr, v_tile);
-        else
-            stage.store(k_rows, nullptr, v_tile, nullptr);
-        if (threadIdx.x < kTile) x_k[threadIdx.x] = xs;
-        __syncthreads();
+        place();
         if (tile + 1 < to) fetch(tile + 1);
-
-        f32x16 dot{};
-        M::template rows<DP>(dot, k_rows, qr);
-        float s[16], unused[1];
-        capped<false>(dot, a.rule, s, unused);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const float4 x = x_k[row_of(i, half)];
-            const float dx = xq - x.x, dy = yq - x.y, dz = zq - x.z;
-            const float r = __builtin_amdgcn_sqrtf(fmaf(dx, dx, fmaf(dy, dy, dz * dz)));
-            s[i] = fmaf(-slope2, r, s[i]);
-        }
-        const int left = t.n_k - tile * kTile;
-        if (left < kTile)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = row_of(i, half) < left ? s[i] : -inf_of();
-        float high = s[0];
-#pragma unroll
-        for (int i = 1; i < 16; ++i) high = fmaxf(high, s[i]);
-        high = fmaxf(top, max_halves(high));
-        const float ref = high == -inf_of() ? 0.f : high;  // nothing but -inf so far
-        const float fade = exp2_of(top - ref);
-        top = high;
-        float part = 0.f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            s[i] = exp2_of(s[i] - ref);
-            part += s[i];
-        }
-        sum = fmaf(sum, fade, part);
-        if (__builtin_amdgcn_ballot_w64(fade != 1.f) != 0)
-#pragma unroll
-            for (int d = 0; d < DP / 32; ++d) acc[d] *= fade;
-        M::template cols<DP>(acc, v_tile, s);
+        if (busy) weigh(t.n_k - tile * kTile);
     }
     sum = sum_halves(sum);
     if (!valid) return;
@@ -553,16 +623,20 @@ __global__ __launch_bounds__(256) void k_structure_join(const StructureArgs a) {
     const int lane = lane_of();
     const int64_t step = rows * (a.dim + 2);
     const float* part = a.part + at * (a.dim + 2);
-    float top = -inf_of();
-    for (int s = 0; s < a.splits; ++s) top = fmaxf(top, part[s * step + a.dim]);
-    const float ref = top == -inf_of() ? 0.f : top;
-    float sum = 0.f, x0 = 0.f, x1 = 0.f;
+    // a lane for each split: its maximum and sum
+    const bool there = lane < a.splits;
+    const float high = there ? part[lane * step + a.dim] : -inf_of();
+    float sum = there ? part[lane * step + a.dim + 1] : 0.f;
+    const float top = join_lanes<max_of>(high, 1);
+    const float w = exp2_of(high - (top == -inf_of() ? 0.f : top));
+    sum = join_lanes<sum_of>(there ? sum * w : 0.f, 1);
+    float x0 = 0.f, x1 = 0.f;
+#pragma unroll 8
     for (int s = 0; s < a.splits; ++s) {
         const float* p = part + s * step;
-        const float w = exp2_of(p[a.dim] - ref);
-        sum = fmaf(w, p[a.dim + 1], sum);
-        if (lane < a.dim) x0 = fmaf(w, p[lane], x0);
-        if (lane + kWave < a.dim) x1 = fmaf(w, p[lane + kWave], x1);
+        const float ws = __shfl(w, s);
+        if (lane < a.dim) x0 = fmaf(ws, p[lane], x0);
+        if (lane + kWave < a.dim) x1 = fmaf(ws, p[lane + kWave], x1);
     }
     const int head = (int)(at / a.n_queries), query = (int)(at % a.n_queries);
     const float by = sum == 0.f ? 0.f : 1.f / sum;
@@ -570,7 +644,7 @@ __global__ __launch_bounds__(256) void k_structure_join(const StructureArgs a) {
     if (lane < a.dim) out[lane] = rounded<T>(x0 * by);
     if (lane + kWave < a.dim) out[lane + kWave] = rounded<T>(x1 * by);
     if (a.lse && lane == 0)
-        a.lse[at] = sum == 0.f ? -inf_of() : ref + __builtin_amdgcn_logf(sum);
+        a.lse[at] = sum == 0.f ? -inf_of() : top + __builtin_amdgcn_logf(sum);
 }
 
 }  // namespace op

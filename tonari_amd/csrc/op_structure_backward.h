@@ -51,14 +51,15 @@ __device__ __forceinline__ void finish_row(const StructureArgs& a, int head, int
 }
 
 // grid: (query tiles, kv_heads * splits).
-template <typename T, int DP, int NW>
-__global__ __launch_bounds__(NW* kWave) void k_structure_dq(const StructureArgs a) {
+template <typename T, int DP, int NW, bool CAP>
+__global__ __launch_bounds__(NW* kWave, waves_held<T>(DP <= 32 ? 64 : 2 * DP)) void k_structure_dq(
+    const StructureArgs a) {
     using M = Mat<T>;
     using Row = typename M::template Row<DP>;
     __shared__ alignas(16) T k_rows[M::kRows(DP)];
     __shared__ alignas(16) T k_cols[M::kSeparateCols ? M::kCols(DP) : 8];
     __shared__ alignas(16) T v_rows[M::kRows(DP)];
-    __shared__ alignas(16) float4 x_k[kTile];
+    __shared__ TilePositions x_k;
 
     const StructureTile t = a.q_tiles[blockIdx.x];
     const int lane = lane_of(), half = lane / 32, wave = threadIdx.x / kWave;
@@ -85,6 +86,7 @@ __global__ __launch_bounds__(NW* kWave) void k_structure_dq(const StructureArgs 
 
     const int row = t.first + wave * kTile + lane % 32;
     const bool valid = row < rows;
+    const bool busy = t.first + wave * kTile < rows;  // a wave without rows only helps to stage
     const int query = t.q_lo + (valid ? row / g : 0), head = kv * g + (valid ? row % g : 0);
     const int64_t at = (int64_t)head * a.n_queries + query;
     const int64_t flat = ((int64_t)query * a.heads + head) * a.dim;
@@ -130,57 +132,81 @@ __global__ __launch_bounds__(NW* kWave) void k_structure_dq(const StructureArgs 
     for (int i = 0; i < kRowSums; ++i) w[i] = 0.f;
 
     StagePair<T, DP, NW> stage;
-    float4 xs{};
+    float xs[3];
     const auto fetch = [&](int tile) {
         const int k0 = tile * kTile, n = t.n_k - k0;
-        stage.load(kb + (int64_t)k0 * a.k_stride[0], a.k_stride[0],
-                   vb + (int64_t)k0 * a.v_stride[0], a.v_stride[0], n, a.dim);
-        if (threadIdx.x < kTile && (int)threadIdx.x < n) {
-            const float* p = xb + 3 * (int64_t)(k0 + threadIdx.x);
-            xs = float4{p[0], p[1], p[2], 0.f};
+        stage.fetch(kb + (int64_t)k0 * a.k_stride[0], (int)a.k_stride[0],
+                   vb + (int64_t)k0 * a.v_stride[0], (int)a.v_stride[0], n, a.dim);
+        if (threadIdx.x < kTile) {
+            const float* p = xb + 3 * (int64_t)(k0 + min((int)threadIdx.x, n - 1));
+#pragma unroll
+            for (int c = 0; c < 3; ++c) xs[c] = p[c];
         }
     };
-    if (from < to) fetch(from);
-    for (int tile = from; tile < to; ++tile) {
+    const auto place = [&] {
         __syncthreads();
-        stage.store(k_rows, M::kSeparateCols ? k_cols : nullptr, v_rows, nullptr);
-        if (threadIdx.x < kTile) x_k[threadIdx.x] = xs;
+        stage.place(k_rows, M::kSeparateCols ? k_cols : nullptr, v_rows, nullptr);
+        if (threadIdx.x < kTile)
+#pragma unroll
+            for (int c = 0; c < 3; ++c) x_k.x[c][threadIdx.x] = xs[c];
         __syncthreads();
-        if (tile + 1 < to) fetch(tile + 1);
-
+    };
+    const auto push = [&](int left) {
         f32x16 dot{}, dp{};
         M::template rows<DP>(dot, k_rows, qr);
         M::template rows<DP>(dp, v_rows, dor);
-        float p[16], th[16];
-        capped<true>(dot, a.rule, p, th);
-        const int left = t.n_k - tile * kTile;
+        float p[16];
+        const bool near = all_near<CAP>(dot, a.rule);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const float4 x = x_k[row_of(i, half)];
-            const float dx = xq - x.x, dy = yq - x.y, dz = zq - x.z;
-            const float r = __builtin_amdgcn_sqrtf(fmaf(dx, dx, fmaf(dy, dy, dz * dz)));
-            float s = exp2_of(fmaf(-slope2, r, p[i]) - lse);
-            if (left < kTile && row_of(i, half) >= left) s = 0.f;
-            const float ds = s * (dp[i] - delta);
-            if (geometry) {
-                const float over = r > 0.f ? __builtin_amdgcn_rcpf(r) : 0.f;
-                const float wd = ds * over, wp = s * over;
-                w[0] += ds;
-                w[1] = fmaf(wd, dx, w[1]);
-                w[2] = fmaf(wd, dy, w[2]);
-                w[3] = fmaf(wd, dz, w[3]);
-                w[4] = fmaf(wp, dx, w[4]);
-                w[5] = fmaf(wp, dy, w[5]);
-                w[6] = fmaf(wp, dz, w[6]);
-                w[7] = fmaf(ds, r, w[7]);
-                w[8] = fmaf(s, r, w[8]);
+        for (int run = 0; run < 4; ++run) {
+            const Vec<float, 4> x = four_of(x_k.x[0], run, half), y = four_of(x_k.x[1], run, half),
+                                z = four_of(x_k.x[2], run, half);
+            float dx[4], dy[4], dz[4], r[4], s[4], u[4], bend[4];
+            capped<CAP>(dot, run, a.rule, near, -lse, u, bend);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                dx[e] = xq - x[e];
+                dy[e] = yq - y[e];
+                dz[e] = zq - z[e];
+                r[e] = __builtin_amdgcn_sqrtf(
+                    fmaf(dx[e], dx[e], fmaf(dy[e], dy[e], dz[e] * dz[e])));
+                s[e] = exp2_of(fmaf(-slope2, r[e], u[e]));
             }
-            p[i] = ds * unit;
-        }
-        if (a.rule.cap > 0.f)
+            if (left < kTile) {
+                asm volatile("");  // a branch: only a structure's last tile pays for the selects
 #pragma unroll
-            for (int i = 0; i < 16; ++i) p[i] *= fmaf(-th[i], th[i], 1.f);
+                for (int e = 0; e < 4; ++e)
+                    if (8 * run + e >= left - 4 * half) s[e] = 0.f;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int i = 4 * run + e;
+                const float ds = s[e] * (dp[i] - delta);
+                p[i] = CAP ? ds * bend[e] : ds;
+                if (kNarrow<T>) p[i] *= unit;
+                if (geometry) {
+                    const float over = r[e] > 0.f ? __builtin_amdgcn_rcpf(r[e]) : 0.f;
+                    const float wd = ds * over, wp = s[e] * over;
+                    w[0] += ds;
+                    w[1] = fmaf(wd, dx[e], w[1]);
+                    w[2] = fmaf(wd, dy[e], w[2]);
+                    w[3] = fmaf(wd, dz[e], w[3]);
+                    w[4] = fmaf(wp, dx[e], w[4]);
+                    w[5] = fmaf(wp, dy[e], w[5]);
+                    w[6] = fmaf(wp, dz[e], w[6]);
+                    w[7] = fmaf(ds, r[e], w[7]);
+                    w[8] = fmaf(s[e], r[e], w[8]);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
         M::template cols<DP>(acc, M::kSeparateCols ? k_cols : k_rows, p);
+    };
+    if (from < to) fetch(from);
+    for (int tile = from; tile < to; ++tile) {
+        place();
+        if (tile + 1 < to) fetch(tile + 1);
+        if (busy) push(t.n_k - tile * kTile);
     }
 #pragma unroll
     for (int i = 0; i < kRowSums; ++i) w[i] = sum_halves(w[i]);
@@ -216,6 +242,7 @@ __global__ __launch_bounds__(256) void k_structure_join_dq(const StructureArgs a
     const int64_t step = rows * (a.dim + kRowSums);
     const float* part = a.part + at * (a.dim + kRowSums);
     float x0 = 0.f, x1 = 0.f, w[kRowSums] = {};
+#pragma unroll 4
     for (int s = 0; s < a.splits; ++s) {
         const float* p = part + s * step;
         if (lane < a.dim) x0 += p[lane];
@@ -239,8 +266,10 @@ __global__ __launch_bounds__(256) void k_structure_join_dq(const StructureArgs a
 }
 
 // grid: (key tiles, kv_heads * k_splits); NW waves of 32 keys each.
-template <typename T, int DP, int NW>
-__global__ __launch_bounds__(NW* kWave) void k_structure_dkv(const StructureArgs a) {
+template <typename T, int DP, int NW, bool CAP>
+__global__ __launch_bounds__(NW* kWave, CAP ? (DP <= 64 && sizeof(T) == 2 ? 2 : 1)
+                                                  : waves_held<T>(DP <= 32 ? 64 : 2 * DP)) void
+k_structure_dkv(const StructureArgs a) {
     using M = Mat<T>;
     using Row = typename M::template Row<DP>;
     constexpr float kLift = kNarrow<T> ? 12.f : 0.f;
@@ -249,8 +278,8 @@ __global__ __launch_bounds__(NW* kWave) void k_structure_dkv(const StructureArgs
     __shared__ alignas(16) T o_rows[M::kRows(DP)];
     __shared__ alignas(16) T q_cols[M::kSeparateCols ? M::kCols(DP) : 8];
     __shared__ alignas(16) T o_cols[M::kSeparateCols ? M::kCols(DP) : 8];
-    __shared__ alignas(16) float4 x_q[kTile];   // position, largest |grad_out|
-    __shared__ alignas(16) float2 stat[kTile];  // log-sum, delta
+    __shared__ TilePositions x_q;
+    __shared__ alignas(16) float stat[3][kTile];  // log-sum, delta, largest |grad_out|
 
     const StructureTile t = a.k_tiles[blockIdx.x];
     const int lane = lane_of(), half = lane / 32, wave = threadIdx.x / kWave;
@@ -291,26 +320,24 @@ __global__ __launch_bounds__(NW* kWave) void k_structure_dkv(const StructureArgs
 
     const int per_head = (t.n_q + kTile - 1) / kTile, tiles = per_head * a.group;
     StagePair<T, DP, NW> stage;
-    float4 xs{};
-    float2 ss{};
+    float xs[3], ss[3];
     const auto fetch = [&](int tile) {
         const int head = kv * a.group + tile / per_head;
         const int q0 = (tile % per_head) * kTile, n = t.n_q - q0;
         const int64_t first = t.q_lo + q0;
-        stage.load((const T*)a.q + first * a.q_stride[0] + head * a.q_stride[1], a.q_stride[0],
+        stage.fetch((const T*)a.q + first * a.q_stride[0] + head * a.q_stride[1], (int)a.q_stride[0],
                    (const T*)a.grad_out + (first * a.heads + head) * a.dim,
-                   (int64_t)a.heads * a.dim, n, a.dim);
+                   a.heads * a.dim, n, a.dim);
         if (threadIdx.x < kTile) {
-            xs = float4{0.f, 0.f, 0.f, 0.f};
-            ss = float2{inf_of(), 0.f};
-            if ((int)threadIdx.x < n) {
-                const int64_t query = first + threadIdx.x;
-                const int64_t at = (int64_t)head * a.n_queries + query;
-                xs = float4{a.x_q[3 * query], a.x_q[3 * query + 1], a.x_q[3 * query + 2],
-                            a.row[2 * at + 1]};
-                ss = float2{a.lse[at], a.row[2 * at]};
-                if (ss.x == -inf_of()) ss.x = inf_of();
-            }
+            const bool in = (int)threadIdx.x < n;
+            const int64_t query = first + (in ? threadIdx.x : 0);
+            const int64_t at = (int64_t)head * a.n_queries + query;
+#pragma unroll
+            for (int c = 0; c < 3; ++c) xs[c] = a.x_q[3 * query + c];
+            ss[0] = in ? a.lse[at] : inf_of();  // no weight beyond the rows
+            if (ss[0] == -inf_of()) ss[0] = inf_of();
+            ss[1] = a.row[2 * at];
+            ss[2] = in ? a.row[2 * at + 1] : 0.f;
         }
     };
     const int each = (tiles + a.k_splits - 1) / a.k_splits;
@@ -318,45 +345,59 @@ __global__ __launch_bounds__(NW* kWave) void k_structure_dkv(const StructureArgs
     if (from < to) fetch(from);
     for (int tile = from; tile < to; ++tile) {
         __syncthreads();
-        stage.store(q_rows, M::kSeparateCols ? q_cols : nullptr, o_rows,
+        stage.place(q_rows, M::kSeparateCols ? q_cols : nullptr, o_rows,
                     M::kSeparateCols ? o_cols : nullptr);
-        if (threadIdx.x < kTile) {
-            x_q[threadIdx.x] = xs;
-            stat[threadIdx.x] = ss;
-        }
+        if (threadIdx.x < kTile)
+#pragma unroll
+            for (int c = 0; c < 3; ++c) {
+                x_q.x[c][threadIdx.x] = xs[c];
+                stat[c][threadIdx.x] = ss[c];
+            }
         __syncthreads();
         const float slope = a.slopes[kv * a.group + tile / per_head], slope2 = slope * kLog2e;
         if (tile + 1 < to) fetch(tile + 1);
 
+        if (t.first + wave * kTile >= t.n_k) continue;  // a wave without keys only helps to stage
+
         f32x16 dot{}, dp{};
         M::template rows<DP>(dot, q_rows, kr);
         M::template rows<DP>(dp, o_rows, vr);
-        float p[16], th[16], dx[16];
-        capped<true>(dot, a.rule, p, th);
+        float p[16], dx[16];
+        const bool near = all_near<CAP>(dot, a.rule);
         float tile_top = 0.f, ux = 0.f, uy = 0.f, uz = 0.f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const float4 x = x_q[row_of(i, half)];
-            const float2 st = stat[row_of(i, half)];
-            const float ex = x.x - xk, ey = x.y - yk, ez = x.z - zk;
-            const float r = __builtin_amdgcn_sqrtf(fmaf(ex, ex, fmaf(ey, ey, ez * ez)));
-            p[i] = exp2_of(fmaf(-slope2, r, p[i]) - st.x + kLift);
-            const float ds = p[i] * kLower * (dp[i] - st.y);
-            if (a.push_k) {
-                const float wd = ds * (r > 0.f ? __builtin_amdgcn_rcpf(r) : 0.f);
-                ux = fmaf(wd, ex, ux);
-                uy = fmaf(wd, ey, uy);
-                uz = fmaf(wd, ez, uz);
+        for (int run = 0; run < 4; ++run) {
+            const Vec<float, 4> x = four_of(x_q.x[0], run, half), y = four_of(x_q.x[1], run, half),
+                                z = four_of(x_q.x[2], run, half),
+                                lse = four_of(stat[0], run, half),
+                                delta = four_of(stat[1], run, half);
+            float u[4], bend[4];
+            capped<CAP>(dot, run, a.rule, near, kLift, u, bend);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int i = 4 * run + e;
+                const float ex = x[e] - xk, ey = y[e] - yk, ez = z[e] - zk;
+                const float r = __builtin_amdgcn_sqrtf(fmaf(ex, ex, fmaf(ey, ey, ez * ez)));
+                p[i] = exp2_of(fmaf(-slope2, r, u[e]) - lse[e]);
+                const float ds = (kNarrow<T> ? p[i] * kLower : p[i]) * (dp[i] - delta[e]);
+                if (a.push_k) {
+                    const float wd = ds * (r > 0.f ? __builtin_amdgcn_rcpf(r) : 0.f);
+                    ux = fmaf(wd, ex, ux);
+                    uy = fmaf(wd, ey, uy);
+                    uz = fmaf(wd, ez, uz);
+                }
+                dx[i] = CAP ? ds * bend[e] : ds;
             }
-            if (kNarrow<T>) tile_top = fmaxf(tile_top, x.w);
-            dx[i] = ds;
+            __builtin_amdgcn_sched_barrier(0);
+            if (kNarrow<T>) {
+                const Vec<float, 4> largest = four_of(stat[2], run, half);
+                tile_top = fmaxf(fmaxf(fmaxf(tile_top, largest[0]), largest[1]),
+                                 fmaxf(largest[2], largest[3]));
+            }
         }
         px = fmaf(slope, ux, px);
         py = fmaf(slope, uy, py);
         pz = fmaf(slope, uz, pz);
-        if (a.rule.cap > 0.f)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) dx[i] *= fmaf(-th[i], th[i], 1.f);
         if (kNarrow<T>) {
             tile_top = max_halves(tile_top);
             const int e = exponent_of(tile_top);

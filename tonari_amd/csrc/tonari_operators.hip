@@ -176,21 +176,24 @@ int check_heads(int32_t dtype, int32_t heads, int32_t kv_heads, int32_t dim, flo
     return TNR_OK;
 }
 
-// Rows are found by 32-bit strides in bytes.
+// Rows of a tile are found by 32-bit offsets.
+constexpr int64_t kMostStride = int64_t(1) << 24;
 bool aligned(const void* p, const int64_t (&stride)[2], int32_t dtype) {
     const int64_t unit = 16 / (int64_t)size_of(dtype);
     for (const int64_t s : stride)
-        if (s % unit != 0 || s < 0 || s >= (int64_t(1) << 29)) return false;
+        if (s % unit != 0 || s < 0 || s > kMostStride) return false;
     return (uintptr_t)p % 16 == 0;
 }
 
 // ------------------------------------------------------- structure attention
 
-// Waves of 32 rows in a workgroup: as many as the batch's structures fill.
-// They share the staged keys; a wave without rows only helps to stage.
+// Waves of 32 rows in a workgroup, which share the staged keys.  With long
+// structures four; with short ones two, of which fewer lie beyond a structure's
+// end: 1,024 molecules of 20 to 120 atoms take 73 us at two and 84 at four, a
+// cluster of 4,001 atoms 246 us at four and 286 at two (its queries' gradients).
 int waves_for(int64_t rows, int64_t structures) {
     const int64_t mean = structures > 0 ? rows / structures : 0;
-    return mean <= 32 ? 1 : mean <= 64 ? 2 : 4;
+    return mean <= 512 ? 2 : 4;
 }
 
 struct StructurePlan {
@@ -198,7 +201,7 @@ struct StructurePlan {
     int64_t q_tiles, k_tiles;
 };
 
-constexpr int64_t kSplitWaves = 4096;
+constexpr int64_t kSplitWaves = 3072;
 
 StructurePlan structure_plan(const tnr_structure_attention& r) {
     StructurePlan p{};
@@ -245,7 +248,7 @@ int check_structure(const tnr_structure_attention* r, bool backward, char* err, 
         return refuse(err, len, "required pointers are null");
     if (!aligned(r->q, r->q_stride, r->dtype) || !aligned(r->k, r->k_stride, r->dtype) ||
         !aligned(r->v, r->v_stride, r->dtype) || (uintptr_t)r->out % 16 != 0)
-        return refuse(err, len, "q, k, v and out must be aligned to 16 bytes, with strides below 2^29");
+        return refuse(err, len, "q, k, v and out must be aligned to 16 bytes, with strides up to 2^24");
     if (backward) {
         if ((r->n_queries > 0 && (!r->grad_out || !r->grad_q || !r->lse)) ||
             (r->n_keys > 0 && (!r->grad_k || !r->grad_v)))
@@ -343,13 +346,17 @@ void with_dim(int32_t dim, F&& f) {
         f(Int<128>{});
 }
 template <typename F>
-void with_waves(int waves, F&& f) {
-    if (waves == 1)
-        f(Int<1>{});
-    else if (waves == 2)
-        f(Int<2>{});
+void with_waves(int waves, bool cap, F&& f) {
+    const auto capped = [&](auto w) {
+        if (cap)
+            f(w, std::true_type{});
+        else
+            f(w, std::false_type{});
+    };
+    if (waves == 2)
+        capped(Int<2>{});
     else
-        f(Int<4>{});
+        capped(Int<4>{});
 }
 
 // -------------------------------------------------------- neighbor attention
@@ -410,7 +417,7 @@ int check_neighbor(const tnr_neighbor_attention* r, bool backward, char* err, si
         return refuse(err, len, "required pointers are null");
     if (!aligned(r->q, r->q_stride, r->dtype) || !aligned(r->k, r->k_stride, r->dtype) ||
         !aligned(r->v, r->v_stride, r->dtype) || (uintptr_t)r->out % 16 != 0)
-        return refuse(err, len, "q, k, v and out must be aligned to 16 bytes, with strides below 2^29");
+        return refuse(err, len, "q, k, v and out must be aligned to 16 bytes, with strides up to 2^24");
     if (backward) {
         if (!r->list.transpose) return refuse(err, len, "the backward needs the rows by target too");
         if ((r->list.n_sources > 0 && (!r->grad_out || !r->grad_q || !r->lse ||
@@ -594,9 +601,10 @@ int tnr_structure_forward(const tnr_structure_attention* req, void* workspace,
         using T = decltype(t);
         with_dim(r.dim, [&](auto d) {
             constexpr int DP = decltype(d)::value;
-            with_waves(p.q_waves, [&](auto w) {
+            with_waves(p.q_waves, r.softcap > 0.f, [&](auto w, auto c) {
                 constexpr int NW = decltype(w)::value;
-                k_structure_forward<T, DP, NW>
+                constexpr bool CAP = decltype(c)::value;
+                k_structure_forward<T, DP, NW, CAP>
                     <<<dim3((unsigned)p.q_tiles, r.kv_heads * p.splits), NW * kWave, 0, st>>>(a);
             });
         });
@@ -637,9 +645,10 @@ int tnr_structure_backward(const tnr_structure_attention* req, void* workspace,
         with_dim(r.dim, [&](auto d) {
             constexpr int DP = decltype(d)::value;
             if (r.n_queries > 0)
-                with_waves(p.q_waves, [&](auto w) {
+                with_waves(p.q_waves, r.softcap > 0.f, [&](auto w, auto c) {
                     constexpr int NW = decltype(w)::value;
-                    k_structure_dq<T, DP, NW>
+                constexpr bool CAP = decltype(c)::value;
+                    k_structure_dq<T, DP, NW, CAP>
                         <<<dim3((unsigned)p.q_tiles, r.kv_heads * p.splits), NW * kWave, 0, st>>>(
                             a);
                 });
@@ -647,9 +656,10 @@ int tnr_structure_backward(const tnr_structure_attention* req, void* workspace,
                 k_structure_join_dq<T>
                     <<<(unsigned)((r.n_queries * r.heads + 3) / 4), 256, 0, st>>>(a);
             if (r.n_keys > 0)
-                with_waves(p.k_waves, [&](auto w) {
+                with_waves(p.k_waves, r.softcap > 0.f, [&](auto w, auto c) {
                     constexpr int NW = decltype(w)::value;
-                    k_structure_dkv<T, DP, NW>
+                constexpr bool CAP = decltype(c)::value;
+                    k_structure_dkv<T, DP, NW, CAP>
                         <<<dim3((unsigned)p.k_tiles, r.kv_heads * p.k_splits), NW * kWave, 0,
                            st>>>(a);
                 });
@@ -747,7 +757,8 @@ int tnr_neighbor_forward(const tnr_neighbor_attention* req, void* stream, char* 
 
 size_t tnr_neighbor_backward_workspace_size(const tnr_neighbor_attention* req) {
     if (!req || req->heads < 1 || req->list.n_sources < 0) return 0;
-    return 2 * padded((size_t)req->list.n_sources * req->heads * 4);
+    const size_t rows = (size_t)req->list.n_sources * req->heads;
+    return padded(rows * sizeof(float2)) + padded(rows * sizeof(float));
 }
 
 int tnr_neighbor_backward(const tnr_neighbor_attention* req, void* workspace,
@@ -760,8 +771,9 @@ int tnr_neighbor_backward(const tnr_neighbor_attention* req, void* workspace,
         return refuse(err, err_len, "workspace is too small or not aligned to 256 bytes");
     const hipStream_t st = (hipStream_t)stream;
     NeighborArgs a = neighbor_args(r);
-    a.delta = (float*)workspace;
-    a.turn = (float*)((char*)workspace + need / 2);
+    a.stat = (float2*)workspace;
+    a.turn = (float*)((char*)workspace +
+                      padded((size_t)r.list.n_sources * r.heads * sizeof(float2)));
     with_type(r.dtype, [&](auto t) {
         using T = decltype(t);
         with_lanes<T>(r.dim, a.group, [&](auto l, auto g) {

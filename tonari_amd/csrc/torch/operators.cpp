@@ -49,7 +49,7 @@ Tensor laid(const Tensor& x) {
     const Tensor t = x.detach();
     const int64_t unit = 16 / t.element_size();
     if (t.numel() == 0) return t.contiguous();
-    const auto fits = [&](int64_t s) { return s % unit == 0 && s < (int64_t(1) << 29); };
+    const auto fits = [&](int64_t s) { return s % unit == 0 && s <= (int64_t(1) << 24); };
     if (t.stride(2) == 1 && fits(t.stride(0)) && fits(t.stride(1)) &&
         (uintptr_t)t.data_ptr() % 16 == 0)
         return t;
