@@ -51,23 +51,46 @@ inline NeighborRows neighbor_rows(void* base, int64_t pairs, int64_t sources, in
 
 // status and the runs are cleared before.  A source whose pairs do not lie
 // together finds its run taken.
+constexpr int kRowsEach = 4, kRowsBlock = 256 * kRowsEach;
 __global__ __launch_bounds__(256) void k_neighbor_rows(const int64_t* sources,
                                                        const int64_t* targets, int64_t n_pairs,
                                                        int64_t n_sources, int64_t n_targets,
                                                        NeighborRows r) {
-    int bad = 0;
-    for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < n_pairs;
-         e += (int64_t)gridDim.x * 256) {
-        const int64_t i = sources[e], j = targets[e];
-        const bool in = i >= 0 && i < n_sources && j >= 0 && j < n_targets;
-        bad |= !in;
-        r.target[e] = in ? (int32_t)j : 0;
-        if (!in) continue;
-        if (e == 0 || sources[e - 1] != i)
-            bad |= atomicExch(&r.sources[i].x, (int)e + 1) != 0;  // 0: none yet
-        if (e + 1 == n_pairs || sources[e + 1] != i) r.sources[i].y = (int)e + 1;
+    // a wave takes kRowsEach x 64 pairs that lie together, a lane one of each 64
+    const int lane = lane_of();
+    const int64_t base =
+        (int64_t)blockIdx.x * kRowsBlock + (threadIdx.x / kWave) * (kWave * kRowsEach) + lane;
+    int64_t i[kRowsEach], j[kRowsEach], edge = -1;
+#pragma unroll
+    for (int u = 0; u < kRowsEach; ++u) {
+        const int64_t e = base + u * kWave;
+        i[u] = e < n_pairs ? sources[e] : -1;
+        j[u] = e < n_pairs ? targets[e] : -1;
     }
-    if (__builtin_amdgcn_ballot_w64(bad != 0) != 0 && lane_of() == 0) atomicOr(r.status, 1);
+    // the sources before the wave's first pair and after its last
+    const int64_t out = lane == 0 ? base - 1 : base + (kRowsEach - 1) * kWave + 1;
+    if ((lane == 0 || lane == kWave - 1) && out >= 0 && out < n_pairs) edge = sources[out];
+    int bad = 0;
+#pragma unroll
+    for (int u = 0; u < kRowsEach; ++u) {
+        const int64_t e = base + u * kWave;
+        int64_t before = __shfl_up((long long)i[u], 1), after = __shfl_down((long long)i[u], 1);
+        const int64_t last = u > 0 ? __shfl((long long)i[u > 0 ? u - 1 : 0], kWave - 1) : edge;
+        const int64_t next = u + 1 < kRowsEach
+                                 ? __shfl((long long)i[u + 1 < kRowsEach ? u + 1 : u], 0)
+                                 : edge;
+        if (lane == 0) before = last;
+        if (lane == kWave - 1) after = next;
+        if (e >= n_pairs) continue;
+        const bool in = i[u] >= 0 && i[u] < n_sources && j[u] >= 0 && j[u] < n_targets;
+        bad |= !in;
+        r.target[e] = in ? (int32_t)j[u] : 0;
+        if (!in) continue;
+        if (e == 0 || before != i[u])
+            bad |= atomicExch(&r.sources[i[u]].x, (int)e + 1) != 0;  // 0: none yet
+        if (e + 1 == n_pairs || after != i[u]) r.sources[i[u]].y = (int)e + 1;
+    }
+    if (__builtin_amdgcn_ballot_w64(bad != 0) != 0 && lane == 0) atomicOr(r.status, 1);
 }
 
 struct PairKeys {
@@ -169,14 +192,38 @@ __device__ __forceinline__ float head_sum(float x) {
     return x;
 }
 
-// u log2(e) of one product, and tanh where there is a cap.
-__device__ __forceinline__ float capped_one(float dot, const ScoreRule& rule, float& t) {
-    t = 0.f;
-    if (rule.cap > 0.f) {
-        t = tanh_of(dot * rule.inv);
-        return t * rule.cap2;
+// u log2(e) of N products, and what their gradients are multiplied by.
+template <bool CAP, int N>
+__device__ __forceinline__ void capped_few(float (&u)[N], const ScoreRule& rule, float (&bend)[N]) {
+    if (!CAP) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            u[i] *= rule.scale2;
+            bend[i] = 1.f;
+        }
+        return;
     }
-    return dot * rule.scale2;
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        u[i] *= rule.inv;
+        top = fmaxf(top, fabsf(u[i]));
+    }
+    // (the empty asm keeps this a branch of the wave: one side only is computed)
+    if (__builtin_amdgcn_ballot_w64(!(top <= kTanhNear)) == 0) {
+        asm volatile("");
+#pragma unroll
+        for (int i = 0; i < N; ++i) u[i] = tanh_near(u[i]);
+    } else {
+        asm volatile("");
+#pragma unroll
+        for (int i = 0; i < N; ++i) u[i] = tanh_of(u[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        bend[i] = fmaf(-u[i], u[i], 1.f);
+        u[i] *= rule.cap2;
+    }
 }
 
 template <typename T>
@@ -251,9 +298,9 @@ struct PairChunk {
 };
 
 // grid: (sources / 4, blocks of units).
-template <typename T, int LPH, int GH>
+template <typename T, int LPH, int GH, bool CAP>
 __global__ __launch_bounds__(256) void k_neighbor_forward(const NeighborArgs a) {
-    constexpr int VEC = Raw<T>::kVec, kAhead = 4;
+    constexpr int VEC = Raw<T>::kVec, kAhead = GH == 1 ? 4 : 2;
     const int64_t i = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
     if (i >= a.n_sources) return;
     const Lane<T, LPH, GH> l(a, blockIdx.y * (a.slot / LPH));
@@ -306,11 +353,13 @@ __global__ __launch_bounds__(256) void k_neighbor_forward(const NeighborArgs a) 
                     if (!in[u]) vx[u] = Raw<T>{};
 #pragma unroll
             for (int g = 0; g < GH; ++g) {
-                float s[kAhead], high = top[g], t;
+                float s[kAhead], high = top[g], unused[kAhead];
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u) s[u] = head_sum<LPH>(q[g].dot(kx[u], 0.f));
+                capped_few<CAP>(s, a.rule, unused);
 #pragma unroll
                 for (int u = 0; u < kAhead; ++u) {
-                    const float dot = head_sum<LPH>(q[g].dot(kx[u], 0.f));
-                    s[u] = fmaf(-slope2[g], d[u], capped_one(dot, a.rule, t));
+                    s[u] = fmaf(-slope2[g], d[u], s[u]);
                     if (!whole && !in[u]) s[u] = -inf_of();
                     high = fmaxf(high, s[u]);
                 }
@@ -364,9 +413,9 @@ __global__ __launch_bounds__(256) void k_neighbor_forward(const NeighborArgs a) 
 // By sources: grad_q, grad_d, delta and the slopes' gradient by rows.  Blocks of
 // units that do not fit a wave follow one another in it, so that a pair's
 // grad_d is summed by one lane.
-template <typename T, int LPH, int GH>
+template <typename T, int LPH, int GH, bool CAP>
 __global__ __launch_bounds__(256) void k_neighbor_dq(const NeighborArgs a) {
-    constexpr int VEC = Raw<T>::kVec, kAhead = GH == 4 ? 2 : 4;
+    constexpr int VEC = Raw<T>::kVec, kAhead = GH == 1 ? 4 : GH == 2 ? 2 : 1;
     const int64_t i = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
     if (i >= a.n_sources) return;
     if (*a.rows.status != 0) {
@@ -427,17 +476,19 @@ __global__ __launch_bounds__(256) void k_neighbor_dq(const NeighborArgs a) {
                 const bool in = whole || p < chunk.left;
                 const int e = chunk.first + p;
                 if (!whole && !in) kx[u] = Raw<T>{};
-                float push = 0.f;
+                float push = 0.f, s[GH], dp[GH], bend[GH];
 #pragma unroll
                 for (int g = 0; g < GH; ++g) {
-                    float t;
-                    const float dot = head_sum<LPH>(q[g].dot(kx[u], 0.f));
-                    const float dp = head_sum<LPH>(go[g].dot(vx[u], 0.f));
-                    const float s =
-                        fmaf(-slope[g] * kLog2e, d[u], capped_one(dot, a.rule, t));
-                    float ds = exp2_of(s - lse[g]) * (dp - delta[g]);
+                    s[g] = head_sum<LPH>(q[g].dot(kx[u], 0.f));
+                    dp[g] = head_sum<LPH>(go[g].dot(vx[u], 0.f));
+                }
+                capped_few<CAP>(s, a.rule, bend);
+#pragma unroll
+                for (int g = 0; g < GH; ++g) {
+                    s[g] = fmaf(-slope[g] * kLog2e, d[u], s[g]);
+                    float ds = exp2_of(s[g] - lse[g]) * (dp[g] - delta[g]);
                     if (!l.mine || (!whole && !in)) ds = 0.f;
-                    kx[u].add(a.rule.cap > 0.f ? ds * fmaf(-t, t, 1.f) : ds, acc[g]);
+                    kx[u].add(CAP ? ds * bend[g] : ds, acc[g]);
                     turn[g] = fmaf(-ds, d[u], turn[g]);
                     push = fmaf(-slope[g], ds, push);
                 }
@@ -468,9 +519,9 @@ __global__ __launch_bounds__(256) void k_neighbor_dq(const NeighborArgs a) {
 
 // By targets: grad_k and grad_v.  grid: (targets / 4, blocks of key heads).  A
 // unit here is a key head; its query heads are taken GH at a time.
-template <typename T, int LPH, int GH>
+template <typename T, int LPH, int GH, bool CAP>
 __global__ __launch_bounds__(256) void k_neighbor_dkv(const NeighborArgs a) {
-    constexpr int VEC = Raw<T>::kVec, kAhead = GH == 1 ? 4 : 2;
+    constexpr int VEC = Raw<T>::kVec, kAhead = GH == 1 ? 4 : GH == 2 ? 2 : 1;
     const int64_t j = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
     if (j >= a.n_targets) return;
     const int lane = lane_of(), slot = lane / a.slot, in_slot = lane % a.slot;
@@ -539,17 +590,20 @@ __global__ __launch_bounds__(256) void k_neighbor_dkv(const NeighborArgs a) {
 #pragma unroll
                     for (int u = 0; u < kAhead; ++u) {
                         const bool in = whole || p0 + u * slots + slot < n;
+                        float s[GH], dp[GH], bend[GH];
 #pragma unroll
                         for (int g = 0; g < GH; ++g) {
-                            float t;
                             if (!whole && !in) qx[u][g] = ox[u][g] = Raw<T>{};
-                            const float dot = head_sum<LPH>(qx[u][g].dot(k, 0.f));
-                            const float dp = head_sum<LPH>(ox[u][g].dot(v, 0.f));
-                            const float s = fmaf(-slope2[g], d[u], capped_one(dot, a.rule, t));
-                            float p = exp2_of(s - st[u][g].x);
+                            s[g] = head_sum<LPH>(qx[u][g].dot(k, 0.f));
+                            dp[g] = head_sum<LPH>(ox[u][g].dot(v, 0.f));
+                        }
+                        capped_few<CAP>(s, a.rule, bend);
+#pragma unroll
+                        for (int g = 0; g < GH; ++g) {
+                            float p = exp2_of(fmaf(-slope2[g], d[u], s[g]) - st[u][g].x);
                             if (!whole && !in) p = 0.f;
-                            float dx = p * (dp - st[u][g].y);
-                            if (a.rule.cap > 0.f) dx *= fmaf(-t, t, 1.f);
+                            float dx = p * (dp[g] - st[u][g].y);
+                            if (CAP) dx *= bend[g];
                             qx[u][g].add(dx, dk);
                             ox[u][g].add(p, dv);
                         }

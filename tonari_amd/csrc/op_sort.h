@@ -41,9 +41,16 @@ inline SortPlan sort_plan(int64_t n_keys) {
     return p;
 }
 inline int64_t sort_tiles(int64_t n) { return (n + kSortTile - 1) / kSortTile; }
-// Counters and digit totals of a pass.
-inline size_t sort_scratch_bytes(int64_t n) {
-    return (size_t)(kSortRadix * (sort_tiles(n) + 1)) * sizeof(int32_t);
+__host__ __device__ inline int64_t sort_stride(int64_t tiles) { return (tiles + 3) / 4 * 4; }  // of a digit's counts
+inline size_t sort_count_bytes(int64_t n) {
+    return (size_t)kSortRadix * sort_stride(sort_tiles(n)) * sizeof(int32_t);
+}
+
+// Workgroups go to the 8 XCDs in turn: each XCD takes a run of tiles, so that
+// what neighbouring tiles write next to each other meets in one L2.
+__device__ __forceinline__ int64_t sort_tile_of(int64_t block, int64_t tiles) {
+    const int64_t each = tiles / 8, left = tiles % 8, xcd = block % 8, at = block / 8;
+    return xcd * each + (xcd < left ? xcd : left) + at;
 }
 
 // Keys and payloads of the first pass; later passes read what the one before
@@ -53,7 +60,7 @@ struct SortKeys {
     __device__ __forceinline__ int operator()(int64_t i) const { return key[i]; }
 };
 
-// counts[digit * tiles + tile]
+// counts[digit * stride + tile]
 template <typename Keys>
 __global__ __launch_bounds__(kSortThreads) void k_sort_count(Keys keys, int64_t n, SortPass pass,
                                                              int32_t* counts) {
@@ -61,15 +68,15 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_count(Keys keys, int64_t 
     const int radix = 1 << pass.bits;
     for (int d = threadIdx.x; d < radix; d += kSortThreads) hist[d] = 0;
     __syncthreads();
-    const int64_t base = (int64_t)blockIdx.x * kSortTile;
-#pragma unroll 4
+    const int64_t tile = sort_tile_of(blockIdx.x, gridDim.x), base = tile * kSortTile;
+#pragma unroll
     for (int r = 0; r < kSortRounds; ++r) {
         const int64_t i = base + r * kSortThreads + threadIdx.x;
         if (i < n) atomicAdd(&hist[(keys(i) >> pass.shift) & (radix - 1)], 1);
     }
     __syncthreads();
     for (int d = threadIdx.x; d < radix; d += kSortThreads)
-        counts[(int64_t)d * gridDim.x + blockIdx.x] = hist[d];
+        counts[(int64_t)d * sort_stride(gridDim.x) + tile] = hist[d];
 }
 
 __device__ __forceinline__ int sort_wave_scan(int x) {  // inclusive
@@ -87,13 +94,21 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_scan(int32_t* counts, int
                                                             int radix, int32_t* totals) {
     const int digit = blockIdx.x * kSortWaves + threadIdx.x / kWave;
     if (digit >= radix) return;
-    int32_t* at = counts + (int64_t)digit * tiles;
+    int32_t* at = counts + (int64_t)digit * sort_stride(tiles);
     int before = 0;
-    for (int64_t t = 0; t < tiles; t += kWave) {
-        const int64_t i = t + lane_of();
-        const int x = i < tiles ? at[i] : 0;
-        const int up = sort_wave_scan(x);
-        if (i < tiles) at[i] = before + up - x;
+    for (int64_t t = 0; t < tiles; t += 4 * kWave) {
+        const int64_t i = t + 4 * lane_of();
+        int4 x = i < tiles ? *(const int4*)(at + i) : int4{};  // (the counts end at a multiple of 4)
+        if (i + 1 >= tiles) x.y = 0;
+        if (i + 2 >= tiles) x.z = 0;
+        if (i + 3 >= tiles) x.w = 0;
+        const int sum = x.x + x.y + x.z + x.w, up = sort_wave_scan(sum);
+        int4 y;
+        y.x = before + up - sum;
+        y.y = y.x + x.x;
+        y.z = y.y + x.y;
+        y.w = y.z + x.z;
+        if (i < tiles) *(int4*)(at + i) = y;
         before += __shfl(up, kWave - 1);
     }
     if (lane_of() == 0) totals[digit] = before;
@@ -105,7 +120,6 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_move(Keys keys, int64_t n
                                                             const int32_t* counts,
                                                             const int32_t* totals, Put put) {
     __shared__ int32_t seen[kSortWaves][kSortRadix];
-    __shared__ int32_t first[kSortRadix];
     __shared__ int32_t wave_sum[kSortWaves];
     const int radix = 1 << pass.bits, lane = lane_of(), wave = threadIdx.x / kWave;
     for (int d = threadIdx.x; d < radix; d += kSortThreads)
@@ -113,7 +127,8 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_move(Keys keys, int64_t n
         for (int w = 0; w < kSortWaves; ++w) seen[w][d] = 0;
     __syncthreads();
     // a wave's items are consecutive, in rounds of 64
-    const int64_t base = (int64_t)blockIdx.x * kSortTile + wave * (kWave * kSortRounds);
+    const int64_t tile = sort_tile_of(blockIdx.x, gridDim.x);
+    const int64_t base = tile * kSortTile + wave * (kWave * kSortRounds);
     int key[kSortRounds], rank[kSortRounds];
 #pragma unroll
     for (int r = 0; r < kSortRounds; ++r) {
@@ -140,7 +155,7 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_move(Keys keys, int64_t n
         __builtin_amdgcn_wave_barrier();
     }
     __syncthreads();
-    // first[digit]: the digit's place in the whole output, plus this tile's share
+    // a digit's place in the whole output, and in it those of this tile's waves
     int carry = 0;
     for (int d0 = 0; d0 < radix; d0 += kSortThreads) {
         const int d = d0 + threadIdx.x;
@@ -155,7 +170,7 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_move(Keys keys, int64_t n
             all += wave_sum[w];
         }
         if (d < radix) {
-            int at = before + up - x + counts[(int64_t)d * gridDim.x + blockIdx.x];
+            int at = before + up - x + counts[(int64_t)d * sort_stride(gridDim.x) + tile];
 #pragma unroll
             for (int w = 0; w < kSortWaves; ++w) {
                 const int c = seen[w][d];

@@ -97,9 +97,10 @@ EmbeddingArgs embedding_args(const tnr_embedding& r) {
 }
 
 // Sorted atoms of a group: enough groups for the device, and no more than 256
-// atoms, whose partial rows are few beside them.
+// atoms, whose partial rows are few beside them.  1,048,576 rows of 128 floats:
+// 223 us at 256 atoms, which leaves two waves to a SIMD.
 int64_t embedding_each(int64_t n) {
-    const int64_t e = n / 4096;
+    const int64_t e = n / 16384;
     return e < 16 ? 16 : e > 256 ? 256 : e;
 }
 
@@ -116,9 +117,9 @@ EmbeddingSpace embedding_space(const tnr_embedding& r, void* base) {
         at += padded(bytes);
         return p;
     };
-    const int64_t tiles = sort_tiles(r.n_atoms), each = embedding_each(r.n_atoms);
+    const int64_t each = embedding_each(r.n_atoms);
     EmbeddingSpace s{};
-    s.counts = (int32_t*)part((size_t)kSortRadix * tiles * 4);
+    s.counts = (int32_t*)part(sort_count_bytes(r.n_atoms));
     s.totals = (int32_t*)part((size_t)kSortRadix * 4);
     for (int i = 0; i < 2; ++i) {
         s.key[i] = (int32_t*)part((size_t)r.n_atoms * 4);
@@ -390,7 +391,7 @@ RowsSpace rows_space(const tnr_neighbor_list& l, void* base) {
     };
     RowsSpace s{};
     if (!l.transpose || l.n_pairs == 0) return s;
-    s.counts = (int32_t*)part((size_t)kSortRadix * sort_tiles(l.n_pairs) * 4);
+    s.counts = (int32_t*)part(sort_count_bytes(l.n_pairs));
     s.totals = (int32_t*)part((size_t)kSortRadix * 4);
     s.key[0] = (int32_t*)part((size_t)l.n_pairs * 4);
     if (sort_plan(l.n_targets).passes > 1) {
@@ -468,15 +469,21 @@ NeighborArgs neighbor_args(const tnr_neighbor_attention& r) {
 // Lanes of 16 bytes that make a head, a power of two (types of 16 bits fill 16 at
 // most), and the query heads that one lane takes.
 template <typename T, typename F>
-void with_lanes(int32_t dim, int group, F&& f) {
+void with_lanes(int32_t dim, int group, bool cap, F&& f) {
     const int units = (int)(dim * sizeof(T) / 16);
+    const auto capped = [&](auto lanes, auto of) {
+        if (cap)
+            f(lanes, of, std::true_type{});
+        else
+            f(lanes, of, std::false_type{});
+    };
     const auto heads = [&](auto lanes) {
         if (group % 4 == 0)
-            f(lanes, Int<4>{});
+            capped(lanes, Int<4>{});
         else if (group % 2 == 0)
-            f(lanes, Int<2>{});
+            capped(lanes, Int<2>{});
         else
-            f(lanes, Int<1>{});
+            capped(lanes, Int<1>{});
     };
     if (units <= 1)
         heads(Int<1>{});
@@ -569,8 +576,12 @@ int tnr_embedding_backward(const tnr_embedding* req, void* workspace, size_t wor
                     k_embedding_runs<T, VEC>
                         <<<dim3((unsigned)((groups + in_block - 1) / in_block), y), 256, 0, st>>>(
                             a, runs, lanes);
+                // few lanes a row: a frequent species has thousands of partial rows
+                const int few = lanes < 8 ? lanes : 8;
                 k_embedding_join<T, VEC>
-                    <<<dim3((unsigned)r.n_species, y), 256, 0, st>>>(a, runs, lanes);
+                    <<<dim3((unsigned)r.n_species,
+                            (unsigned)((r.channels + few * VEC - 1) / (few * VEC))),
+                       256, 0, st>>>(a, runs, few);
             }
         });
     });
@@ -707,8 +718,7 @@ int tnr_neighbor_rows(const tnr_neighbor_list* list, void* workspace, size_t wor
     // status and the runs, which lie at the front
     zero(rows.status, (char*)rows.target - (char*)rows.status, st);
     if (l.n_pairs > 0) {
-        const int64_t blocks = (l.n_pairs + 1023) / 1024;
-        k_neighbor_rows<<<(unsigned)(blocks < 8192 ? blocks : 8192), 256, 0, st>>>(
+        k_neighbor_rows<<<(unsigned)((l.n_pairs + kRowsBlock - 1) / kRowsBlock), 256, 0, st>>>(
             l.sources, l.targets, l.n_pairs, l.n_sources, l.n_targets, rows);
         if (l.transpose) {
             const SortPlan plan = sort_plan(l.n_targets);
@@ -742,12 +752,13 @@ int tnr_neighbor_forward(const tnr_neighbor_attention* req, void* stream, char* 
     NeighborArgs a = neighbor_args(r);
     with_type(r.dtype, [&](auto t) {
         using T = decltype(t);
-        with_lanes<T>(r.dim, a.group, [&](auto l, auto g) {
+        with_lanes<T>(r.dim, a.group, r.softcap > 0.f, [&](auto l, auto g, auto c) {
             constexpr int LPH = decltype(l)::value, GH = decltype(g)::value;
+            constexpr bool CAP = decltype(c)::value;
             const int units = r.heads / GH;
             a.slot = slot_of(LPH, units);
             const int block = a.slot / LPH;
-            k_neighbor_forward<T, LPH, GH>
+            k_neighbor_forward<T, LPH, GH, CAP>
                 <<<dim3((unsigned)((r.list.n_sources + 3) / 4), (units + block - 1) / block), 256, 0,
                    (hipStream_t)stream>>>(a);
         });
@@ -776,16 +787,17 @@ int tnr_neighbor_backward(const tnr_neighbor_attention* req, void* workspace,
                       padded((size_t)r.list.n_sources * r.heads * sizeof(float2)));
     with_type(r.dtype, [&](auto t) {
         using T = decltype(t);
-        with_lanes<T>(r.dim, a.group, [&](auto l, auto g) {
+        with_lanes<T>(r.dim, a.group, r.softcap > 0.f, [&](auto l, auto g, auto c) {
             constexpr int LPH = decltype(l)::value, GH = decltype(g)::value;
+            constexpr bool CAP = decltype(c)::value;
             a.slot = slot_of(LPH, r.heads / GH);
             if (r.list.n_sources > 0)
-                k_neighbor_dq<T, LPH, GH>
+                k_neighbor_dq<T, LPH, GH, CAP>
                     <<<(unsigned)((r.list.n_sources + 3) / 4), 256, 0, st>>>(a);
             a.slot = slot_of(LPH, r.kv_heads);
             const int block = a.slot / LPH;
             if (r.list.n_targets > 0)
-                k_neighbor_dkv<T, LPH, GH><<<dim3((unsigned)((r.list.n_targets + 3) / 4),
+                k_neighbor_dkv<T, LPH, GH, CAP><<<dim3((unsigned)((r.list.n_targets + 3) / 4),
                                                   (r.kv_heads + block - 1) / block),
                                              256, 0, st>>>(a);
         });
