@@ -110,17 +110,27 @@ __global__ __launch_bounds__(256) void k_embedding_runs(const EmbeddingArgs a, c
         }
     };
     constexpr int kAhead = 8;
+    int next_key[kAhead], next_atom[kAhead];
+    const auto look = [&](int64_t p0) {
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            const int64_t p = min(p0 + j, to - 1);
+            next_key[j] = r.key[p];
+            next_atom[j] = r.atom[p];
+        }
+    };
+    look(from);
     for (int64_t p0 = from; p0 < to; p0 += kAhead) {
         float x[kAhead][VEC];
         int key[kAhead];
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
-            const int64_t p = min(p0 + j, to - 1);
-            key[j] = r.key[p];
+            key[j] = next_key[j];
             if (mine)
-                load_floats<T, VEC>((const T*)a.grad_out + (int64_t)r.atom[p] * a.channels + c,
+                load_floats<T, VEC>((const T*)a.grad_out + (int64_t)next_atom[j] * a.channels + c,
                                     x[j]);
         }
+        look(p0 + kAhead);
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
             if (p0 + j >= to) break;

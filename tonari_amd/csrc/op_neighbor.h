@@ -192,13 +192,30 @@ __device__ __forceinline__ float head_sum(float x) {
     return x;
 }
 
-// u log2(e) of N products, and what their gradients are multiplied by.
+// Sum over the heads of a slot of what all lanes of a head hold, in all of them.
+template <int LPH>
+__device__ __forceinline__ float slot_sum(float x, int slot) {
+    if (LPH <= 1 && slot > 1) x += dpp_of<0xb1>(x);
+    if (LPH <= 2 && slot > 2) x += dpp_of<0x4e>(x);
+    if (LPH <= 4 && slot > 4) x += dpp_of<0x141>(x);
+    if (LPH <= 8 && slot > 8) x += dpp_of<0x140>(x);
+    if (LPH <= 16 && slot > 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x),
+                                                        false, false);
+        x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    if (slot > 32) x = sum_halves(x);
+    return x;
+}
+
+// u log2(e) + shift of N products, and what their gradients are multiplied by.
 template <bool CAP, int N>
-__device__ __forceinline__ void capped_few(float (&u)[N], const ScoreRule& rule, float (&bend)[N]) {
+__device__ __forceinline__ void capped_few(float (&u)[N], const ScoreRule& rule, float shift,
+                                           float (&bend)[N]) {
     if (!CAP) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            u[i] *= rule.scale2;
+            u[i] = fmaf(u[i], rule.scale2, shift);
             bend[i] = 1.f;
         }
         return;
@@ -222,7 +239,7 @@ __device__ __forceinline__ void capped_few(float (&u)[N], const ScoreRule& rule,
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         bend[i] = fmaf(-u[i], u[i], 1.f);
-        u[i] *= rule.cap2;
+        u[i] = fmaf(u[i], rule.cap2, shift);
     }
 }
 
@@ -270,6 +287,9 @@ __device__ __forceinline__ const char* row_at(const char* base, int row, uint32_
     return base + (uint64_t)(uint32_t)row * bytes;
 }
 
+// Waves that a SIMD is to hold: the gather lives by what is in flight.
+constexpr int kHeld = 4, kHeldBack = 3;
+
 // 64 pairs of a source, one to a lane, and the next 64 on their way.  A lane
 // beyond the run holds its last pair.
 struct PairChunk {
@@ -299,7 +319,7 @@ struct PairChunk {
 
 // grid: (sources / 4, blocks of units).
 template <typename T, int LPH, int GH, bool CAP>
-__global__ __launch_bounds__(256) void k_neighbor_forward(const NeighborArgs a) {
+__global__ __launch_bounds__(256, kHeld) void k_neighbor_forward(const NeighborArgs a) {
     constexpr int VEC = Raw<T>::kVec, kAhead = GH == 1 ? 4 : 2;
     const int64_t i = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
     if (i >= a.n_sources) return;
@@ -351,31 +371,48 @@ __global__ __launch_bounds__(256) void k_neighbor_forward(const NeighborArgs a) 
 #pragma unroll
                 for (int u = 0; u < kAhead; ++u)
                     if (!in[u]) vx[u] = Raw<T>{};
+            // weights relative to the slot's maximum when it was last set, which
+            // is set anew where a score passes it by more than 2^8
+            float s[GH][kAhead], high[GH], unused[kAhead];
+            bool anew = false;
 #pragma unroll
             for (int g = 0; g < GH; ++g) {
-                float s[kAhead], high = top[g], unused[kAhead];
 #pragma unroll
-                for (int u = 0; u < kAhead; ++u) s[u] = head_sum<LPH>(q[g].dot(kx[u], 0.f));
-                capped_few<CAP>(s, a.rule, unused);
+                for (int u = 0; u < kAhead; ++u) s[g][u] = head_sum<LPH>(q[g].dot(kx[u], 0.f));
+                const float ref = top[g] == -inf_of() ? 0.f : top[g];
+                capped_few<CAP>(s[g], a.rule, -ref, unused);
+                high[g] = -inf_of();
 #pragma unroll
                 for (int u = 0; u < kAhead; ++u) {
-                    s[u] = fmaf(-slope2[g], d[u], s[u]);
-                    if (!whole && !in[u]) s[u] = -inf_of();
-                    high = fmaxf(high, s[u]);
+                    s[g][u] = fmaf(-slope2[g], d[u], s[g][u]);
+                    if (!whole && !in[u]) s[g][u] = -inf_of();
+                    high[g] = fmaxf(high[g], s[g][u]);
                 }
-                const float ref = high == -inf_of() ? 0.f : high;
-                const float fade = exp2_of(top[g] - ref);
-                top[g] = high;
-                sum[g] *= fade;
+                anew |= high[g] > 8.f || (top[g] == -inf_of() && high[g] > -inf_of());
+            }
+            if (__builtin_amdgcn_ballot_w64(anew) != 0) {
+                asm volatile("");
 #pragma unroll
-                for (int x = 0; x < VEC; ++x) acc[g][x] *= fade;
+                for (int g = 0; g < GH; ++g) {
+                    const bool first = top[g] == -inf_of();
+                    const bool move = first ? high[g] > -inf_of() : high[g] > 0.f;
+                    const float up = move ? high[g] : 0.f, fade = exp2_of(-up);
+                    if (move) top[g] = (first ? 0.f : top[g]) + high[g];
+                    sum[g] *= fade;
+#pragma unroll
+                    for (int x = 0; x < VEC; ++x) acc[g][x] *= fade;
+#pragma unroll
+                    for (int u = 0; u < kAhead; ++u) s[g][u] -= up;
+                }
+            }
+#pragma unroll
+            for (int g = 0; g < GH; ++g)
 #pragma unroll
                 for (int u = 0; u < kAhead; ++u) {
-                    const float p = exp2_of(s[u] - ref);
+                    const float p = exp2_of(s[g][u]);
                     sum[g] += p;
                     vx[u].add(p, acc[g]);
                 }
-            }
         };
         for (; chunk.left > 0; chunk.next(a, run)) {
             const int n = min(chunk.left, kWave), stride = l.slots * kAhead;
@@ -414,7 +451,7 @@ __global__ __launch_bounds__(256) void k_neighbor_forward(const NeighborArgs a) 
 // units that do not fit a wave follow one another in it, so that a pair's
 // grad_d is summed by one lane.
 template <typename T, int LPH, int GH, bool CAP>
-__global__ __launch_bounds__(256) void k_neighbor_dq(const NeighborArgs a) {
+__global__ __launch_bounds__(256, kHeldBack) void k_neighbor_dq(const NeighborArgs a) {
     constexpr int VEC = Raw<T>::kVec, kAhead = GH == 1 ? 4 : GH == 2 ? 2 : 1;
     const int64_t i = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
     if (i >= a.n_sources) return;
@@ -459,6 +496,9 @@ __global__ __launch_bounds__(256) void k_neighbor_dq(const NeighborArgs a) {
         const char* k = (const char*)((const T*)a.k + l.kv * a.k_stride[1] + l.c);
         const char* v = (const char*)((const T*)a.v + l.kv * a.v_stride[1] + l.c);
         PairChunk chunk(a, run);
+        // The sum of ds over a row is 0, so the slope's gradient may count
+        // distances from any one of them: what they share cancels exactly.
+        const float near = __shfl(chunk.distance, 0);
         const auto step = [&](int p0, auto whole) {
             Raw<T> kx[kAhead], vx[kAhead];
             float d[kAhead];
@@ -482,17 +522,17 @@ __global__ __launch_bounds__(256) void k_neighbor_dq(const NeighborArgs a) {
                     s[g] = head_sum<LPH>(q[g].dot(kx[u], 0.f));
                     dp[g] = head_sum<LPH>(go[g].dot(vx[u], 0.f));
                 }
-                capped_few<CAP>(s, a.rule, bend);
+                capped_few<CAP>(s, a.rule, 0.f, bend);
 #pragma unroll
                 for (int g = 0; g < GH; ++g) {
                     s[g] = fmaf(-slope[g] * kLog2e, d[u], s[g]);
                     float ds = exp2_of(s[g] - lse[g]) * (dp[g] - delta[g]);
                     if (!l.mine || (!whole && !in)) ds = 0.f;
                     kx[u].add(CAP ? ds * bend[g] : ds, acc[g]);
-                    turn[g] = fmaf(-ds, d[u], turn[g]);
+                    turn[g] = fmaf(-ds, d[u] - near, turn[g]);
                     push = fmaf(-slope[g], ds, push);
                 }
-                for (int w = LPH; w < a.slot; w <<= 1) push += __shfl_xor(push, w);
+                push = slot_sum<LPH>(push, a.slot);
                 if (in && l.in_slot == 0)
                     a.grad_distances[e] = first == 0 ? push : a.grad_distances[e] + push;
             }
@@ -520,7 +560,7 @@ __global__ __launch_bounds__(256) void k_neighbor_dq(const NeighborArgs a) {
 // By targets: grad_k and grad_v.  grid: (targets / 4, blocks of key heads).  A
 // unit here is a key head; its query heads are taken GH at a time.
 template <typename T, int LPH, int GH, bool CAP>
-__global__ __launch_bounds__(256) void k_neighbor_dkv(const NeighborArgs a) {
+__global__ __launch_bounds__(256, kHeldBack) void k_neighbor_dkv(const NeighborArgs a) {
     constexpr int VEC = Raw<T>::kVec, kAhead = GH == 1 ? 4 : GH == 2 ? 2 : 1;
     const int64_t j = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
     if (j >= a.n_targets) return;
@@ -597,7 +637,7 @@ __global__ __launch_bounds__(256) void k_neighbor_dkv(const NeighborArgs a) {
                             s[g] = head_sum<LPH>(qx[u][g].dot(k, 0.f));
                             dp[g] = head_sum<LPH>(ox[u][g].dot(v, 0.f));
                         }
-                        capped_few<CAP>(s, a.rule, bend);
+                        capped_few<CAP>(s, a.rule, 0.f, bend);
 #pragma unroll
                         for (int g = 0; g < GH; ++g) {
                             float p = exp2_of(fmaf(-slope2[g], d[u], s[g]) - st[u][g].x);
