@@ -49,6 +49,14 @@ __device__ __forceinline__ float max_halves(float x) {
     return fmaxf(h.low, h.high);
 }
 
+// Workgroups go to the 8 XCDs in turn; in this order each XCD takes a run of
+// the work, so that what neighbours share, or write next to each other, meets
+// in one L2.
+__device__ __forceinline__ int64_t xcd_order(int64_t block, int64_t blocks) {
+    const int64_t each = blocks / 8, left = blocks % 8, xcd = block % 8, at = block / 8;
+    return xcd * each + (xcd < left ? xcd : left) + at;
+}
+
 template <int CTRL>
 __device__ __forceinline__ float dpp_of(float x) {
     return __int_as_float(

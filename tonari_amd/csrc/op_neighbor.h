@@ -321,7 +321,7 @@ struct PairChunk {
 template <typename T, int LPH, int GH, bool CAP>
 __global__ __launch_bounds__(256, kHeld) void k_neighbor_forward(const NeighborArgs a) {
     constexpr int VEC = Raw<T>::kVec, kAhead = GH == 1 ? 4 : 2;
-    const int64_t i = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
+    const int64_t i = xcd_order(blockIdx.x, gridDim.x) * 4 + threadIdx.x / kWave;
     if (i >= a.n_sources) return;
     const Lane<T, LPH, GH> l(a, blockIdx.y * (a.slot / LPH));
     const int64_t row = i * a.heads + l.head;
@@ -453,7 +453,7 @@ __global__ __launch_bounds__(256, kHeld) void k_neighbor_forward(const NeighborA
 template <typename T, int LPH, int GH, bool CAP>
 __global__ __launch_bounds__(256, kHeldBack) void k_neighbor_dq(const NeighborArgs a) {
     constexpr int VEC = Raw<T>::kVec, kAhead = GH == 1 ? 4 : GH == 2 ? 2 : 1;
-    const int64_t i = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
+    const int64_t i = xcd_order(blockIdx.x, gridDim.x) * 4 + threadIdx.x / kWave;
     if (i >= a.n_sources) return;
     if (*a.rows.status != 0) {
         const int lane = lane_of();
@@ -562,7 +562,7 @@ __global__ __launch_bounds__(256, kHeldBack) void k_neighbor_dq(const NeighborAr
 template <typename T, int LPH, int GH, bool CAP>
 __global__ __launch_bounds__(256, kHeldBack) void k_neighbor_dkv(const NeighborArgs a) {
     constexpr int VEC = Raw<T>::kVec, kAhead = GH == 1 ? 4 : GH == 2 ? 2 : 1;
-    const int64_t j = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
+    const int64_t j = xcd_order(blockIdx.x, gridDim.x) * 4 + threadIdx.x / kWave;
     if (j >= a.n_targets) return;
     const int lane = lane_of(), slot = lane / a.slot, in_slot = lane % a.slot;
     const int slots = kWave / a.slot;

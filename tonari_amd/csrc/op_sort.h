@@ -46,13 +46,6 @@ inline size_t sort_count_bytes(int64_t n) {
     return (size_t)kSortRadix * sort_stride(sort_tiles(n)) * sizeof(int32_t);
 }
 
-// Workgroups go to the 8 XCDs in turn: each XCD takes a run of tiles, so that
-// what neighbouring tiles write next to each other meets in one L2.
-__device__ __forceinline__ int64_t sort_tile_of(int64_t block, int64_t tiles) {
-    const int64_t each = tiles / 8, left = tiles % 8, xcd = block % 8, at = block / 8;
-    return xcd * each + (xcd < left ? xcd : left) + at;
-}
-
 // Keys and payloads of the first pass; later passes read what the one before
 // wrote.
 struct SortKeys {
@@ -68,7 +61,7 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_count(Keys keys, int64_t 
     const int radix = 1 << pass.bits;
     for (int d = threadIdx.x; d < radix; d += kSortThreads) hist[d] = 0;
     __syncthreads();
-    const int64_t tile = sort_tile_of(blockIdx.x, gridDim.x), base = tile * kSortTile;
+    const int64_t tile = xcd_order(blockIdx.x, gridDim.x), base = tile * kSortTile;
 #pragma unroll
     for (int r = 0; r < kSortRounds; ++r) {
         const int64_t i = base + r * kSortThreads + threadIdx.x;
@@ -127,7 +120,7 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_move(Keys keys, int64_t n
         for (int w = 0; w < kSortWaves; ++w) seen[w][d] = 0;
     __syncthreads();
     // a wave's items are consecutive, in rounds of 64
-    const int64_t tile = sort_tile_of(blockIdx.x, gridDim.x);
+    const int64_t tile = xcd_order(blockIdx.x, gridDim.x);
     const int64_t base = tile * kSortTile + wave * (kWave * kSortRounds);
     int key[kSortRounds], rank[kSortRounds];
 #pragma unroll

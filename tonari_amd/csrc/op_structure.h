@@ -325,31 +325,43 @@ struct Mat<float> {
     static constexpr bool kSeparateCols = false;
 };
 
-// Two staged tensors of 32 rows; the workgroup's threads share the units.  With
-// one unit each they are loaded a tile ahead, with more (few waves, wide heads)
-// when their tile is placed: their registers are worth more than the wait.
+// Two staged tensors, kTiles tiles of 32 rows each: as many as give the
+// workgroup's threads a unit each.  With one unit they are loaded a stage ahead,
+// with more (few waves, wide heads) when their stage is placed: their registers
+// are worth more than the wait.
 template <typename T, int DP, int NW>
 struct StagePair {
     using S = typename Mat<T>::template Stage<DP>;
-    static constexpr int kAll = 2 * S::kUnits, kThreads = NW * kWave;
+    static constexpr int kOne = S::kUnits, kThreads = NW * kWave;
+    static constexpr int kTiles = kThreads >= 8 * kOne ? 4 : kThreads >= 4 * kOne ? 2 : 1;
+    static constexpr int kAll = 2 * kOne * kTiles;
     static constexpr int kEach = (kAll + kThreads - 1) / kThreads;
     static constexpr bool kAhead = kEach == 1;
+    static constexpr int kRows = Mat<T>::kRows(DP);  // elements of a tile, as rows and as columns
+    static constexpr int kCols = Mat<T>::kSeparateCols ? Mat<T>::kCols(DP) : 0;
     const T *a, *b;
     int a_stride, b_stride, rows, dim;
     S ahead;
 
+    // unit u: of tile u / (2 kOne), and there of one tensor, then of the other
     __device__ __forceinline__ void load(S& s, int u) const {
-        if (u < S::kUnits)
-            s.load(u, a, a_stride, rows, dim);
-        else if (u < kAll)
-            s.load(u - S::kUnits, b, b_stride, rows, dim);
+        const int tile = u / (2 * kOne), v = u % (2 * kOne);
+        const bool first = v < kOne;
+        if (u < kAll)
+            s.load(first ? v : v - kOne, (first ? a : b) + (int64_t)tile * kTile * (first ? a_stride : b_stride),
+                   first ? a_stride : b_stride, rows - tile * kTile, dim);
     }
+    // (null: that form of the tensor is not wanted)
     static __device__ __forceinline__ void put(const S& s, int u, T* a_row, T* a_col, T* b_row,
                                                T* b_col) {
-        if (u < S::kUnits)
-            s.store(u, a_row, a_col);
-        else if (u < kAll)
-            s.store(u - S::kUnits, b_row, b_col);
+        const int tile = u / (2 * kOne), v = u % (2 * kOne);
+        const bool first = v < kOne;
+        if (u >= kAll) return;
+        if (first)
+            s.store(v, a_row ? a_row + tile * kRows : nullptr, a_col ? a_col + tile * kCols : nullptr);
+        else
+            s.store(v - kOne, b_row ? b_row + tile * kRows : nullptr,
+                    b_col ? b_col + tile * kCols : nullptr);
     }
     __device__ __forceinline__ void fetch(const T* a_, int a_stride_, const T* b_, int b_stride_,
                                           int rows_, int dim_) {
@@ -431,8 +443,9 @@ __device__ __forceinline__ void capped(const f32x16& dot, int run, const ScoreRu
 }
 
 // Positions of a staged tile, by axes: a lane's 16 rows are 4 runs of 4.
+template <int TILES>
 struct TilePositions {
-    alignas(16) float x[3][kTile];
+    alignas(16) float x[3][TILES * kTile];
 };
 __device__ __forceinline__ Vec<float, 4> four_of(const float* x, int run, int half) {
     return *(const Vec<float, 4>*)(x + 8 * run + 4 * half);
@@ -451,17 +464,21 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP)) void k_structure_forw
     const StructureArgs a) {
     using M = Mat<T>;
     using Row = typename M::template Row<DP>;
-    __shared__ alignas(16) T k_rows[M::kRows(DP)];
-    __shared__ alignas(16) T v_tile[M::kSeparateCols ? M::kCols(DP) : M::kRows(DP)];
-    __shared__ TilePositions x_k;
+    using Pair = StagePair<T, DP, NW>;
+    constexpr int kTiles = Pair::kTiles, kKeys = kTiles * kTile;
+    constexpr int kValues = M::kSeparateCols ? Pair::kCols : Pair::kRows;
+    __shared__ alignas(16) T k_rows[kTiles * Pair::kRows];
+    __shared__ alignas(16) T v_tile[kTiles * kValues];
+    __shared__ TilePositions<kTiles> x_k;
 
-    const StructureTile t = a.q_tiles[blockIdx.x];
+    const int64_t block = xcd_order(blockIdx.x, gridDim.x);
+    const StructureTile t = a.q_tiles[block];
     const int lane = lane_of(), half = lane / 32, wave = threadIdx.x / kWave;
     const int kv = blockIdx.y % a.kv_heads, split = blockIdx.y / a.kv_heads;
     const int g = a.group;
     if (t.n_q < 0) {  // NaN for the rows that lie here in the batch
         const int64_t all = (int64_t)a.n_queries * g;
-        const int64_t row = (int64_t)blockIdx.x * (NW * kTile) + wave * kTile + lane % 32;
+        const int64_t row = block * (NW * kTile) + wave * kTile + lane % 32;
         if (row >= all || split > 0 || half) return;
         const int query = (int)(row / g), head = kv * g + (int)(row % g);
         T* out = (T*)a.out + ((int64_t)query * a.heads + head) * a.dim;
@@ -507,13 +524,13 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP)) void k_structure_forw
     for (int d = 0; d < DP / 32; ++d) acc[d] = f32x16{};
     float top = -inf_of(), sum = 0.f;
 
-    StagePair<T, DP, NW> stage;
+    Pair stage;
     float xs[3];
     const auto fetch = [&](int tile) {
-        const int k0 = tile * kTile, n = t.n_k - k0;
+        const int k0 = tile * kTile, n = min(t.n_k, to * kTile) - k0;
         stage.fetch(kb + (int64_t)k0 * a.k_stride[0], (int)a.k_stride[0],
                    vb + (int64_t)k0 * a.v_stride[0], (int)a.v_stride[0], n, a.dim);
-        if (threadIdx.x < kTile) {
+        if (threadIdx.x < kKeys) {
             const float* p = xb + 3 * (int64_t)(k0 + min((int)threadIdx.x, n - 1));
 #pragma unroll
             for (int c = 0; c < 3; ++c) xs[c] = p[c];
@@ -525,7 +542,7 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP)) void k_structure_forw
             stage.place(k_rows, nullptr, nullptr, v_tile);
         else
             stage.place(k_rows, nullptr, v_tile, nullptr);
-        if (threadIdx.x < kTile)
+        if (threadIdx.x < kKeys)
 #pragma unroll
             for (int c = 0; c < 3; ++c) x_k.x[c][threadIdx.x] = xs[c];
         __syncthreads();
@@ -533,17 +550,19 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP)) void k_structure_forw
     // Weights are taken relative to `top`, the maximum when it was last set: it
     // is set anew only where a score passes it by more than 2^8 (the row's sums
     // then change their unit), so that most tiles neither subtract nor rescale.
-    const auto weigh = [&](int left) {
+    const auto weigh = [&](int sub, int left) {
         f32x16 dot{};
-        M::template rows<DP>(dot, k_rows, qr);
+        M::template rows<DP>(dot, k_rows + sub * Pair::kRows, qr);
         float s[16], unused[4];
         const float ref = top == -inf_of() ? 0.f : top;
         const bool near = all_near<CAP>(dot, a.rule);
         float high = -inf_of();
 #pragma unroll
         for (int run = 0; run < 4; ++run) {
-            const Vec<float, 4> x = four_of(x_k.x[0], run, half), y = four_of(x_k.x[1], run, half),
-                                z = four_of(x_k.x[2], run, half);
+            const int first = sub * kTile;
+            const Vec<float, 4> x = four_of(x_k.x[0] + first, run, half),
+                                y = four_of(x_k.x[1] + first, run, half),
+                                z = four_of(x_k.x[2] + first, run, half);
             float u[4];
             capped<CAP>(dot, run, a.rule, near, -ref, u, unused);
 #pragma unroll
@@ -581,13 +600,15 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP)) void k_structure_forw
             part[i % 4] += s[i];
         }
         sum += (part[0] + part[1]) + (part[2] + part[3]);
-        M::template cols<DP>(acc, v_tile, s);
+        M::template cols<DP>(acc, v_tile + sub * kValues, s);
     };
     if (from < to) fetch(from);
-    for (int tile = from; tile < to; ++tile) {
+    for (int tile = from; tile < to; tile += kTiles) {
         place();
-        if (tile + 1 < to) fetch(tile + 1);
-        if (busy) weigh(t.n_k - tile * kTile);
+        if (tile + kTiles < to) fetch(tile + kTiles);
+        if (busy)
+            for (int sub = 0; sub < min(kTiles, to - tile); ++sub)
+                weigh(sub, t.n_k - (tile + sub) * kTile);
     }
     sum = sum_halves(sum);
     if (!valid) return;

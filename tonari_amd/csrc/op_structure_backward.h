@@ -56,17 +56,20 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP <= 32 ? 64 : 2 * DP)) v
     const StructureArgs a) {
     using M = Mat<T>;
     using Row = typename M::template Row<DP>;
-    __shared__ alignas(16) T k_rows[M::kRows(DP)];
-    __shared__ alignas(16) T k_cols[M::kSeparateCols ? M::kCols(DP) : 8];
-    __shared__ alignas(16) T v_rows[M::kRows(DP)];
-    __shared__ TilePositions x_k;
+    using Pair = StagePair<T, DP, NW>;
+    constexpr int kTiles = Pair::kTiles, kKeys = kTiles * kTile;
+    __shared__ alignas(16) T k_rows[kTiles * Pair::kRows];
+    __shared__ alignas(16) T k_cols[M::kSeparateCols ? kTiles * Pair::kCols : 8];
+    __shared__ alignas(16) T v_rows[kTiles * Pair::kRows];
+    __shared__ TilePositions<kTiles> x_k;
 
-    const StructureTile t = a.q_tiles[blockIdx.x];
+    const int64_t block = xcd_order(blockIdx.x, gridDim.x);
+    const StructureTile t = a.q_tiles[block];
     const int lane = lane_of(), half = lane / 32, wave = threadIdx.x / kWave;
     const int kv = blockIdx.y % a.kv_heads, split = blockIdx.y / a.kv_heads;
     const int g = a.group;
     if (t.n_q < 0) {
-        const int64_t row = (int64_t)blockIdx.x * (NW * kTile) + wave * kTile + lane % 32;
+        const int64_t row = block * (NW * kTile) + wave * kTile + lane % 32;
         if (row >= (int64_t)a.n_queries * g || half) return;
         const int query = (int)(row / g), head = kv * g + (int)(row % g);
         const int64_t at = (int64_t)head * a.n_queries + query;
@@ -131,13 +134,13 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP <= 32 ? 64 : 2 * DP)) v
 #pragma unroll
     for (int i = 0; i < kRowSums; ++i) w[i] = 0.f;
 
-    StagePair<T, DP, NW> stage;
+    Pair stage;
     float xs[3];
     const auto fetch = [&](int tile) {
-        const int k0 = tile * kTile, n = t.n_k - k0;
+        const int k0 = tile * kTile, n = min(t.n_k, to * kTile) - k0;
         stage.fetch(kb + (int64_t)k0 * a.k_stride[0], (int)a.k_stride[0],
                    vb + (int64_t)k0 * a.v_stride[0], (int)a.v_stride[0], n, a.dim);
-        if (threadIdx.x < kTile) {
+        if (threadIdx.x < kKeys) {
             const float* p = xb + 3 * (int64_t)(k0 + min((int)threadIdx.x, n - 1));
 #pragma unroll
             for (int c = 0; c < 3; ++c) xs[c] = p[c];
@@ -146,21 +149,23 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP <= 32 ? 64 : 2 * DP)) v
     const auto place = [&] {
         __syncthreads();
         stage.place(k_rows, M::kSeparateCols ? k_cols : nullptr, v_rows, nullptr);
-        if (threadIdx.x < kTile)
+        if (threadIdx.x < kKeys)
 #pragma unroll
             for (int c = 0; c < 3; ++c) x_k.x[c][threadIdx.x] = xs[c];
         __syncthreads();
     };
-    const auto push = [&](int left) {
+    const auto push = [&](int sub, int left) {
         f32x16 dot{}, dp{};
-        M::template rows<DP>(dot, k_rows, qr);
-        M::template rows<DP>(dp, v_rows, dor);
+        M::template rows<DP>(dot, k_rows + sub * Pair::kRows, qr);
+        M::template rows<DP>(dp, v_rows + sub * Pair::kRows, dor);
         float p[16];
         const bool near = all_near<CAP>(dot, a.rule);
 #pragma unroll
         for (int run = 0; run < 4; ++run) {
-            const Vec<float, 4> x = four_of(x_k.x[0], run, half), y = four_of(x_k.x[1], run, half),
-                                z = four_of(x_k.x[2], run, half);
+            const int first = sub * kTile;
+            const Vec<float, 4> x = four_of(x_k.x[0] + first, run, half),
+                                y = four_of(x_k.x[1] + first, run, half),
+                                z = four_of(x_k.x[2] + first, run, half);
             float dx[4], dy[4], dz[4], r[4], s[4], u[4], bend[4];
             capped<CAP>(dot, run, a.rule, near, -lse, u, bend);
 #pragma unroll
@@ -200,13 +205,23 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP <= 32 ? 64 : 2 * DP)) v
             }
             __builtin_amdgcn_sched_barrier(0);
         }
-        M::template cols<DP>(acc, M::kSeparateCols ? k_cols : k_rows, p);
+        // Their sum over a row is 0, so grad_q is a difference: what the rounding of
+        // dx leaves out goes through a second product.
+        const T* cols = M::kSeparateCols ? k_cols + sub * Pair::kCols : k_rows + sub * Pair::kRows;
+        M::template cols<DP>(acc, cols, p);
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) p[i] -= (float)rounded<T>(p[i]);
+            M::template cols<DP>(acc, cols, p);
+        }
     };
     if (from < to) fetch(from);
-    for (int tile = from; tile < to; ++tile) {
+    for (int tile = from; tile < to; tile += kTiles) {
         place();
-        if (tile + 1 < to) fetch(tile + 1);
-        if (busy) push(t.n_k - tile * kTile);
+        if (tile + kTiles < to) fetch(tile + kTiles);
+        if (busy)
+            for (int sub = 0; sub < min(kTiles, to - tile); ++sub)
+                push(sub, t.n_k - (tile + sub) * kTile);
     }
 #pragma unroll
     for (int i = 0; i < kRowSums; ++i) w[i] = sum_halves(w[i]);
@@ -274,18 +289,21 @@ k_structure_dkv(const StructureArgs a) {
     using Row = typename M::template Row<DP>;
     constexpr float kLift = kNarrow<T> ? 12.f : 0.f;
     constexpr float kLower = kNarrow<T> ? 1.f / 4096.f : 1.f;
-    __shared__ alignas(16) T q_rows[M::kRows(DP)];
-    __shared__ alignas(16) T o_rows[M::kRows(DP)];
-    __shared__ alignas(16) T q_cols[M::kSeparateCols ? M::kCols(DP) : 8];
-    __shared__ alignas(16) T o_cols[M::kSeparateCols ? M::kCols(DP) : 8];
-    __shared__ TilePositions x_q;
-    __shared__ alignas(16) float stat[3][kTile];  // log-sum, delta, largest |grad_out|
+    using Pair = StagePair<T, DP, NW>;
+    constexpr int kTiles = Pair::kTiles, kQueries = kTiles * kTile;
+    __shared__ alignas(16) T q_rows[kTiles * Pair::kRows];
+    __shared__ alignas(16) T o_rows[kTiles * Pair::kRows];
+    __shared__ alignas(16) T q_cols[M::kSeparateCols ? kTiles * Pair::kCols : 8];
+    __shared__ alignas(16) T o_cols[M::kSeparateCols ? kTiles * Pair::kCols : 8];
+    __shared__ TilePositions<kTiles> x_q;
+    __shared__ alignas(16) float stat[3][kQueries];  // log-sum, delta, largest |grad_out|
 
-    const StructureTile t = a.k_tiles[blockIdx.x];
+    const int64_t block = xcd_order(blockIdx.x, gridDim.x);
+    const StructureTile t = a.k_tiles[block];
     const int lane = lane_of(), half = lane / 32, wave = threadIdx.x / kWave;
     const int kv = blockIdx.y % a.kv_heads, split = blockIdx.y / a.kv_heads;
     if (t.n_q < 0) {
-        const int64_t key = (int64_t)blockIdx.x * (NW * kTile) + wave * kTile + lane % 32;
+        const int64_t key = block * (NW * kTile) + wave * kTile + lane % 32;
         if (key >= a.n_keys || half) return;
         if (a.k_splits > 1) {
             float* part = a.part_k + (((int64_t)split * a.kv_heads + kv) * a.n_keys + key) *
@@ -318,17 +336,18 @@ k_structure_dkv(const StructureArgs a) {
     float px = 0.f, py = 0.f, pz = 0.f;
     int scale_e = kNoScale;  // exponent of what dk is held in
 
-    const int per_head = (t.n_q + kTile - 1) / kTile, tiles = per_head * a.group;
-    StagePair<T, DP, NW> stage;
+    // stages of kTiles tiles, of one head after the other
+    const int per_head = (t.n_q + kQueries - 1) / kQueries, stages = per_head * a.group;
+    Pair stage;
     float xs[3], ss[3];
-    const auto fetch = [&](int tile) {
-        const int head = kv * a.group + tile / per_head;
-        const int q0 = (tile % per_head) * kTile, n = t.n_q - q0;
+    const auto fetch = [&](int at_stage) {
+        const int head = kv * a.group + at_stage / per_head;
+        const int q0 = (at_stage % per_head) * kQueries, n = t.n_q - q0;
         const int64_t first = t.q_lo + q0;
         stage.fetch((const T*)a.q + first * a.q_stride[0] + head * a.q_stride[1], (int)a.q_stride[0],
-                   (const T*)a.grad_out + (first * a.heads + head) * a.dim,
-                   a.heads * a.dim, n, a.dim);
-        if (threadIdx.x < kTile) {
+                    (const T*)a.grad_out + (first * a.heads + head) * a.dim, a.heads * a.dim, n,
+                    a.dim);
+        if (threadIdx.x < kQueries) {
             const bool in = (int)threadIdx.x < n;
             const int64_t query = first + (in ? threadIdx.x : 0);
             const int64_t at = (int64_t)head * a.n_queries + query;
@@ -340,37 +359,22 @@ k_structure_dkv(const StructureArgs a) {
             ss[2] = in ? a.row[2 * at + 1] : 0.f;
         }
     };
-    const int each = (tiles + a.k_splits - 1) / a.k_splits;
-    const int from = min(tiles, split * each), to = min(tiles, from + each);
-    if (from < to) fetch(from);
-    for (int tile = from; tile < to; ++tile) {
-        __syncthreads();
-        stage.place(q_rows, M::kSeparateCols ? q_cols : nullptr, o_rows,
-                    M::kSeparateCols ? o_cols : nullptr);
-        if (threadIdx.x < kTile)
-#pragma unroll
-            for (int c = 0; c < 3; ++c) {
-                x_q.x[c][threadIdx.x] = xs[c];
-                stat[c][threadIdx.x] = ss[c];
-            }
-        __syncthreads();
-        const float slope = a.slopes[kv * a.group + tile / per_head], slope2 = slope * kLog2e;
-        if (tile + 1 < to) fetch(tile + 1);
-
-        if (t.first + wave * kTile >= t.n_k) continue;  // a wave without keys only helps to stage
-
+    const auto pull = [&](int sub, float slope) {
+        const float slope2 = slope * kLog2e;
         f32x16 dot{}, dp{};
-        M::template rows<DP>(dot, q_rows, kr);
-        M::template rows<DP>(dp, o_rows, vr);
+        M::template rows<DP>(dot, q_rows + sub * Pair::kRows, kr);
+        M::template rows<DP>(dp, o_rows + sub * Pair::kRows, vr);
         float p[16], dx[16];
         const bool near = all_near<CAP>(dot, a.rule);
         float tile_top = 0.f, ux = 0.f, uy = 0.f, uz = 0.f;
 #pragma unroll
         for (int run = 0; run < 4; ++run) {
-            const Vec<float, 4> x = four_of(x_q.x[0], run, half), y = four_of(x_q.x[1], run, half),
-                                z = four_of(x_q.x[2], run, half),
-                                lse = four_of(stat[0], run, half),
-                                delta = four_of(stat[1], run, half);
+            const int first = sub * kTile;
+            const Vec<float, 4> x = four_of(x_q.x[0] + first, run, half),
+                                y = four_of(x_q.x[1] + first, run, half),
+                                z = four_of(x_q.x[2] + first, run, half),
+                                lse = four_of(stat[0] + first, run, half),
+                                delta = four_of(stat[1] + first, run, half);
             float u[4], bend[4];
             capped<CAP>(dot, run, a.rule, near, kLift, u, bend);
 #pragma unroll
@@ -390,7 +394,7 @@ k_structure_dkv(const StructureArgs a) {
             }
             __builtin_amdgcn_sched_barrier(0);
             if (kNarrow<T>) {
-                const Vec<float, 4> largest = four_of(stat[2], run, half);
+                const Vec<float, 4> largest = four_of(stat[2] + first, run, half);
                 tile_top = fmaxf(fmaxf(fmaxf(tile_top, largest[0]), largest[1]),
                                  fmaxf(largest[2], largest[3]));
             }
@@ -411,8 +415,31 @@ k_structure_dkv(const StructureArgs a) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) dx[i] *= unit;
         }
-        M::template cols<DP>(dv, M::kSeparateCols ? o_cols : o_rows, p);
-        M::template cols<DP>(dk, M::kSeparateCols ? q_cols : q_rows, dx);
+        M::template cols<DP>(
+            dv, M::kSeparateCols ? o_cols + sub * Pair::kCols : o_rows + sub * Pair::kRows, p);
+        M::template cols<DP>(
+            dk, M::kSeparateCols ? q_cols + sub * Pair::kCols : q_rows + sub * Pair::kRows, dx);
+    };
+    const bool busy = t.first + wave * kTile < t.n_k;  // a wave without keys only helps to stage
+    const int each = (stages + a.k_splits - 1) / a.k_splits;
+    const int from = min(stages, split * each), to = min(stages, from + each);
+    if (from < to) fetch(from);
+    for (int i = from; i < to; ++i) {
+        __syncthreads();
+        stage.place(q_rows, M::kSeparateCols ? q_cols : nullptr, o_rows,
+                    M::kSeparateCols ? o_cols : nullptr);
+        if (threadIdx.x < kQueries)
+#pragma unroll
+            for (int c = 0; c < 3; ++c) {
+                x_q.x[c][threadIdx.x] = xs[c];
+                stat[c][threadIdx.x] = ss[c];
+            }
+        __syncthreads();
+        if (i + 1 < to) fetch(i + 1);
+        const int n = t.n_q - (i % per_head) * kQueries;
+        if (busy)
+            for (int sub = 0; sub < kTiles && sub * kTile < n; ++sub)
+                pull(sub, a.slopes[kv * a.group + i / per_head]);
     }
     px = sum_halves(px);
     py = sum_halves(py);
