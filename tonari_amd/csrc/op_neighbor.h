@@ -474,7 +474,7 @@ __global__ __launch_bounds__(256, kHeldBack) void k_neighbor_dq(const NeighborAr
         for (int g = 0; g < GH; ++g) {
             q[g] = go[g] = Raw<T>{};
             delta[g] = turn[g] = slope[g] = 0.f;
-            lse[g] = inf_of();  // a lane without channels weighs nothing
+            lse[g] = inf_of();
             if (l.mine) {
                 const int64_t at = (row + g) * a.dim + l.c;
                 float o[VEC];
@@ -484,6 +484,8 @@ __global__ __launch_bounds__(256, kHeldBack) void k_neighbor_dq(const NeighborAr
                 load_wide<VEC>(a.out_full + at, o);
 #pragma unroll
                 for (int x = 0; x < VEC; ++x) delta[g] = fmaf((float)go[g].x[x], o[x], delta[g]);
+            }
+            if (l.there) {  // in every lane of the head: slot_sum takes any of them
                 lse[g] = a.lse[row + g];
                 if (lse[g] == -inf_of()) lse[g] = inf_of();
                 slope[g] = a.slopes[l.head + g];
@@ -527,7 +529,7 @@ __global__ __launch_bounds__(256, kHeldBack) void k_neighbor_dq(const NeighborAr
                 for (int g = 0; g < GH; ++g) {
                     s[g] = fmaf(-slope[g] * kLog2e, d[u], s[g]);
                     float ds = exp2_of(s[g] - lse[g]) * (dp[g] - delta[g]);
-                    if (!l.mine || (!whole && !in)) ds = 0.f;
+                    if (!l.there || (!whole && !in)) ds = 0.f;
                     kx[u].add(CAP ? ds * bend[g] : ds, acc[g]);
                     turn[g] = fmaf(-ds, d[u] - near, turn[g]);
                     push = fmaf(-slope[g], ds, push);

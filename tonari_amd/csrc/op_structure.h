@@ -128,6 +128,10 @@ __device__ __forceinline__ int row_of(int i, int half) { return 8 * (i / 4) + 4 
 template <typename T>
 struct Mat;
 
+// The scheduler keeps the work on four products together, which bounds the
+// registers, but may read the next four's rows from LDS meanwhile.
+constexpr int kLoadsPass = 0x100;
+
 template <typename T, typename F>
 struct Mat16 {
     using Frag = Vec<T, 8>;
@@ -176,16 +180,17 @@ struct Mat16 {
         for (int s = 0; s < DP / 16; ++s) acc = F::mma(*(const Frag*)(p + 16 * s), b.x[s], acc);
     }
 
+    // A lane's 16 weights of a tile, rounded for the second product.
+    struct Weights {
+        Frag b[2];
+        __device__ __forceinline__ void set(int i, float x) { b[i / 8][i % 8] = rounded<T>(x); }
+        __device__ __forceinline__ float get(int i) const { return (float)b[i / 8][i % 8]; }
+    };
     // acc[channel block] += tile^T . p
     template <int DP>
     static __device__ __forceinline__ void cols(f32x16 (&acc)[DP / 32], const T* tile,
-                                                const float (&p)[16]) {
+                                                const Weights& p) {
         const int lane = lane_of();
-        Frag b[2];
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) b[s][e] = rounded<T>(p[8 * s + e]);
         const T* at = tile + (lane % 32) * (kTile + 4) + 4 * (lane / 32);
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d)
@@ -194,7 +199,7 @@ struct Mat16 {
                 const T* c = at + d * 32 * (kTile + 4) + 16 * s;
                 const Vec<T, 4> lo = *(const Vec<T, 4>*)c, hi = *(const Vec<T, 4>*)(c + 8);
                 const Frag a = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-                acc[d] = F::mma(a, b[s], acc[d]);
+                acc[d] = F::mma(a, p.b[s], acc[d]);
             }
     }
 
@@ -288,9 +293,14 @@ struct Mat<float> {
         }
     }
 
+    struct Weights {
+        float b[16];
+        __device__ __forceinline__ void set(int i, float x) { b[i] = x; }
+        __device__ __forceinline__ float get(int i) const { return b[i]; }
+    };
     template <int DP>
     static __device__ __forceinline__ void cols(f32x16 (&acc)[DP / 32], const float* tile,
-                                                const float (&p)[16]) {
+                                                const Weights& p) {
         const int lane = lane_of();
         const float* at = tile + lane % 32;
 #pragma unroll
@@ -298,7 +308,7 @@ struct Mat<float> {
 #pragma unroll
             for (int i = 0; i < 16; ++i)
                 acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(
-                    at[row_of(i, lane / 32) * (DP + 4) + 32 * d], p[i], acc[d], 0, 0, 0);
+                    at[row_of(i, lane / 32) * (DP + 4) + 32 * d], p.b[i], acc[d], 0, 0, 0);
     }
 
     // Threads stage units of 4 rows x 4 channels.
@@ -579,7 +589,7 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP)) void k_structure_forw
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) high = fmaxf(high, s[4 * run + e]);
-            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_sched_barrier(kLoadsPass);
         }
         high = max_halves(high);
         const bool anew = high > 8.f || (top == -inf_of() && high > -inf_of());
@@ -594,13 +604,15 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP)) void k_structure_forw
             for (int i = 0; i < 16; ++i) s[i] -= up;
         }
         float part[4] = {};
+        typename M::Weights p;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            s[i] = exp2_of(s[i]);
-            part[i % 4] += s[i];
+            const float w = exp2_of(s[i]);
+            part[i % 4] += w;
+            p.set(i, w);
         }
         sum += (part[0] + part[1]) + (part[2] + part[3]);
-        M::template cols<DP>(acc, v_tile + sub * kValues, s);
+        M::template cols<DP>(acc, v_tile + sub * kValues, p);
     };
     if (from < to) fetch(from);
     for (int tile = from; tile < to; tile += kTiles) {

@@ -30,7 +30,7 @@ constexpr bool kNarrow<f16> = true;
 constexpr int kNoScale = -1000;
 
 // Sums of a query row besides grad_q: e, sum (ds u, p u) for the unit vectors
-// u, sum (ds r, p r).
+// u, sum (ds (r - r'), p (r - r')) for one r' of the row.
 constexpr int kRowSums = 9;
 
 __device__ __forceinline__ float power_of(int e) { return __builtin_amdgcn_ldexpf(1.f, e); }
@@ -123,6 +123,15 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP <= 32 ? 64 : 2 * DP)) v
     const T* vb = (const T*)a.v + (int64_t)t.k_lo * a.v_stride[0] + kv * a.v_stride[1];
     const float* xb = a.x_k + 3 * (int64_t)t.k_lo;
 
+    // distances in the slope's sums count from that of one key: what they share
+    // cancels (sum ds = 0), exactly
+    float r_mid = 0.f;
+    if (valid && t.n_k > 0) {
+        const float* p = xb + 3 * (int64_t)(t.n_k / 2);
+        const float ex = xq - p[0], ey = yq - p[1], ez = zq - p[2];
+        r_mid = __builtin_amdgcn_sqrtf(fmaf(ex, ex, fmaf(ey, ey, ez * ez)));
+    }
+
     const int tiles = (t.n_k + kTile - 1) / kTile;
     const int each = (tiles + a.splits - 1) / a.splits;
     const int from = min(tiles, split * each), to = min(tiles, from + each);
@@ -158,7 +167,7 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP <= 32 ? 64 : 2 * DP)) v
         f32x16 dot{}, dp{};
         M::template rows<DP>(dot, k_rows + sub * Pair::kRows, qr);
         M::template rows<DP>(dp, v_rows + sub * Pair::kRows, dor);
-        float p[16];
+        typename M::Weights p, rest;
         const bool near = all_near<CAP>(dot, a.rule);
 #pragma unroll
         for (int run = 0; run < 4; ++run) {
@@ -183,37 +192,40 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP <= 32 ? 64 : 2 * DP)) v
                 for (int e = 0; e < 4; ++e)
                     if (8 * run + e >= left - 4 * half) s[e] = 0.f;
             }
+            float ds[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int i = 4 * run + e;
-                const float ds = s[e] * (dp[i] - delta);
-                p[i] = CAP ? ds * bend[e] : ds;
-                if (kNarrow<T>) p[i] *= unit;
-                if (geometry) {
+                ds[e] = s[e] * (dp[i] - delta);
+                float dx_i = CAP ? ds[e] * bend[e] : ds[e];
+                if (kNarrow<T>) dx_i *= unit;
+                p.set(i, dx_i);
+                if (sizeof(T) == 2) rest.set(i, dx_i - p.get(i));
+            }
+            if (geometry) {
+                asm volatile("");  // one branch for the run
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
                     const float over = r[e] > 0.f ? __builtin_amdgcn_rcpf(r[e]) : 0.f;
-                    const float wd = ds * over, wp = s[e] * over;
-                    w[0] += ds;
+                    const float wd = ds[e] * over, wp = s[e] * over;
+                    w[0] += ds[e];
                     w[1] = fmaf(wd, dx[e], w[1]);
                     w[2] = fmaf(wd, dy[e], w[2]);
                     w[3] = fmaf(wd, dz[e], w[3]);
                     w[4] = fmaf(wp, dx[e], w[4]);
                     w[5] = fmaf(wp, dy[e], w[5]);
                     w[6] = fmaf(wp, dz[e], w[6]);
-                    w[7] = fmaf(ds, r[e], w[7]);
-                    w[8] = fmaf(s[e], r[e], w[8]);
+                    w[7] = fmaf(ds[e], r[e] - r_mid, w[7]);
+                    w[8] = fmaf(s[e], r[e] - r_mid, w[8]);
                 }
             }
-            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_sched_barrier(kLoadsPass);
         }
         // Their sum over a row is 0, so grad_q is a difference: what the rounding of
         // dx leaves out goes through a second product.
         const T* cols = M::kSeparateCols ? k_cols + sub * Pair::kCols : k_rows + sub * Pair::kRows;
         M::template cols<DP>(acc, cols, p);
-        if constexpr (sizeof(T) == 2) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) p[i] -= (float)rounded<T>(p[i]);
-            M::template cols<DP>(acc, cols, p);
-        }
+        if constexpr (sizeof(T) == 2) M::template cols<DP>(acc, cols, rest);
     };
     if (from < to) fetch(from);
     for (int tile = from; tile < to; tile += kTiles) {
@@ -282,8 +294,7 @@ __global__ __launch_bounds__(256) void k_structure_join_dq(const StructureArgs a
 
 // grid: (key tiles, kv_heads * k_splits); NW waves of 32 keys each.
 template <typename T, int DP, int NW, bool CAP>
-__global__ __launch_bounds__(NW* kWave, CAP ? (DP <= 64 && sizeof(T) == 2 ? 2 : 1)
-                                                  : waves_held<T>(DP <= 32 ? 64 : 2 * DP)) void
+__global__ __launch_bounds__(NW* kWave, DP > 64 ? 1 : DP > 32 || CAP || sizeof(T) == 4 ? 2 : 3) void
 k_structure_dkv(const StructureArgs a) {
     using M = Mat<T>;
     using Row = typename M::template Row<DP>;
@@ -364,9 +375,28 @@ k_structure_dkv(const StructureArgs a) {
         f32x16 dot{}, dp{};
         M::template rows<DP>(dot, q_rows + sub * Pair::kRows, kr);
         M::template rows<DP>(dp, o_rows + sub * Pair::kRows, vr);
-        float p[16], dx[16];
+        typename M::Weights p, dx;
         const bool near = all_near<CAP>(dot, a.rule);
-        float tile_top = 0.f, ux = 0.f, uy = 0.f, uz = 0.f;
+        float unit = 1.f;
+        if (kNarrow<T>) {
+            float tile_top = 0.f;
+#pragma unroll
+            for (int run = 0; run < 4; ++run) {
+                const Vec<float, 4> largest = four_of(stat[2] + sub * kTile, run, half);
+                tile_top = fmaxf(fmaxf(fmaxf(tile_top, largest[0]), largest[1]),
+                                 fmaxf(largest[2], largest[3]));
+            }
+            tile_top = max_halves(tile_top);
+            const int e = exponent_of(tile_top);
+            if (tile_top > 0.f && e > scale_e) {  // (all zeros: dx is zero whatever the scale)
+                const float by = scale_e == kNoScale ? 1.f : power_of(scale_e - e);
+#pragma unroll
+                for (int d = 0; d < DP / 32; ++d) dk[d] *= by;
+                scale_e = e;
+            }
+            unit = scale_e == kNoScale ? 1.f : power_of(-scale_e);
+        }
+        float ux = 0.f, uy = 0.f, uz = 0.f;
 #pragma unroll
         for (int run = 0; run < 4; ++run) {
             const int first = sub * kTile;
@@ -377,44 +407,36 @@ k_structure_dkv(const StructureArgs a) {
                                 delta = four_of(stat[1] + first, run, half);
             float u[4], bend[4];
             capped<CAP>(dot, run, a.rule, near, kLift, u, bend);
+            float ex[4], ey[4], ez[4], r[4], ds[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int i = 4 * run + e;
-                const float ex = x[e] - xk, ey = y[e] - yk, ez = z[e] - zk;
-                const float r = __builtin_amdgcn_sqrtf(fmaf(ex, ex, fmaf(ey, ey, ez * ez)));
-                p[i] = exp2_of(fmaf(-slope2, r, u[e]) - lse[e]);
-                const float ds = (kNarrow<T> ? p[i] * kLower : p[i]) * (dp[i] - delta[e]);
-                if (a.push_k) {
-                    const float wd = ds * (r > 0.f ? __builtin_amdgcn_rcpf(r) : 0.f);
-                    ux = fmaf(wd, ex, ux);
-                    uy = fmaf(wd, ey, uy);
-                    uz = fmaf(wd, ez, uz);
+                ex[e] = x[e] - xk;
+                ey[e] = y[e] - yk;
+                ez[e] = z[e] - zk;
+                r[e] = __builtin_amdgcn_sqrtf(
+                    fmaf(ex[e], ex[e], fmaf(ey[e], ey[e], ez[e] * ez[e])));
+                const float w = exp2_of(fmaf(-slope2, r[e], u[e]) - lse[e]);
+                ds[e] = (kNarrow<T> ? w * kLower : w) * (dp[i] - delta[e]);
+                p.set(i, w);
+                const float dx_i = CAP ? ds[e] * bend[e] : ds[e];
+                dx.set(i, kNarrow<T> ? dx_i * unit : dx_i);
+            }
+            if (a.push_k) {
+                asm volatile("");  // one branch for the run
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float wd = ds[e] * (r[e] > 0.f ? __builtin_amdgcn_rcpf(r[e]) : 0.f);
+                    ux = fmaf(wd, ex[e], ux);
+                    uy = fmaf(wd, ey[e], uy);
+                    uz = fmaf(wd, ez[e], uz);
                 }
-                dx[i] = CAP ? ds * bend[e] : ds;
             }
-            __builtin_amdgcn_sched_barrier(0);
-            if (kNarrow<T>) {
-                const Vec<float, 4> largest = four_of(stat[2] + first, run, half);
-                tile_top = fmaxf(fmaxf(fmaxf(tile_top, largest[0]), largest[1]),
-                                 fmaxf(largest[2], largest[3]));
-            }
+            __builtin_amdgcn_sched_barrier(kLoadsPass);
         }
         px = fmaf(slope, ux, px);
         py = fmaf(slope, uy, py);
         pz = fmaf(slope, uz, pz);
-        if (kNarrow<T>) {
-            tile_top = max_halves(tile_top);
-            const int e = exponent_of(tile_top);
-            if (tile_top > 0.f && e > scale_e) {  // (all zeros: dx is zero whatever the scale)
-                const float by = scale_e == kNoScale ? 1.f : power_of(scale_e - e);
-#pragma unroll
-                for (int d = 0; d < DP / 32; ++d) dk[d] *= by;
-                scale_e = e;
-            }
-            const float unit = scale_e == kNoScale ? 1.f : power_of(-scale_e);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) dx[i] *= unit;
-        }
         M::template cols<DP>(
             dv, M::kSeparateCols ? o_cols + sub * Pair::kCols : o_rows + sub * Pair::kRows, p);
         M::template cols<DP>(
