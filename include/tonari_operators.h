@@ -83,23 +83,27 @@ typedef struct tnr_structure_attention {
     const void* k;                  /* T[n_keys][kv_heads][dim] */
     const void* v;
     int64_t q_stride[2], k_stride[2], v_stride[2];  /* atom, head */
-    const float* query_positions;   /* [n_queries][3] (may be positions) */
+    const float* query_positions;   /* [n_queries][3]; NULL: the queries are the keys' atoms, at
+                                       positions (n_queries == n_keys) */
     const float* positions;         /* [n_keys][3] */
     const float* slopes;            /* [heads] */
     float scale, softcap;
+    void* tiles;                    /* tnr_structure_tiles_size() bytes, 256-byte aligned: the batch
+                                       as the forward cuts it up; the backward reads it */
     void* out;                      /* T[n_queries][heads][dim] */
     float* lse;                     /* [heads][n_queries]: what the backward needs; NULL: not wanted */
-    /* backward: out and lse of the forward, and */
+    /* backward: tiles, out and lse of the forward, and */
     const void* grad_out;           /* T[n_queries][heads][dim] */
     void* grad_q;                   /* contiguous, like q, k and v; written whole */
     void* grad_k;
     void* grad_v;
-    float* grad_query_positions;    /* NULL: not wanted, or added to grad_positions (see there) */
-    float* grad_positions;          /* NULL: not wanted.  Where query_positions is positions, the
-                                       queries' share is in it and grad_query_positions is NULL */
+    float* grad_query_positions;    /* NULL: not wanted */
+    float* grad_positions;          /* NULL: not wanted; holds the queries' share too where
+                                       query_positions is NULL */
     float* grad_slopes;             /* [heads]; NULL: not wanted */
 } tnr_structure_attention;
 
+size_t tnr_structure_tiles_size(const tnr_structure_attention* req);
 size_t tnr_structure_forward_workspace_size(const tnr_structure_attention* req);
 int tnr_structure_forward(const tnr_structure_attention* req, void* workspace,
                           size_t workspace_bytes, void* stream, char* err, size_t err_len);

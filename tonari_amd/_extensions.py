@@ -114,6 +114,161 @@ class SkinList(ctypes.Structure):
     ]
 
 
+# include/tonari_operators.h: the operators beside the search.
+OPERATORS_VERSION = 1
+OPERATOR_EXPORTS = (
+    "tnr_operators_version",
+    "tnr_embedding_forward",
+    "tnr_embedding_workspace_size",
+    "tnr_embedding_backward",
+    "tnr_structure_tiles_size",
+    "tnr_structure_forward_workspace_size",
+    "tnr_structure_forward",
+    "tnr_structure_backward_workspace_size",
+    "tnr_structure_backward",
+    "tnr_neighbor_rows_size",
+    "tnr_neighbor_rows_workspace_size",
+    "tnr_neighbor_rows",
+    "tnr_neighbor_forward",
+    "tnr_neighbor_backward_workspace_size",
+    "tnr_neighbor_backward",
+)
+
+
+class Embedding(ctypes.Structure):
+    """``tnr_embedding`` of include/tonari_operators.h."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("index_bytes", ctypes.c_int32),
+        ("n_atoms", ctypes.c_int64),
+        ("n_species", ctypes.c_int64),
+        ("channels", ctypes.c_int64),
+        ("species", ctypes.c_void_p),
+        ("weight", ctypes.c_void_p),
+        ("scale", ctypes.c_float),
+        ("out", ctypes.c_void_p),
+        ("grad_out", ctypes.c_void_p),
+        ("grad_weight", ctypes.c_void_p),
+    ]
+
+
+class StructureAttention(ctypes.Structure):
+    """``tnr_structure_attention`` of include/tonari_operators.h."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("heads", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("dim", ctypes.c_int32),
+        ("n_structures", ctypes.c_int64),
+        ("n_queries", ctypes.c_int64),
+        ("n_keys", ctypes.c_int64),
+        ("query_ptr", ctypes.c_void_p),
+        ("key_ptr", ctypes.c_void_p),
+        ("q", ctypes.c_void_p),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("q_stride", ctypes.c_int64 * 2),
+        ("k_stride", ctypes.c_int64 * 2),
+        ("v_stride", ctypes.c_int64 * 2),
+        ("query_positions", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("slopes", ctypes.c_void_p),
+        ("scale", ctypes.c_float),
+        ("softcap", ctypes.c_float),
+        ("tiles", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p),
+        ("grad_out", ctypes.c_void_p),
+        ("grad_q", ctypes.c_void_p),
+        ("grad_k", ctypes.c_void_p),
+        ("grad_v", ctypes.c_void_p),
+        ("grad_query_positions", ctypes.c_void_p),
+        ("grad_positions", ctypes.c_void_p),
+        ("grad_slopes", ctypes.c_void_p),
+    ]
+
+
+class NeighborList(ctypes.Structure):
+    """``tnr_neighbor_list`` of include/tonari_operators.h."""
+
+    _fields_ = [
+        ("n_pairs", ctypes.c_int64),
+        ("n_sources", ctypes.c_int64),
+        ("n_targets", ctypes.c_int64),
+        ("sources", ctypes.c_void_p),
+        ("targets", ctypes.c_void_p),
+        ("transpose", ctypes.c_int32),
+        ("rows", ctypes.c_void_p),
+    ]
+
+
+class NeighborAttention(ctypes.Structure):
+    """``tnr_neighbor_attention`` of include/tonari_operators.h."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("heads", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("dim", ctypes.c_int32),
+        ("list", NeighborList),
+        ("q", ctypes.c_void_p),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("q_stride", ctypes.c_int64 * 2),
+        ("k_stride", ctypes.c_int64 * 2),
+        ("v_stride", ctypes.c_int64 * 2),
+        ("distances", ctypes.c_void_p),
+        ("slopes", ctypes.c_void_p),
+        ("scale", ctypes.c_float),
+        ("softcap", ctypes.c_float),
+        ("out", ctypes.c_void_p),
+        ("out32", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p),
+        ("grad_out", ctypes.c_void_p),
+        ("grad_q", ctypes.c_void_p),
+        ("grad_k", ctypes.c_void_p),
+        ("grad_v", ctypes.c_void_p),
+        ("grad_distances", ctypes.c_void_p),
+        ("grad_slopes", ctypes.c_void_p),
+    ]
+
+
+def _declare_operators(lib: ctypes.CDLL) -> None:
+    """Signatures of OPERATOR_EXPORTS (the torch module calls them from native code)."""
+    tail = [ctypes.c_void_p, ctypes.c_char_p, ctypes.c_size_t]  # stream, err, err_len
+    space = [ctypes.c_void_p, ctypes.c_size_t]
+    lib.tnr_operators_version.restype = ctypes.c_int
+    lib.tnr_operators_version.argtypes = []
+    for name, struct in (("embedding", Embedding), ("structure", StructureAttention),
+                         ("neighbor", NeighborAttention)):
+        forward = getattr(lib, f"tnr_{name}_forward")
+        forward.restype = ctypes.c_int
+        forward.argtypes = [ctypes.POINTER(struct), *(space if name == "structure" else []), *tail]
+        backward = getattr(lib, f"tnr_{name}_backward")
+        backward.restype = ctypes.c_int
+        backward.argtypes = [ctypes.POINTER(struct), *space, *tail]
+    for name, struct in (("embedding_workspace_size", Embedding),
+                         ("structure_tiles_size", StructureAttention),
+                         ("structure_forward_workspace_size", StructureAttention),
+                         ("structure_backward_workspace_size", StructureAttention),
+                         ("neighbor_rows_size", NeighborList),
+                         ("neighbor_rows_workspace_size", NeighborList),
+                         ("neighbor_backward_workspace_size", NeighborAttention)):
+        size = getattr(lib, f"tnr_{name}")
+        size.restype = ctypes.c_size_t
+        size.argtypes = [ctypes.POINTER(struct)]
+    lib.tnr_neighbor_rows.restype = ctypes.c_int
+    lib.tnr_neighbor_rows.argtypes = [ctypes.POINTER(NeighborList), *space, *tail]
+    version = lib.tnr_operators_version()
+    if version != OPERATORS_VERSION:
+        raise ImportError(
+            f"libtonari_hip.so has operators version {version}, expected {OPERATORS_VERSION}; "
+            "rebuild it"
+        )
+
+
 def open_library(path: str = LIBRARY) -> ctypes.CDLL:
     """Open the shared library and declare every exported signature."""
     if not os.path.exists(path):
@@ -201,6 +356,7 @@ def open_library(path: str = LIBRARY) -> ctypes.CDLL:
         raise ImportError(
             f"libtonari_hip.so has ABI version {version}, expected {ABI_VERSION}; rebuild it"
         )
+    _declare_operators(lib)
     return lib
 
 

@@ -53,12 +53,16 @@ struct SortKeys {
     __device__ __forceinline__ int operator()(int64_t i) const { return key[i]; }
 };
 
-// counts[digit * stride + tile]
+// counts[digit * stride + tile]; and `clear`, which a later kernel wants zero.
 template <typename Keys>
 __global__ __launch_bounds__(kSortThreads) void k_sort_count(Keys keys, int64_t n, SortPass pass,
-                                                             int32_t* counts) {
+                                                             int32_t* counts, int32_t* clear,
+                                                             int64_t clear_words) {
     __shared__ int32_t hist[kSortRadix];
     const int radix = 1 << pass.bits;
+    for (int64_t w = (int64_t)blockIdx.x * kSortThreads + threadIdx.x; w < clear_words;
+         w += (int64_t)gridDim.x * kSortThreads)
+        clear[w] = 0;
     for (int d = threadIdx.x; d < radix; d += kSortThreads) hist[d] = 0;
     __syncthreads();
     const int64_t tile = xcd_order(blockIdx.x, gridDim.x), base = tile * kSortTile;

@@ -41,8 +41,7 @@ struct StructureTile {
 };
 
 struct StructureArgs {
-    const StructureTile* q_tiles;
-    const StructureTile* k_tiles;
+    StructureTile *q_tiles, *k_tiles;
     const void *q, *k, *v;
     int64_t q_stride[2], k_stride[2], v_stride[2];
     const float *x_q, *x_k, *slopes;
@@ -125,6 +124,16 @@ __global__ __launch_bounds__(256) void k_structure_tiles(const int64_t* q_ptr, c
 // row_of(i, half).
 __device__ __forceinline__ int row_of(int i, int half) { return 8 * (i / 4) + 4 * half + i % 4; }
 
+// The value at a lane's own row and column of a 32 x 32 result.
+__device__ __forceinline__ float diagonal(const f32x16& all) {
+    const int lane = lane_of();
+    float x = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+        if (row_of(i, lane / 32) == lane % 32) x = all[i];
+    return sum_halves(x);  // the other half's lane has none
+}
+
 template <typename T>
 struct Mat;
 
@@ -153,13 +162,13 @@ struct Mat16 {
                 if (p && c < dim) x[s] = *(const Frag*)(p + c);
             }
         }
+        // Row for row, by the matrix product that also makes a query's product
+        // with a value: equal rows give equal bits.
         __device__ __forceinline__ float dot(const Row& o) const {
-            float sum = 0.f;
+            f32x16 all{};
 #pragma unroll
-            for (int s = 0; s < DP / 16; ++s)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) sum = fmaf((float)x[s][e], (float)o.x[s][e], sum);
-            return sum_halves(sum);
+            for (int s = 0; s < DP / 16; ++s) all = F::mma(o.x[s], x[s], all);
+            return diagonal(all);
         }
         __device__ __forceinline__ float largest() const {
             float top = 0.f;
@@ -270,12 +279,13 @@ struct Mat<float> {
             }
         }
         __device__ __forceinline__ float dot(const Row& o) const {
-            float sum = 0.f;
+            f32x16 all{};
 #pragma unroll
             for (int s = 0; s < DP / 8; ++s)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sum = fmaf(x[s][e], o.x[s][e], sum);
-            return sum_halves(sum);
+                for (int e = 0; e < 4; ++e)
+                    all = __builtin_amdgcn_mfma_f32_32x32x2f32(o.x[s][e], x[s][e], all, 0, 0, 0);
+            return diagonal(all);
         }
         __device__ __forceinline__ float largest() const { return 1.f; }
     };

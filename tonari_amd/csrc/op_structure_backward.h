@@ -197,6 +197,7 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP <= 32 ? 64 : 2 * DP)) v
             for (int e = 0; e < 4; ++e) {
                 const int i = 4 * run + e;
                 ds[e] = s[e] * (dp[i] - delta);
+                w[0] += ds[e];
                 float dx_i = CAP ? ds[e] * bend[e] : ds[e];
                 if (kNarrow<T>) dx_i *= unit;
                 p.set(i, dx_i);
@@ -208,7 +209,6 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP <= 32 ? 64 : 2 * DP)) v
                 for (int e = 0; e < 4; ++e) {
                     const float over = r[e] > 0.f ? __builtin_amdgcn_rcpf(r[e]) : 0.f;
                     const float wd = ds[e] * over, wp = s[e] * over;
-                    w[0] += ds[e];
                     w[1] = fmaf(wd, dx[e], w[1]);
                     w[2] = fmaf(wd, dy[e], w[2]);
                     w[3] = fmaf(wd, dz[e], w[3]);
@@ -519,11 +519,22 @@ __global__ __launch_bounds__(256) void k_structure_join_dkv(const StructureArgs 
         a.push_k[3 * at + c - 2 * a.dim] = sum;
 }
 
-// Sums over the heads of the positions' gradients, threads over atoms and axes.
-__global__ __launch_bounds__(256) void k_structure_finish(const StructureArgs a, float* grad_x_q,
-                                                          float* grad_x_k, int shared) {
+// Sums over the heads of the positions' gradients, threads over atoms and axes;
+// where slopes are wanted, the first `heads` workgroups sum their rows.
+__global__ __launch_bounds__(1024) void k_structure_finish(const StructureArgs a, float* grad_x_q,
+                                                           float* grad_x_k, float* grad_slopes,
+                                                           int shared) {
+    int64_t block = blockIdx.x;
+    if (grad_slopes) {
+        if (block < a.heads) {
+            const float sum = block_sum(a.turn + block * a.n_queries, a.n_queries);
+            if (threadIdx.x == 0) grad_slopes[block] = sum;
+            return;
+        }
+        block -= a.heads;
+    }
     const int64_t nk = 3 * (int64_t)a.n_keys, nq = 3 * (int64_t)a.n_queries;
-    int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    int64_t i = block * 1024 + threadIdx.x;
     if (grad_x_k) {
         if (i < nk) {
             float sum = 0.f;

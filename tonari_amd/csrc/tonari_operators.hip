@@ -134,10 +134,10 @@ EmbeddingSpace embedding_space(const tnr_embedding& r, void* base) {
 // A pass over `keys`, whose items `put` writes.
 template <typename Keys, typename Put>
 void sort_pass(Keys keys, int64_t n, SortPass pass, int32_t* counts, int32_t* totals, Put put,
-               hipStream_t stream) {
+               hipStream_t stream, int32_t* clear = nullptr, int64_t clear_words = 0) {
     const unsigned tiles = (unsigned)sort_tiles(n);
     const int radix = 1 << pass.bits;
-    k_sort_count<<<tiles, kSortThreads, 0, stream>>>(keys, n, pass, counts);
+    k_sort_count<<<tiles, kSortThreads, 0, stream>>>(keys, n, pass, counts, clear, clear_words);
     k_sort_scan<<<(radix + kSortWaves - 1) / kSortWaves, kSortThreads, 0, stream>>>(
         counts, tiles, radix, totals);
     k_sort_move<<<tiles, kSortThreads, 0, stream>>>(keys, n, pass, counts, totals, put);
@@ -151,7 +151,8 @@ void sort_species(const tnr_embedding& r, const EmbeddingSpace& s, RunArgs& runs
     for (int p = 0; p < plan.passes; ++p) {
         if (p == 0)
             sort_pass(SpeciesOf<I>{(const I*)r.species, r.n_species}, r.n_atoms, plan.pass[p],
-                      s.counts, s.totals, PutAtom{s.key[0], s.atom[0]}, stream);
+                      s.counts, s.totals, PutAtom{s.key[0], s.atom[0]}, stream, (int32_t*)s.runs,
+                      2 * r.n_species);
         else {
             sort_pass(SortKeys{s.key[from]}, r.n_atoms, plan.pass[p], s.counts, s.totals,
                       MoveAtom{s.atom[from], s.key[1 - from], s.atom[1 - from]}, stream);
@@ -235,6 +236,8 @@ int check_structure(const tnr_structure_attention* r, bool backward, char* err, 
     if (r->n_structures < 0 || r->n_queries < 0 || r->n_keys < 0 ||
         (r->n_structures == 0 && (r->n_queries > 0 || r->n_keys > 0)))
         return refuse(err, len, "invalid sizes");
+    if (!r->query_positions && r->n_queries != r->n_keys)
+        return refuse(err, len, "queries of their own need positions of their own");
     if (r->n_queries >= INT32_MAX / r->heads || r->n_keys >= INT32_MAX / r->kv_heads ||
         r->n_structures >= INT32_MAX)
         return refuse(err, len, "too many atoms");
@@ -244,7 +247,9 @@ int check_structure(const tnr_structure_attention* r, bool backward, char* err, 
         return refuse(err, len, "too many atoms");
     if (r->n_structures > 0 && (!r->query_ptr || !r->key_ptr))
         return refuse(err, len, "required pointers are null");
-    if (!r->slopes || (r->n_queries > 0 && (!r->q || !r->query_positions || !r->out)) ||
+    if (r->n_structures > 0 && (!r->tiles || (uintptr_t)r->tiles % 256 != 0))
+        return refuse(err, len, "tiles must be given and aligned to 256 bytes");
+    if (!r->slopes || (r->n_queries > 0 && (!r->q || !r->out)) ||
         (r->n_keys > 0 && (!r->k || !r->v || !r->positions)))
         return refuse(err, len, "required pointers are null");
     if (!aligned(r->q, r->q_stride, r->dtype) || !aligned(r->k, r->k_stride, r->dtype) ||
@@ -257,12 +262,24 @@ int check_structure(const tnr_structure_attention* r, bool backward, char* err, 
         if ((uintptr_t)r->grad_out % 16 != 0 || (uintptr_t)r->grad_q % 16 != 0 ||
             (uintptr_t)r->grad_k % 16 != 0 || (uintptr_t)r->grad_v % 16 != 0)
             return refuse(err, len, "gradients must be aligned to 16 bytes");
+        if (r->grad_query_positions && !r->query_positions)
+            return refuse(err, len, "the queries' positions are the keys'");
     }
     return TNR_OK;
 }
 
+// The batch's tiles: the queries', and the keys' for the backward.
+size_t q_tile_bytes(const StructurePlan& p) {
+    return padded((size_t)p.q_tiles * sizeof(StructureTile));
+}
+size_t k_tile_bytes(const StructurePlan& p) {
+    return padded((size_t)p.k_tiles * sizeof(StructureTile));
+}
+
 StructureArgs structure_args(const tnr_structure_attention& r, const StructurePlan& p) {
     StructureArgs a{};
+    a.q_tiles = (StructureTile*)r.tiles;
+    a.k_tiles = (StructureTile*)((char*)r.tiles + q_tile_bytes(p));
     a.q = r.q;
     a.k = r.k;
     a.v = r.v;
@@ -271,7 +288,7 @@ StructureArgs structure_args(const tnr_structure_attention& r, const StructurePl
         a.k_stride[i] = r.k_stride[i];
         a.v_stride[i] = r.v_stride[i];
     }
-    a.x_q = r.query_positions;
+    a.x_q = r.query_positions ? r.query_positions : r.positions;
     a.x_k = r.positions;
     a.slopes = r.slopes;
     a.rule = ScoreRule::of(r.scale, r.softcap);
@@ -292,9 +309,7 @@ StructureArgs structure_args(const tnr_structure_attention& r, const StructurePl
     return a;
 }
 
-// Where the batch has no tile table of its own size, the pointers into it.
 struct StructureSpace {
-    StructureTile *q_tiles, *k_tiles;
     float *part, *part_k, *row, *push_q, *push_k, *turn;
     size_t bytes;
 };
@@ -308,11 +323,9 @@ StructureSpace structure_space(const tnr_structure_attention& r, const Structure
     };
     const size_t rows = (size_t)r.heads * r.n_queries;
     StructureSpace s{};
-    s.q_tiles = (StructureTile*)part((size_t)p.q_tiles * sizeof(StructureTile));
     if (p.splits > 1)
         s.part = (float*)part(rows * p.splits * (r.dim + (backward ? kRowSums : 2)) * 4);
     if (backward) {
-        s.k_tiles = (StructureTile*)part((size_t)p.k_tiles * sizeof(StructureTile));
         if (p.k_splits > 1)
             s.part_k = (float*)part((size_t)r.kv_heads * r.n_keys * p.k_splits *
                                     (2 * r.dim + 3) * 4);
@@ -327,12 +340,12 @@ StructureSpace structure_space(const tnr_structure_attention& r, const Structure
     return s;
 }
 
-void lay_tiles(const tnr_structure_attention& r, const StructurePlan& p, const StructureSpace& s,
-               hipStream_t stream) {
+void lay_tiles(const tnr_structure_attention& r, const StructurePlan& p, const StructureArgs& a,
+               bool keys, hipStream_t stream) {
     const int64_t blocks = (r.n_structures + 3) / 4;
     k_structure_tiles<<<(unsigned)(blocks < 64 ? blocks : 64), 256, 0, stream>>>(
         r.query_ptr, r.key_ptr, r.n_structures, r.n_queries, r.n_keys, p.group, p.q_waves * kTile,
-        p.k_waves * kTile, s.q_tiles, s.k_tiles);
+        p.k_waves * kTile, a.q_tiles, keys ? a.k_tiles : nullptr);
 }
 
 template <typename F>
@@ -555,8 +568,9 @@ int tnr_embedding_backward(const tnr_embedding* req, void* workspace, size_t wor
     runs.runs = s.runs;
     runs.partial = s.partial;
     runs.each = embedding_each(r.n_atoms);
-    zero(s.runs, (size_t)r.n_species * 8, st);
-    if (r.n_atoms > 0) {
+    if (r.n_atoms == 0) {
+        zero(s.runs, (size_t)r.n_species * 8, st);
+    } else {
         if (r.index_bytes == 4)
             sort_species<int32_t>(r, s, runs, st);
         else
@@ -588,8 +602,16 @@ int tnr_embedding_backward(const tnr_embedding* req, void* workspace, size_t wor
     return launched(err, err_len);
 }
 
+size_t tnr_structure_tiles_size(const tnr_structure_attention* req) {
+    if (!req || req->n_structures < 0 || req->n_queries < 0 || req->n_keys < 0 || req->heads < 1 ||
+        req->kv_heads < 1 || req->heads % req->kv_heads != 0)
+        return 0;
+    const StructurePlan p = structure_plan(*req);
+    return q_tile_bytes(p) + k_tile_bytes(p);
+}
+
 size_t tnr_structure_forward_workspace_size(const tnr_structure_attention* req) {
-    if (check_structure(req, false, nullptr, 0) != TNR_OK) return 0;
+    if (tnr_structure_tiles_size(req) == 0) return 0;
     return structure_space(*req, structure_plan(*req), false, nullptr).bytes;
 }
 
@@ -598,16 +620,16 @@ int tnr_structure_forward(const tnr_structure_attention* req, void* workspace,
     const int code = check_structure(req, false, err, err_len);
     if (code != TNR_OK) return code;
     const tnr_structure_attention& r = *req;
-    if (r.n_queries == 0) return TNR_OK;
+    if (r.n_structures == 0) return TNR_OK;
     const StructurePlan p = structure_plan(r);
     const StructureSpace s = structure_space(r, p, false, workspace);
-    if (!workspace || (uintptr_t)workspace % 256 != 0 || workspace_bytes < s.bytes)
+    if (s.bytes > 0 && (!workspace || (uintptr_t)workspace % 256 != 0 || workspace_bytes < s.bytes))
         return refuse(err, err_len, "workspace is too small or not aligned to 256 bytes");
     const hipStream_t st = (hipStream_t)stream;
     StructureArgs a = structure_args(r, p);
-    a.q_tiles = s.q_tiles;
     a.part = s.part;
-    lay_tiles(r, p, s, st);
+    lay_tiles(r, p, a, r.lse != nullptr, st);
+    if (r.n_queries == 0) return launched(err, err_len);
     with_type(r.dtype, [&](auto t) {
         using T = decltype(t);
         with_dim(r.dim, [&](auto d) {
@@ -627,7 +649,7 @@ int tnr_structure_forward(const tnr_structure_attention* req, void* workspace,
 }
 
 size_t tnr_structure_backward_workspace_size(const tnr_structure_attention* req) {
-    if (check_structure(req, false, nullptr, 0) != TNR_OK) return 0;
+    if (tnr_structure_tiles_size(req) == 0) return 0;
     return structure_space(*req, structure_plan(*req), true, nullptr).bytes;
 }
 
@@ -638,19 +660,16 @@ int tnr_structure_backward(const tnr_structure_attention* req, void* workspace,
     const tnr_structure_attention& r = *req;
     const StructurePlan p = structure_plan(r);
     const StructureSpace s = structure_space(r, p, true, workspace);
-    if (!workspace || (uintptr_t)workspace % 256 != 0 || workspace_bytes < s.bytes)
+    if (s.bytes > 0 && (!workspace || (uintptr_t)workspace % 256 != 0 || workspace_bytes < s.bytes))
         return refuse(err, err_len, "workspace is too small or not aligned to 256 bytes");
     const hipStream_t st = (hipStream_t)stream;
     StructureArgs a = structure_args(r, p);
-    a.q_tiles = s.q_tiles;
-    a.k_tiles = s.k_tiles;
     a.part = s.part;
     a.part_k = s.part_k;
     a.row = s.row;
     a.push_q = s.push_q;
     a.push_k = s.push_k;
     a.turn = s.turn;
-    if (r.n_structures > 0) lay_tiles(r, p, s, st);
     with_type(r.dtype, [&](auto t) {
         using T = decltype(t);
         with_dim(r.dim, [&](auto d) {
@@ -680,14 +699,13 @@ int tnr_structure_backward(const tnr_structure_attention* req, void* workspace,
                        st>>>(a);
         });
     });
-    const int shared = r.grad_positions && !r.grad_query_positions &&
-                       r.query_positions == r.positions && r.n_queries == r.n_keys;
+    const int shared = !r.query_positions;
     const int64_t items = (r.grad_positions ? 3 * r.n_keys : 0) +
-                    (r.grad_query_positions ? 3 * r.n_queries : 0);
-    if (items > 0)
-        k_structure_finish<<<(unsigned)((items + 255) / 256), 256, 0, st>>>(
-            a, r.grad_query_positions, r.grad_positions, shared);
-    if (r.grad_slopes) k_slopes<<<r.heads, 1024, 0, st>>>(a.turn, r.n_queries, r.grad_slopes);
+                          (r.grad_query_positions ? 3 * r.n_queries : 0);
+    const int64_t blocks = (items + 1023) / 1024 + (r.grad_slopes ? r.heads : 0);
+    if (blocks > 0)
+        k_structure_finish<<<(unsigned)blocks, 1024, 0, st>>>(a, r.grad_query_positions,
+                                                              r.grad_positions, r.grad_slopes, shared);
     return launched(err, err_len);
 }
 

@@ -192,15 +192,16 @@ variable_list graph_of(const Tensor& out, const Tensor& upstream, const variable
 // ------------------------------------------------------ structure attention
 
 struct StructureCall {
-    Tensor q, k, v, query_positions, positions, slopes, query_ptr, key_ptr;
+    Tensor q, k, v, query_positions, positions, slopes, query_ptr, key_ptr, tiles;
     tnr_structure_attention r{};
 
     StructureCall(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& x,
                   const Tensor& slopes_, const Tensor& x_q, const Tensor& batch_ptr,
-                  const Tensor& query_ptr_, double scale, double softcap)
+                  const Tensor& query_ptr_, double scale, double softcap,
+                  const Tensor& tiles_ = Tensor())
         : q(laid(q_)), k(laid(k_)), v(laid(v_)), positions(x.detach().contiguous()),
           slopes(slopes_.detach().contiguous()), key_ptr(batch_ptr.contiguous()) {
-        query_positions = x_q.defined() ? x_q.detach().contiguous() : positions;
+        if (x_q.defined()) query_positions = x_q.detach().contiguous();
         query_ptr = query_ptr_.defined() ? query_ptr_.contiguous() : key_ptr;
         r.dtype = code_of(q);
         r.heads = (int32_t)q.size(1);
@@ -217,11 +218,13 @@ struct StructureCall {
         set_strides(r.q_stride, q);
         set_strides(r.k_stride, k);
         set_strides(r.v_stride, v);
-        r.query_positions = (const float*)query_positions.data_ptr();
+        if (x_q.defined()) r.query_positions = (const float*)query_positions.data_ptr();
         r.positions = (const float*)positions.data_ptr();
         r.slopes = (const float*)slopes.data_ptr();
         r.scale = (float)scale;
         r.softcap = (float)softcap;
+        tiles = tiles_.defined() ? tiles_ : bytes_on(q, tnr_structure_tiles_size(&r));
+        r.tiles = tiles.data_ptr();
     }
 };
 
@@ -250,7 +253,8 @@ struct StructureAttention : torch::autograd::Function<StructureAttention> {
         StructureCall c(q, k, v, x, slopes, x_q, batch_ptr, query_ptr, scale, softcap);
         Tensor lse;
         const Tensor out = structure_forward(c, &lse);
-        ctx->save_for_backward({q, k, v, x, slopes, x_q, batch_ptr, query_ptr, out, lse});
+        ctx->save_for_backward(
+            {q, k, v, x, slopes, x_q, batch_ptr, query_ptr, out, lse, c.tiles});
         ctx->saved_data["scale"] = scale;
         ctx->saved_data["softcap"] = softcap;
         return out;
@@ -288,7 +292,7 @@ struct StructureAttention : torch::autograd::Function<StructureAttention> {
             for (size_t i = 0; i < 6; ++i) all[i] = found[i];
             return all;
         }
-        StructureCall c(s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], scale, softcap);
+        StructureCall c(s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], scale, softcap, s[10]);
         const Tensor &out = s[8], &lse = s[9];
         const Tensor go = flat(grads[0]);
         c.r.out = out.data_ptr();
