@@ -237,6 +237,18 @@ def test_gradient_of_the_gradient():
         assert_near(a, e, name)
 
 
+def test_inputs_that_depend_on_each_other():
+    # q and d of one tensor: the graph's gradient takes each path once
+    i, j = random_list(20, 20, 6, seed=9)
+    c = make(i, j, 20, 20, 2, 1, 16, torch.float32, grad=False)
+    found = []
+    for graph in (False, True):
+        x = c["d"].detach().clone().requires_grad_()
+        d = dict(c, d=x, q=c["q"] * x.sum() * 0.01, v=c["v"] * x.mean())
+        found.append(torch.autograd.grad(call(d, 5.0), x, c["upstream"], create_graph=graph)[0])
+    assert_near(found[1], found[0])
+
+
 @pytest.mark.parametrize("i,j", [
     ([0, 1, 0], [1, 0, 2]),          # the pairs of 0 do not lie together
     ([0, 0, 3], [1, 2, 0]),          # no such source

@@ -304,6 +304,19 @@ def test_gradient_of_the_gradient():
         assert_near(a, e, name)
 
 
+def test_inputs_that_depend_on_each_other():
+    # q, k and v of the positions: the graph's gradient takes each path once
+    c = make([9, 0, 14], 2, 1, 16, torch.float32, seed=19, grad=False)
+    g = torch.Generator().manual_seed(2)
+    mix = [torch.randn(3, h * 16, generator=g).to(DEV) * 0.3 for h in (2, 1, 1)]
+    found = []
+    for graph in (False, True):
+        x = c["positions"].detach().clone().requires_grad_()
+        d = dict(c, positions=x, **{n: (x @ m).view(23, -1, 16) for n, m in zip("qkv", mix)})
+        found.append(torch.autograd.grad(call(d, 5.0), x, c["upstream"], create_graph=graph)[0])
+    assert_near(found[1], found[0])
+
+
 @pytest.mark.parametrize("ptr", [[0, 5, 3, 10], [1, 5, 7, 10], [0, 5, 7, 9], [0, 5, 7, 11]])
 def test_wrong_pointers_are_nan(ptr):
     c = make([10], 2, 2, 16, torch.float32, grad=False)

@@ -22,7 +22,8 @@ import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
-SOURCES = [os.path.join(HERE, "csrc", name) for name in ("tonari_hip.hip", "tonari_operators.hip")]
+SOURCES = [os.path.join(HERE, "csrc", name) for name in (
+    "tonari_hip.hip", "tonari_operators.hip", "tonari_structure.hip")]
 HEADERS = [os.path.join(HERE, "csrc", "nl_device.h"), os.path.join(ROOT, "include", "tonari_hip.h")]
 OUTPUT = os.path.join(HERE, "_lib", "libtonari_hip.so")
 CPU_SOURCES = [os.path.join(HERE, "csrc", "cpu", "nl_cpu.cpp")]
@@ -44,6 +45,7 @@ def command(output: str = OUTPUT, extra: list[str] | None = None) -> list[str]:
     return [
         hipcc(),
         f"--offload-arch={ARCH}",
+        f"-parallel-jobs={len(SOURCES)}",
         "-O3",
         "-std=c++17",
         "-fPIC",

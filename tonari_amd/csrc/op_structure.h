@@ -180,13 +180,17 @@ struct Mat16 {
         }
     };
 
-    // acc += tile . row^T
+    // acc += tile . row^T over the first `dim` channels
     template <int DP>
-    static __device__ __forceinline__ void rows(f32x16& acc, const T* tile, const Row<DP>& b) {
+    static __device__ __forceinline__ void rows(f32x16& acc, const T* tile, const Row<DP>& b,
+                                                int dim) {
         const int lane = lane_of();
         const T* p = tile + (lane % 32) * (DP + 8) + 8 * (lane / 32);
 #pragma unroll
-        for (int s = 0; s < DP / 16; ++s) acc = F::mma(*(const Frag*)(p + 16 * s), b.x[s], acc);
+        for (int s = 0; s < DP / 16; ++s) {
+            if (16 * s > DP - 32 && 16 * s >= dim) break;
+            acc = F::mma(*(const Frag*)(p + 16 * s), b.x[s], acc);
+        }
     }
 
     // A lane's 16 weights of a tile, rounded for the second product.
@@ -260,7 +264,8 @@ struct Mat<f16> : Mat16<f16, MmaF16> {};
 
 // 32-bit products: two channels to an instruction, of which the lower lanes
 // take those of the row's first half and the upper lanes the second's, so that
-// a lane reads neighbouring floats.
+// a lane reads neighbouring floats.  They run at a sixteenth of the 16-bit rate
+// and bound the 32-bit kernels, so channels beyond `dim` are left out.
 template <>
 struct Mat<float> {
     static constexpr int kRows(int dp) { return kTile * (dp + 4); }
@@ -273,9 +278,9 @@ struct Mat<float> {
             const int half = lane_of() / 32;
 #pragma unroll
             for (int s = 0; s < DP / 8; ++s) {
-                const int c = half * (DP / 2) + 4 * s;
                 x[s] = Vec<float, 4>{};
-                if (p && c < dim) x[s] = *(const Vec<float, 4>*)(p + c);
+                if (p && 8 * s < dim)
+                    x[s] = *(const Vec<float, 4>*)(p + half * (dim / 2) + 4 * s);
             }
         }
         __device__ __forceinline__ float dot(const Row& o) const {
@@ -291,11 +296,13 @@ struct Mat<float> {
     };
 
     template <int DP>
-    static __device__ __forceinline__ void rows(f32x16& acc, const float* tile, const Row<DP>& b) {
+    static __device__ __forceinline__ void rows(f32x16& acc, const float* tile, const Row<DP>& b,
+                                                int dim) {
         const int lane = lane_of();
-        const float* p = tile + (lane % 32) * (DP + 4) + (lane / 32) * (DP / 2);
+        const float* p = tile + (lane % 32) * (DP + 4) + (lane / 32) * (dim / 2);
 #pragma unroll
         for (int s = 0; s < DP / 8; ++s) {
+            if (8 * s > DP - 32 && 8 * s >= dim) break;
             const Vec<float, 4> a = *(const Vec<float, 4>*)(p + 4 * s);
 #pragma unroll
             for (int e = 0; e < 4; ++e)
@@ -572,7 +579,7 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP)) void k_structure_forw
     // then change their unit), so that most tiles neither subtract nor rescale.
     const auto weigh = [&](int sub, int left) {
         f32x16 dot{};
-        M::template rows<DP>(dot, k_rows + sub * Pair::kRows, qr);
+        M::template rows<DP>(dot, k_rows + sub * Pair::kRows, qr, a.dim);
         float s[16], unused[4];
         const float ref = top == -inf_of() ? 0.f : top;
         const bool near = all_near<CAP>(dot, a.rule);

@@ -165,8 +165,8 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP <= 32 ? 64 : 2 * DP)) v
     };
     const auto push = [&](int sub, int left) {
         f32x16 dot{}, dp{};
-        M::template rows<DP>(dot, k_rows + sub * Pair::kRows, qr);
-        M::template rows<DP>(dp, v_rows + sub * Pair::kRows, dor);
+        M::template rows<DP>(dot, k_rows + sub * Pair::kRows, qr, a.dim);
+        M::template rows<DP>(dp, v_rows + sub * Pair::kRows, dor, a.dim);
         typename M::Weights p, rest;
         const bool near = all_near<CAP>(dot, a.rule);
 #pragma unroll
@@ -373,8 +373,8 @@ k_structure_dkv(const StructureArgs a) {
     const auto pull = [&](int sub, float slope) {
         const float slope2 = slope * kLog2e;
         f32x16 dot{}, dp{};
-        M::template rows<DP>(dot, q_rows + sub * Pair::kRows, kr);
-        M::template rows<DP>(dp, o_rows + sub * Pair::kRows, vr);
+        M::template rows<DP>(dot, q_rows + sub * Pair::kRows, kr, a.dim);
+        M::template rows<DP>(dp, o_rows + sub * Pair::kRows, vr, a.dim);
         typename M::Weights p, dx;
         const bool near = all_near<CAP>(dot, a.rule);
         float unit = 1.f;

@@ -1,49 +1,13 @@
-// C ABI of the operators (include/tonari_operators.h): checks of requests,
-// workspaces and launches.  Every call returns a code; no exception crosses it.
+// C ABI of the species embedding and of neighbor attention
+// (include/tonari_operators.h): checks of requests, workspaces and launches.
+// Every call returns a code; no exception crosses it.
 #include "op_embedding.h"
+#include "op_host.h"
 #include "op_neighbor.h"
-#include "op_structure_backward.h"
-
-#include <cstdio>
 
 using namespace tnr::op;
 
 namespace {
-
-int refuse(char* err, size_t len, const char* message) {
-    if (err && len) std::snprintf(err, len, "%s", message);
-    return TNR_INPUT_ERROR;
-}
-
-int launched(char* err, size_t len) {
-    const hipError_t e = hipGetLastError();
-    if (e == hipSuccess) return TNR_OK;
-    if (err && len) std::snprintf(err, len, "HIP error: %s", hipGetErrorString(e));
-    return TNR_DEVICE_ERROR;
-}
-
-bool is_type(int32_t dtype) {
-    return dtype == TNR_FLOAT32 || dtype == TNR_BFLOAT16 || dtype == TNR_FLOAT16;
-}
-size_t size_of(int32_t dtype) { return dtype == TNR_FLOAT32 ? 4 : 2; }
-size_t padded(size_t bytes) { return (bytes + 255) / 256 * 256; }
-
-template <typename F>
-void with_type(int32_t dtype, F&& f) {
-    if (dtype == TNR_FLOAT32)
-        f(float{});
-    else if (dtype == TNR_BFLOAT16)
-        f(bf16{});
-    else
-        f(f16{});
-}
-template <int N>
-struct Int {
-    static constexpr int value = N;
-};
-
-// A launch of more than 2^32 threads is not possible.
-constexpr int64_t kMostThreads = (int64_t(1) << 32) - 1;
 
 void zero(void* p, size_t bytes, hipStream_t stream) {
     const int64_t words = (int64_t)(bytes / 4);
@@ -161,216 +125,6 @@ void sort_species(const tnr_embedding& r, const EmbeddingSpace& s, RunArgs& runs
     }
     runs.key = s.key[from];
     runs.atom = s.atom[from];
-}
-
-// ------------------------------------------------------------------ attention
-
-int check_heads(int32_t dtype, int32_t heads, int32_t kv_heads, int32_t dim, float scale,
-                float softcap, char* err, size_t len) {
-    if (!is_type(dtype)) return refuse(err, len, "dtype must be float32, bfloat16 or float16");
-    if (heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || heads > 1024)
-        return refuse(err, len, "heads must be a multiple of the key and value heads, at most 1024");
-    if (dim < 8 || dim > 128 || dim % 8 != 0)
-        return refuse(err, len, "the head dimension must be a multiple of 8, from 8 to 128");
-    if (!std::isfinite(scale)) return refuse(err, len, "scale must be finite");
-    if (!std::isfinite(softcap) || softcap < 0.f)
-        return refuse(err, len, "softcap must be finite and positive");
-    return TNR_OK;
-}
-
-// Rows of a tile are found by 32-bit offsets.
-constexpr int64_t kMostStride = int64_t(1) << 24;
-bool aligned(const void* p, const int64_t (&stride)[2], int32_t dtype) {
-    const int64_t unit = 16 / (int64_t)size_of(dtype);
-    for (const int64_t s : stride)
-        if (s % unit != 0 || s < 0 || s > kMostStride) return false;
-    return (uintptr_t)p % 16 == 0;
-}
-
-// ------------------------------------------------------- structure attention
-
-// Waves of 32 rows in a workgroup, which share the staged keys.  With long
-// structures four; with short ones two, of which fewer lie beyond a structure's
-// end: 1,024 molecules of 20 to 120 atoms take 73 us at two and 84 at four, a
-// cluster of 4,001 atoms 246 us at four and 286 at two (its queries' gradients).
-int waves_for(int64_t rows, int64_t structures) {
-    const int64_t mean = structures > 0 ? rows / structures : 0;
-    return mean <= 512 ? 2 : 4;
-}
-
-struct StructurePlan {
-    int group, q_waves, k_waves, splits, k_splits;
-    int64_t q_tiles, k_tiles;
-};
-
-constexpr int64_t kSplitWaves = 3072;
-
-StructurePlan structure_plan(const tnr_structure_attention& r) {
-    StructurePlan p{};
-    p.group = r.heads / r.kv_heads;
-    p.q_waves = waves_for(r.n_queries * p.group, r.n_structures);
-    p.k_waves = waves_for(r.n_keys, r.n_structures);
-    p.q_tiles = tile_start(r.n_queries, p.group, p.q_waves * kTile, r.n_structures);
-    p.k_tiles = tile_start(r.n_keys, 1, p.k_waves * kTile, r.n_structures);
-    // Few rows: the keys (or, for the keys' gradients, the rows) are split over
-    // workgroups, at least 8 tiles each, until there are waves enough for the
-    // device.
-    const auto split = [&](int64_t rows, int64_t others) {
-        const int64_t waves = (rows / kTile + r.n_structures) * r.kv_heads;
-        const int64_t most = r.n_structures > 0 ? others / r.n_structures / (8 * kTile) : 0;
-        int64_t n = waves > 0 ? kSplitWaves / waves : 1;
-        if (n > most) n = most;
-        if (n > 64) n = 64;
-        return n < 2 ? 1 : (int)n;
-    };
-    p.splits = split(r.n_queries * p.group, r.n_keys);
-    p.k_splits = split(r.n_keys, r.n_queries * p.group);
-    return p;
-}
-
-int check_structure(const tnr_structure_attention* r, bool backward, char* err, size_t len) {
-    if (!r) return refuse(err, len, "request is null");
-    const int code = check_heads(r->dtype, r->heads, r->kv_heads, r->dim, r->scale, r->softcap, err,
-                                 len);
-    if (code != TNR_OK) return code;
-    if (r->n_structures < 0 || r->n_queries < 0 || r->n_keys < 0 ||
-        (r->n_structures == 0 && (r->n_queries > 0 || r->n_keys > 0)))
-        return refuse(err, len, "invalid sizes");
-    if (!r->query_positions && r->n_queries != r->n_keys)
-        return refuse(err, len, "queries of their own need positions of their own");
-    if (r->n_queries >= INT32_MAX / r->heads || r->n_keys >= INT32_MAX / r->kv_heads ||
-        r->n_structures >= INT32_MAX)
-        return refuse(err, len, "too many atoms");
-    const StructurePlan p = structure_plan(*r);
-    if (p.q_tiles * p.q_waves * kWave > kMostThreads || p.k_tiles * p.k_waves * kWave > kMostThreads ||
-        (int64_t)r->kv_heads * p.splits > 65535)
-        return refuse(err, len, "too many atoms");
-    if (r->n_structures > 0 && (!r->query_ptr || !r->key_ptr))
-        return refuse(err, len, "required pointers are null");
-    if (r->n_structures > 0 && (!r->tiles || (uintptr_t)r->tiles % 256 != 0))
-        return refuse(err, len, "tiles must be given and aligned to 256 bytes");
-    if (!r->slopes || (r->n_queries > 0 && (!r->q || !r->out)) ||
-        (r->n_keys > 0 && (!r->k || !r->v || !r->positions)))
-        return refuse(err, len, "required pointers are null");
-    if (!aligned(r->q, r->q_stride, r->dtype) || !aligned(r->k, r->k_stride, r->dtype) ||
-        !aligned(r->v, r->v_stride, r->dtype) || (uintptr_t)r->out % 16 != 0)
-        return refuse(err, len, "q, k, v and out must be aligned to 16 bytes, with strides up to 2^24");
-    if (backward) {
-        if ((r->n_queries > 0 && (!r->grad_out || !r->grad_q || !r->lse)) ||
-            (r->n_keys > 0 && (!r->grad_k || !r->grad_v)))
-            return refuse(err, len, "required pointers are null");
-        if ((uintptr_t)r->grad_out % 16 != 0 || (uintptr_t)r->grad_q % 16 != 0 ||
-            (uintptr_t)r->grad_k % 16 != 0 || (uintptr_t)r->grad_v % 16 != 0)
-            return refuse(err, len, "gradients must be aligned to 16 bytes");
-        if (r->grad_query_positions && !r->query_positions)
-            return refuse(err, len, "the queries' positions are the keys'");
-    }
-    return TNR_OK;
-}
-
-// The batch's tiles: the queries', and the keys' for the backward.
-size_t q_tile_bytes(const StructurePlan& p) {
-    return padded((size_t)p.q_tiles * sizeof(StructureTile));
-}
-size_t k_tile_bytes(const StructurePlan& p) {
-    return padded((size_t)p.k_tiles * sizeof(StructureTile));
-}
-
-StructureArgs structure_args(const tnr_structure_attention& r, const StructurePlan& p) {
-    StructureArgs a{};
-    a.q_tiles = (StructureTile*)r.tiles;
-    a.k_tiles = (StructureTile*)((char*)r.tiles + q_tile_bytes(p));
-    a.q = r.q;
-    a.k = r.k;
-    a.v = r.v;
-    for (int i = 0; i < 2; ++i) {
-        a.q_stride[i] = r.q_stride[i];
-        a.k_stride[i] = r.k_stride[i];
-        a.v_stride[i] = r.v_stride[i];
-    }
-    a.x_q = r.query_positions ? r.query_positions : r.positions;
-    a.x_k = r.positions;
-    a.slopes = r.slopes;
-    a.rule = ScoreRule::of(r.scale, r.softcap);
-    a.heads = r.heads;
-    a.kv_heads = r.kv_heads;
-    a.group = p.group;
-    a.dim = r.dim;
-    a.n_queries = (int)r.n_queries;
-    a.n_keys = (int)r.n_keys;
-    a.splits = p.splits;
-    a.k_splits = p.k_splits;
-    a.out = r.out;
-    a.lse = r.lse;
-    a.grad_out = r.grad_out;
-    a.grad_q = r.grad_q;
-    a.grad_k = r.grad_k;
-    a.grad_v = r.grad_v;
-    return a;
-}
-
-struct StructureSpace {
-    float *part, *part_k, *row, *push_q, *push_k, *turn;
-    size_t bytes;
-};
-StructureSpace structure_space(const tnr_structure_attention& r, const StructurePlan& p,
-                               bool backward, void* base) {
-    size_t at = 0;
-    const auto part = [&](size_t bytes) {
-        char* q = (char*)base + at;
-        at += padded(bytes);
-        return q;
-    };
-    const size_t rows = (size_t)r.heads * r.n_queries;
-    StructureSpace s{};
-    if (p.splits > 1)
-        s.part = (float*)part(rows * p.splits * (r.dim + (backward ? kRowSums : 2)) * 4);
-    if (backward) {
-        if (p.k_splits > 1)
-            s.part_k = (float*)part((size_t)r.kv_heads * r.n_keys * p.k_splits *
-                                    (2 * r.dim + 3) * 4);
-        s.row = (float*)part(rows * 8);
-        if (r.grad_positions || r.grad_query_positions) {
-            s.push_q = (float*)part(rows * 12);
-            s.push_k = (float*)part((size_t)r.kv_heads * r.n_keys * 12);
-        }
-        if (r.grad_slopes) s.turn = (float*)part(rows * 4);
-    }
-    s.bytes = at;
-    return s;
-}
-
-void lay_tiles(const tnr_structure_attention& r, const StructurePlan& p, const StructureArgs& a,
-               bool keys, hipStream_t stream) {
-    const int64_t blocks = (r.n_structures + 3) / 4;
-    k_structure_tiles<<<(unsigned)(blocks < 64 ? blocks : 64), 256, 0, stream>>>(
-        r.query_ptr, r.key_ptr, r.n_structures, r.n_queries, r.n_keys, p.group, p.q_waves * kTile,
-        p.k_waves * kTile, a.q_tiles, keys ? a.k_tiles : nullptr);
-}
-
-template <typename F>
-void with_dim(int32_t dim, F&& f) {
-    if (dim <= 32)
-        f(Int<32>{});
-    else if (dim <= 64)
-        f(Int<64>{});
-    else if (dim <= 96)
-        f(Int<96>{});
-    else
-        f(Int<128>{});
-}
-template <typename F>
-void with_waves(int waves, bool cap, F&& f) {
-    const auto capped = [&](auto w) {
-        if (cap)
-            f(w, std::true_type{});
-        else
-            f(w, std::false_type{});
-    };
-    if (waves == 2)
-        capped(Int<2>{});
-    else
-        capped(Int<4>{});
 }
 
 // -------------------------------------------------------- neighbor attention
@@ -599,113 +353,6 @@ int tnr_embedding_backward(const tnr_embedding* req, void* workspace, size_t wor
             }
         });
     });
-    return launched(err, err_len);
-}
-
-size_t tnr_structure_tiles_size(const tnr_structure_attention* req) {
-    if (!req || req->n_structures < 0 || req->n_queries < 0 || req->n_keys < 0 || req->heads < 1 ||
-        req->kv_heads < 1 || req->heads % req->kv_heads != 0)
-        return 0;
-    const StructurePlan p = structure_plan(*req);
-    return q_tile_bytes(p) + k_tile_bytes(p);
-}
-
-size_t tnr_structure_forward_workspace_size(const tnr_structure_attention* req) {
-    if (tnr_structure_tiles_size(req) == 0) return 0;
-    return structure_space(*req, structure_plan(*req), false, nullptr).bytes;
-}
-
-int tnr_structure_forward(const tnr_structure_attention* req, void* workspace,
-                          size_t workspace_bytes, void* stream, char* err, size_t err_len) {
-    const int code = check_structure(req, false, err, err_len);
-    if (code != TNR_OK) return code;
-    const tnr_structure_attention& r = *req;
-    if (r.n_structures == 0) return TNR_OK;
-    const StructurePlan p = structure_plan(r);
-    const StructureSpace s = structure_space(r, p, false, workspace);
-    if (s.bytes > 0 && (!workspace || (uintptr_t)workspace % 256 != 0 || workspace_bytes < s.bytes))
-        return refuse(err, err_len, "workspace is too small or not aligned to 256 bytes");
-    const hipStream_t st = (hipStream_t)stream;
-    StructureArgs a = structure_args(r, p);
-    a.part = s.part;
-    lay_tiles(r, p, a, r.lse != nullptr, st);
-    if (r.n_queries == 0) return launched(err, err_len);
-    with_type(r.dtype, [&](auto t) {
-        using T = decltype(t);
-        with_dim(r.dim, [&](auto d) {
-            constexpr int DP = decltype(d)::value;
-            with_waves(p.q_waves, r.softcap > 0.f, [&](auto w, auto c) {
-                constexpr int NW = decltype(w)::value;
-                constexpr bool CAP = decltype(c)::value;
-                k_structure_forward<T, DP, NW, CAP>
-                    <<<dim3((unsigned)p.q_tiles, r.kv_heads * p.splits), NW * kWave, 0, st>>>(a);
-            });
-        });
-        if (p.splits > 1)
-            k_structure_join<T>
-                <<<(unsigned)((r.n_queries * r.heads + 3) / 4), 256, 0, st>>>(a);
-    });
-    return launched(err, err_len);
-}
-
-size_t tnr_structure_backward_workspace_size(const tnr_structure_attention* req) {
-    if (tnr_structure_tiles_size(req) == 0) return 0;
-    return structure_space(*req, structure_plan(*req), true, nullptr).bytes;
-}
-
-int tnr_structure_backward(const tnr_structure_attention* req, void* workspace,
-                           size_t workspace_bytes, void* stream, char* err, size_t err_len) {
-    const int code = check_structure(req, true, err, err_len);
-    if (code != TNR_OK) return code;
-    const tnr_structure_attention& r = *req;
-    const StructurePlan p = structure_plan(r);
-    const StructureSpace s = structure_space(r, p, true, workspace);
-    if (s.bytes > 0 && (!workspace || (uintptr_t)workspace % 256 != 0 || workspace_bytes < s.bytes))
-        return refuse(err, err_len, "workspace is too small or not aligned to 256 bytes");
-    const hipStream_t st = (hipStream_t)stream;
-    StructureArgs a = structure_args(r, p);
-    a.part = s.part;
-    a.part_k = s.part_k;
-    a.row = s.row;
-    a.push_q = s.push_q;
-    a.push_k = s.push_k;
-    a.turn = s.turn;
-    with_type(r.dtype, [&](auto t) {
-        using T = decltype(t);
-        with_dim(r.dim, [&](auto d) {
-            constexpr int DP = decltype(d)::value;
-            if (r.n_queries > 0)
-                with_waves(p.q_waves, r.softcap > 0.f, [&](auto w, auto c) {
-                    constexpr int NW = decltype(w)::value;
-                constexpr bool CAP = decltype(c)::value;
-                    k_structure_dq<T, DP, NW, CAP>
-                        <<<dim3((unsigned)p.q_tiles, r.kv_heads * p.splits), NW * kWave, 0, st>>>(
-                            a);
-                });
-            if (r.n_queries > 0 && p.splits > 1)
-                k_structure_join_dq<T>
-                    <<<(unsigned)((r.n_queries * r.heads + 3) / 4), 256, 0, st>>>(a);
-            if (r.n_keys > 0)
-                with_waves(p.k_waves, r.softcap > 0.f, [&](auto w, auto c) {
-                    constexpr int NW = decltype(w)::value;
-                constexpr bool CAP = decltype(c)::value;
-                    k_structure_dkv<T, DP, NW, CAP>
-                        <<<dim3((unsigned)p.k_tiles, r.kv_heads * p.k_splits), NW * kWave, 0,
-                           st>>>(a);
-                });
-            if (r.n_keys > 0 && p.k_splits > 1)
-                k_structure_join_dkv<T>
-                    <<<(unsigned)((r.kv_heads * r.n_keys * (2 * r.dim + 3) + 255) / 256), 256, 0,
-                       st>>>(a);
-        });
-    });
-    const int shared = !r.query_positions;
-    const int64_t items = (r.grad_positions ? 3 * r.n_keys : 0) +
-                          (r.grad_query_positions ? 3 * r.n_queries : 0);
-    const int64_t blocks = (items + 1023) / 1024 + (r.grad_slopes ? r.heads : 0);
-    if (blocks > 0)
-        k_structure_finish<<<(unsigned)blocks, 1024, 0, st>>>(a, r.grad_query_positions,
-                                                              r.grad_positions, r.grad_slopes, shared);
     return launched(err, err_len);
 }
 

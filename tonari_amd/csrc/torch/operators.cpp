@@ -175,6 +175,15 @@ Tensor pair_attention(const Tensor& q, const Tensor& k, const Tensor& v, const T
         .to(q.scalar_type());
 }
 
+// The inputs as nodes of their own: the gradient for one of them then takes no
+// path through another (q may well depend on the positions).
+variable_list own_nodes(const variable_list& saved, size_t n) {
+    variable_list nodes;
+    for (size_t i = 0; i < n; ++i)
+        nodes.push_back(saved[i].defined() ? saved[i].view_as(saved[i]) : Tensor());
+    return nodes;
+}
+
 // The gradients, with a graph, of `out` for the inputs that need one.
 variable_list graph_of(const Tensor& out, const Tensor& upstream, const variable_list& inputs,
                        const std::vector<bool>& needed) {
@@ -270,7 +279,8 @@ struct StructureAttention : torch::autograd::Function<StructureAttention> {
         std::vector<bool> needed;
         for (size_t i = 0; i < 6; ++i) needed.push_back(s[i].defined() && ctx->needs_input_grad(i));
         if (at::GradMode::is_enabled()) {
-            const Tensor &x = s[3], &x_q = s[5], &kp = s[6], &qp = s[7].defined() ? s[7] : s[6];
+            const variable_list n = own_nodes(s, 6);
+            const Tensor &x = n[3], &x_q = n[5], &kp = s[6], &qp = s[7].defined() ? s[7] : s[6];
             const Tensor nq = qp.slice(0, 1) - qp.slice(0, 0, -1);
             const Tensor nk = kp.slice(0, 1) - kp.slice(0, 0, -1);
             const Tensor pairs = nq * nk;
@@ -286,9 +296,8 @@ struct StructureAttention : torch::autograd::Function<StructureAttention> {
             const Tensor apart = r2.gt(0);
             const Tensor r = at::where(apart, at::where(apart, r2, one).sqrt(), one * 0);
             const Tensor out =
-                pair_attention(s[0], s[1], s[2], r, s[4], source, target, scale, softcap);
-            const variable_list found =
-                graph_of(out, grads[0], {s[0], s[1], s[2], s[3], s[4], s[5]}, needed);
+                pair_attention(n[0], n[1], n[2], r, n[4], source, target, scale, softcap);
+            const variable_list found = graph_of(out, grads[0], n, needed);
             for (size_t i = 0; i < 6; ++i) all[i] = found[i];
             return all;
         }
@@ -428,10 +437,10 @@ struct NeighborAttention : torch::autograd::Function<NeighborAttention> {
         if (at::GradMode::is_enabled()) {
             std::vector<bool> needed;
             for (size_t i = 0; i < 5; ++i) needed.push_back(ctx->needs_input_grad(i));
+            const variable_list n = own_nodes(s, 5);
             const Tensor out =
-                pair_attention(s[0], s[1], s[2], s[3], s[4], s[6], s[7], scale, softcap);
-            const variable_list found =
-                graph_of(out, grads[0], {s[0], s[1], s[2], s[3], s[4]}, needed);
+                pair_attention(n[0], n[1], n[2], n[3], n[4], s[6], s[7], scale, softcap);
+            const variable_list found = graph_of(out, grads[0], n, needed);
             for (size_t i = 0; i < 5; ++i) all[i] = found[i];
             return all;
         }
