@@ -169,6 +169,8 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP <= 32 ? 64 : 2 * DP)) v
         M::template rows<DP>(dp, v_rows + sub * Pair::kRows, dor, a.dim);
         typename M::Weights p, rest;
         const bool near = all_near<CAP>(dot, a.rule);
+        // the tile's own sums: a long row's are then sums of few terms each
+        float tw[kRowSums] = {};
 #pragma unroll
         for (int run = 0; run < 4; ++run) {
             const int first = sub * kTile;
@@ -197,7 +199,7 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP <= 32 ? 64 : 2 * DP)) v
             for (int e = 0; e < 4; ++e) {
                 const int i = 4 * run + e;
                 ds[e] = s[e] * (dp[i] - delta);
-                w[0] += ds[e];
+                tw[0] += ds[e];
                 float dx_i = CAP ? ds[e] * bend[e] : ds[e];
                 if (kNarrow<T>) dx_i *= unit;
                 p.set(i, dx_i);
@@ -209,18 +211,20 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP <= 32 ? 64 : 2 * DP)) v
                 for (int e = 0; e < 4; ++e) {
                     const float over = r[e] > 0.f ? __builtin_amdgcn_rcpf(r[e]) : 0.f;
                     const float wd = ds[e] * over, wp = s[e] * over;
-                    w[1] = fmaf(wd, dx[e], w[1]);
-                    w[2] = fmaf(wd, dy[e], w[2]);
-                    w[3] = fmaf(wd, dz[e], w[3]);
-                    w[4] = fmaf(wp, dx[e], w[4]);
-                    w[5] = fmaf(wp, dy[e], w[5]);
-                    w[6] = fmaf(wp, dz[e], w[6]);
-                    w[7] = fmaf(ds[e], r[e] - r_mid, w[7]);
-                    w[8] = fmaf(s[e], r[e] - r_mid, w[8]);
+                    tw[1] = fmaf(wd, dx[e], tw[1]);
+                    tw[2] = fmaf(wd, dy[e], tw[2]);
+                    tw[3] = fmaf(wd, dz[e], tw[3]);
+                    tw[4] = fmaf(wp, dx[e], tw[4]);
+                    tw[5] = fmaf(wp, dy[e], tw[5]);
+                    tw[6] = fmaf(wp, dz[e], tw[6]);
+                    tw[7] = fmaf(ds[e], r[e] - r_mid, tw[7]);
+                    tw[8] = fmaf(s[e], r[e] - r_mid, tw[8]);
                 }
             }
             __builtin_amdgcn_sched_barrier(kLoadsPass);
         }
+#pragma unroll
+        for (int i = 0; i < kRowSums; ++i) w[i] += tw[i];
         // Their sum over a row is 0, so grad_q is a difference: what the rounding of
         // dx leaves out goes through a second product.
         const T* cols = M::kSeparateCols ? k_cols + sub * Pair::kCols : k_rows + sub * Pair::kRows;
