@@ -149,27 +149,34 @@ struct NeighborArgs {
     float* turn;   // [heads][n_sources]
 };
 
-// 16 bytes of a row, as they are loaded: products of 16-bit values go two at a
-// time into a 32-bit sum.
-template <typename T>
+// A lane's part of a row, as it is loaded: R times 16 bytes.  Products of 16-bit
+// values go two at a time into a 32-bit sum.
+template <typename T, int R>
 struct Raw {
-    static constexpr int kVec = 16 / sizeof(T);
-    Vec<T, kVec> x;
+    static constexpr int kEach = 16 / sizeof(T), kVec = R * kEach;
+    Vec<T, kEach> x[R];
     __device__ __forceinline__ static Raw at(const char* p) {
-        return {*(const Vec<T, kVec>*)p};
+        Raw raw;
+#pragma unroll
+        for (int r = 0; r < R; ++r) raw.x[r] = ((const Vec<T, kEach>*)p)[r];
+        return raw;
     }
+    __device__ __forceinline__ float get(int i) const { return (float)x[i / kEach][i % kEach]; }
     __device__ __forceinline__ float dot(const Raw& o, float sum) const {
-        if constexpr (sizeof(T) == 4) {
 #pragma unroll
-            for (int i = 0; i < kVec; ++i) sum = fmaf(x[i], o.x[i], sum);
-        } else {
+        for (int r = 0; r < R; ++r) {
+            if constexpr (sizeof(T) == 4) {
 #pragma unroll
-            for (int i = 0; i < kVec; i += 2) {
-                const Vec<T, 2> a = {x[i], x[i + 1]}, b = {o.x[i], o.x[i + 1]};
-                if constexpr (std::is_same_v<T, bf16>)
-                    sum = __builtin_amdgcn_fdot2_f32_bf16(a, b, sum, false);
-                else
-                    sum = __builtin_amdgcn_fdot2(a, b, sum, false);
+                for (int i = 0; i < kEach; ++i) sum = fmaf(x[r][i], o.x[r][i], sum);
+            } else {
+#pragma unroll
+                for (int i = 0; i < kEach; i += 2) {
+                    const Vec<T, 2> a = {x[r][i], x[r][i + 1]}, b = {o.x[r][i], o.x[r][i + 1]};
+                    if constexpr (std::is_same_v<T, bf16>)
+                        sum = __builtin_amdgcn_fdot2_f32_bf16(a, b, sum, false);
+                    else
+                        sum = __builtin_amdgcn_fdot2(a, b, sum, false);
+                }
             }
         }
         return sum;
@@ -177,9 +184,21 @@ struct Raw {
     // acc += p x
     __device__ __forceinline__ void add(float p, float (&acc)[kVec]) const {
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) acc[i] = fmaf(p, (float)x[i], acc[i]);
+        for (int i = 0; i < kVec; ++i) acc[i] = fmaf(p, get(i), acc[i]);
     }
 };
+// 16 bytes at a time.
+template <typename T, int N>
+__device__ __forceinline__ void store_wide(T* p, const float (&x)[N]) {
+    constexpr int kEach = 16 / sizeof(T);
+#pragma unroll
+    for (int b = 0; b < N; b += kEach) {
+        Vec<T, kEach> v;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) v[i] = rounded<T>(x[b + i]);
+        *(Vec<T, kEach>*)(p + b) = v;
+    }
+}
 
 // Sum over the LPH lanes of a head, in all of them.
 template <int LPH>
@@ -259,13 +278,13 @@ __device__ __forceinline__ void load_wide(const float* p, float (&x)[N]) {
     }
 }
 
-// What a lane of a wave takes: 16 bytes of a key head's channels, for GH query
-// heads that share it (`head` is the first).  A slot holds `block` such units.
+// What a lane of a wave takes: R times 16 bytes of a key head's channels, for GH
+// query heads that share it (`head` is the first).  A slot holds `block` such units.
 // Lanes whose head or channels do not exist read those of others and add
 // nothing.
-template <typename T, int LPH, int GH>
+template <typename T, int LPH, int GH, int R>
 struct Lane {
-    static constexpr int VEC = Raw<T>::kVec;
+    static constexpr int VEC = Raw<T, R>::kVec;
     int lane, slot, in_slot, slots, head, kv, c;
     bool there, mine;  // the head exists; the channels too
     __device__ __forceinline__ Lane(const NeighborArgs& a, int first) {
@@ -318,12 +337,12 @@ struct PairChunk {
 };
 
 // grid: (sources / 4, blocks of units).
-template <typename T, int LPH, int GH, bool CAP>
+template <typename T, int LPH, int GH, int R, bool CAP>
 __global__ __launch_bounds__(256, kHeld) void k_neighbor_forward(const NeighborArgs a) {
-    constexpr int VEC = Raw<T>::kVec, kAhead = GH == 1 ? 4 : 2;
+    constexpr int VEC = Raw<T, R>::kVec, kAhead = GH == 1 && R == 1 ? 4 : 2;
     const int64_t i = xcd_order(blockIdx.x, gridDim.x) * 4 + threadIdx.x / kWave;
     if (i >= a.n_sources) return;
-    const Lane<T, LPH, GH> l(a, blockIdx.y * (a.slot / LPH));
+    const Lane<T, LPH, GH, R> l(a, blockIdx.y * (a.slot / LPH));
     const int64_t row = i * a.heads + l.head;
     float acc[GH][VEC], top[GH], sum[GH];
 #pragma unroll
@@ -335,13 +354,13 @@ __global__ __launch_bounds__(256, kHeld) void k_neighbor_forward(const NeighborA
     }
     const bool valid = *a.rows.status == 0;
     if (valid) {
-        Raw<T> q[GH];
+        Raw<T, R> q[GH];
         float slope2[GH];
 #pragma unroll
         for (int g = 0; g < GH; ++g) {
-            q[g] = Raw<T>{};
+            q[g] = Raw<T, R>{};
             if (l.mine)
-                q[g] = Raw<T>::at((const char*)((const T*)a.q + i * a.q_stride[0] +
+                q[g] = Raw<T, R>::at((const char*)((const T*)a.q + i * a.q_stride[0] +
                                                 (l.head + g) * a.q_stride[1] + l.c));
             slope2[g] = a.slopes[l.head + g] * kLog2e;
         }
@@ -355,7 +374,7 @@ __global__ __launch_bounds__(256, kHeld) void k_neighbor_forward(const NeighborA
         // weight 0.
         PairChunk chunk(a, run);
         const auto step = [&](int p0, auto whole) {
-            Raw<T> kx[kAhead], vx[kAhead];
+            Raw<T, R> kx[kAhead], vx[kAhead];
             float d[kAhead];
             bool in[kAhead];
 #pragma unroll
@@ -364,13 +383,13 @@ __global__ __launch_bounds__(256, kHeld) void k_neighbor_forward(const NeighborA
                 in[u] = whole || p < chunk.left;
                 const int j = __shfl(chunk.target, p);
                 d[u] = __shfl(chunk.distance, p);
-                kx[u] = Raw<T>::at(row_at<T>(k, j, k_row));
-                vx[u] = Raw<T>::at(row_at<T>(v, j, v_row));
+                kx[u] = Raw<T, R>::at(row_at<T>(k, j, k_row));
+                vx[u] = Raw<T, R>::at(row_at<T>(v, j, v_row));
             }
             if (!whole)
 #pragma unroll
                 for (int u = 0; u < kAhead; ++u)
-                    if (!in[u]) vx[u] = Raw<T>{};
+                    if (!in[u]) vx[u] = Raw<T, R>{};
             // weights relative to the slot's maximum when it was last set, which
             // is set anew where a score passes it by more than 2^8
             float s[GH][kAhead], high[GH], unused[kAhead];
@@ -438,8 +457,8 @@ __global__ __launch_bounds__(256, kHeld) void k_neighbor_forward(const NeighborA
         const int64_t at = (row + g) * a.dim + l.c;
 #pragma unroll
         for (int x = 0; x < VEC; ++x) acc[g][x] = valid ? acc[g][x] * by : nan_of();
-        store_floats<T, VEC>((T*)a.out + at, acc[g]);
-        if (a.out32) store_floats<float, VEC>(a.out32 + at, acc[g]);
+        store_wide<T, VEC>((T*)a.out + at, acc[g]);
+        if (a.out32) store_wide<float, VEC>(a.out32 + at, acc[g]);
         if (a.lse && l.c == 0)
             a.lse[row + g] = !valid        ? nan_of()
                              : sum[g] == 0.f ? -inf_of()
@@ -450,9 +469,9 @@ __global__ __launch_bounds__(256, kHeld) void k_neighbor_forward(const NeighborA
 // By sources: grad_q, grad_d, delta and the slopes' gradient by rows.  Blocks of
 // units that do not fit a wave follow one another in it, so that a pair's
 // grad_d is summed by one lane.
-template <typename T, int LPH, int GH, bool CAP>
+template <typename T, int LPH, int GH, int R, bool CAP>
 __global__ __launch_bounds__(256, kHeldBack) void k_neighbor_dq(const NeighborArgs a) {
-    constexpr int VEC = Raw<T>::kVec, kAhead = GH == 1 ? 4 : GH == 2 ? 2 : 1;
+    constexpr int VEC = Raw<T, R>::kVec, kAhead = GH == 4 ? 1 : GH == 2 || R == 2 ? 2 : 4;
     const int64_t i = xcd_order(blockIdx.x, gridDim.x) * 4 + threadIdx.x / kWave;
     if (i >= a.n_sources) return;
     if (*a.rows.status != 0) {
@@ -466,24 +485,24 @@ __global__ __launch_bounds__(256, kHeldBack) void k_neighbor_dq(const NeighborAr
     const uint32_t k_row = (uint32_t)(a.k_stride[0] * sizeof(T));
     const uint32_t v_row = (uint32_t)(a.v_stride[0] * sizeof(T));
     for (int first = 0; first * GH < a.heads; first += a.slot / LPH) {
-        const Lane<T, LPH, GH> l(a, first);
+        const Lane<T, LPH, GH, R> l(a, first);
         const int64_t row = i * a.heads + l.head;
-        Raw<T> q[GH], go[GH];
+        Raw<T, R> q[GH], go[GH];
         float acc[GH][VEC], delta[GH], turn[GH], lse[GH], slope[GH];
 #pragma unroll
         for (int g = 0; g < GH; ++g) {
-            q[g] = go[g] = Raw<T>{};
+            q[g] = go[g] = Raw<T, R>{};
             delta[g] = turn[g] = slope[g] = 0.f;
             lse[g] = inf_of();
             if (l.mine) {
                 const int64_t at = (row + g) * a.dim + l.c;
                 float o[VEC];
-                q[g] = Raw<T>::at((const char*)((const T*)a.q + i * a.q_stride[0] +
+                q[g] = Raw<T, R>::at((const char*)((const T*)a.q + i * a.q_stride[0] +
                                                 (l.head + g) * a.q_stride[1] + l.c));
-                go[g] = Raw<T>::at((const char*)((const T*)a.grad_out + at));
+                go[g] = Raw<T, R>::at((const char*)((const T*)a.grad_out + at));
                 load_wide<VEC>(a.out_full + at, o);
 #pragma unroll
-                for (int x = 0; x < VEC; ++x) delta[g] = fmaf((float)go[g].x[x], o[x], delta[g]);
+                for (int x = 0; x < VEC; ++x) delta[g] = fmaf(go[g].get(x), o[x], delta[g]);
             }
             if (l.there) {  // in every lane of the head: slot_sum takes any of them
                 lse[g] = a.lse[row + g];
@@ -502,22 +521,22 @@ __global__ __launch_bounds__(256, kHeldBack) void k_neighbor_dq(const NeighborAr
         // distances from any one of them: what they share cancels exactly.
         const float near = __shfl(chunk.distance, 0);
         const auto step = [&](int p0, auto whole) {
-            Raw<T> kx[kAhead], vx[kAhead];
+            Raw<T, R> kx[kAhead], vx[kAhead];
             float d[kAhead];
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
                 const int p = p0 + u * l.slots + l.slot;
                 const int j = __shfl(chunk.target, p);
                 d[u] = __shfl(chunk.distance, p);
-                kx[u] = Raw<T>::at(row_at<T>(k, j, k_row));
-                vx[u] = Raw<T>::at(row_at<T>(v, j, v_row));
+                kx[u] = Raw<T, R>::at(row_at<T>(k, j, k_row));
+                vx[u] = Raw<T, R>::at(row_at<T>(v, j, v_row));
             }
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
                 const int p = p0 + u * l.slots + l.slot;
                 const bool in = whole || p < chunk.left;
                 const int e = chunk.first + p;
-                if (!whole && !in) kx[u] = Raw<T>{};
+                if (!whole && !in) kx[u] = Raw<T, R>{};
                 float push = 0.f, s[GH], dp[GH], bend[GH];
 #pragma unroll
                 for (int g = 0; g < GH; ++g) {
@@ -552,7 +571,7 @@ __global__ __launch_bounds__(256, kHeldBack) void k_neighbor_dq(const NeighborAr
             for (int x = 0; x < VEC; ++x)
                 acc[g][x] = join_lanes<sum_of>(acc[g][x], a.slot) * a.rule.scale;
             if (l.mine && l.slot == 0) {
-                store_floats<T, VEC>((T*)a.grad_q + (row + g) * a.dim + l.c, acc[g]);
+                store_wide<T, VEC>((T*)a.grad_q + (row + g) * a.dim + l.c, acc[g]);
                 if (l.c == 0) a.turn[(int64_t)(l.head + g) * a.n_sources + i] = turn[g];
             }
         }
@@ -561,9 +580,9 @@ __global__ __launch_bounds__(256, kHeldBack) void k_neighbor_dq(const NeighborAr
 
 // By targets: grad_k and grad_v.  grid: (targets / 4, blocks of key heads).  A
 // unit here is a key head; its query heads are taken GH at a time.
-template <typename T, int LPH, int GH, bool CAP>
+template <typename T, int LPH, int GH, int R, bool CAP>
 __global__ __launch_bounds__(256, kHeldBack) void k_neighbor_dkv(const NeighborArgs a) {
-    constexpr int VEC = Raw<T>::kVec, kAhead = GH == 1 ? 4 : GH == 2 ? 2 : 1;
+    constexpr int VEC = Raw<T, R>::kVec, kAhead = GH == 4 ? 1 : GH == 2 || R == 2 ? 2 : 4;
     const int64_t j = xcd_order(blockIdx.x, gridDim.x) * 4 + threadIdx.x / kWave;
     if (j >= a.n_targets) return;
     const int lane = lane_of(), slot = lane / a.slot, in_slot = lane % a.slot;
@@ -578,10 +597,10 @@ __global__ __launch_bounds__(256, kHeldBack) void k_neighbor_dkv(const NeighborA
 #pragma unroll
     for (int x = 0; x < VEC; ++x) dk[x] = dv[x] = valid ? 0.f : nan_of();
     if (valid) {
-        Raw<T> k{}, v{};
+        Raw<T, R> k{}, v{};
         if (mine) {
-            k = Raw<T>::at((const char*)((const T*)a.k + j * a.k_stride[0] + kv * a.k_stride[1] + c));
-            v = Raw<T>::at((const char*)((const T*)a.v + j * a.v_stride[0] + kv * a.v_stride[1] + c));
+            k = Raw<T, R>::at((const char*)((const T*)a.k + j * a.k_stride[0] + kv * a.k_stride[1] + c));
+            v = Raw<T, R>::at((const char*)((const T*)a.v + j * a.v_stride[0] + kv * a.v_stride[1] + c));
         }
         const int2 run = run_of(a.rows.targets, j);
         const uint32_t q_row = (uint32_t)(a.q_stride[0] * sizeof(T));
@@ -611,7 +630,7 @@ __global__ __launch_bounds__(256, kHeldBack) void k_neighbor_dkv(const NeighborA
                 fetch(from + kWave);
                 const int n = min(run.y - from, kWave);
                 const auto step = [&](int p0, auto whole) {
-                    Raw<T> qx[kAhead][GH], ox[kAhead][GH];
+                    Raw<T, R> qx[kAhead][GH], ox[kAhead][GH];
                     float d[kAhead];
                     float2 st[kAhead][GH];
 #pragma unroll
@@ -624,8 +643,8 @@ __global__ __launch_bounds__(256, kHeldBack) void k_neighbor_dkv(const NeighborA
                         const float2* si = (const float2*)row_at<T>(stat, i, stat_row);
 #pragma unroll
                         for (int g = 0; g < GH; ++g) {
-                            qx[u][g] = Raw<T>::at(qi + g * q_head);
-                            ox[u][g] = Raw<T>::at(oi + g * o_head);
+                            qx[u][g] = Raw<T, R>::at(qi + g * q_head);
+                            ox[u][g] = Raw<T, R>::at(oi + g * o_head);
                             st[u][g] = si[g];
                         }
                     }
@@ -635,7 +654,7 @@ __global__ __launch_bounds__(256, kHeldBack) void k_neighbor_dkv(const NeighborA
                         float s[GH], dp[GH], bend[GH];
 #pragma unroll
                         for (int g = 0; g < GH; ++g) {
-                            if (!whole && !in) qx[u][g] = ox[u][g] = Raw<T>{};
+                            if (!whole && !in) qx[u][g] = ox[u][g] = Raw<T, R>{};
                             s[g] = head_sum<LPH>(qx[u][g].dot(k, 0.f));
                             dp[g] = head_sum<LPH>(ox[u][g].dot(v, 0.f));
                         }
@@ -666,8 +685,8 @@ __global__ __launch_bounds__(256, kHeldBack) void k_neighbor_dkv(const NeighborA
     if (!mine || slot != 0) return;
 #pragma unroll
     for (int x = 0; x < VEC; ++x) dk[x] *= a.rule.scale;
-    store_floats<T, VEC>((T*)a.grad_k + flat, dk);
-    store_floats<T, VEC>((T*)a.grad_v + flat, dv);
+    store_wide<T, VEC>((T*)a.grad_k + flat, dk);
+    store_wide<T, VEC>((T*)a.grad_v + flat, dv);
 }
 
 }  // namespace op

@@ -233,37 +233,46 @@ NeighborArgs neighbor_args(const tnr_neighbor_attention& r) {
     return a;
 }
 
-// Lanes of 16 bytes that make a head, a power of two (types of 16 bits fill 16 at
-// most), and the query heads that one lane takes.
+// How heads lie on lanes: R times 16 bytes to a lane, as many lanes as make a
+// head's channels (a power of two), GH query heads to a lane where they share a
+// key head.  What is done once for each score is done by every lane of a head,
+// so one query head takes two pieces where the channels allow: 256 crystals (1.3 M
+// pairs) of 8 capped heads of 16 floats take 51 + 74 + 67 us, forward and both
+// passes back, and 53 + 96 + 82 at one piece.
 template <typename T, typename F>
 void with_lanes(int32_t dim, int group, bool cap, F&& f) {
-    const int units = (int)(dim * sizeof(T) / 16);
-    const auto capped = [&](auto lanes, auto of) {
+    const auto capped = [&](auto lanes, auto of, auto pieces) {
         if (cap)
-            f(lanes, of, std::true_type{});
+            f(lanes, of, pieces, std::true_type{});
         else
-            f(lanes, of, std::false_type{});
+            f(lanes, of, pieces, std::false_type{});
     };
-    const auto heads = [&](auto lanes) {
-        if (group % 4 == 0)
-            capped(lanes, Int<4>{});
-        else if (group % 2 == 0)
-            capped(lanes, Int<2>{});
-        else
-            capped(lanes, Int<1>{});
+    const int units = (int)(dim * sizeof(T) / 16);
+    const auto lanes_of = [&](int n, auto of, auto pieces) {
+        constexpr int kMost = (int)(128 * sizeof(T) / 16) / decltype(pieces)::value;
+        if (n <= 1)
+            capped(Int<1>{}, of, pieces);
+        else if (n <= 2)
+            capped(Int<2>{}, of, pieces);
+        else if (n <= 4)
+            capped(Int<4>{}, of, pieces);
+        else if (n <= 8)
+            capped(Int<8>{}, of, pieces);
+        else if constexpr (kMost >= 16) {
+            if (n <= 16)
+                capped(Int<16>{}, of, pieces);
+            else if constexpr (kMost >= 32)
+                capped(Int<32>{}, of, pieces);
+        }
     };
-    if (units <= 1)
-        heads(Int<1>{});
-    else if (units <= 2)
-        heads(Int<2>{});
-    else if (units <= 4)
-        heads(Int<4>{});
-    else if (units <= 8)
-        heads(Int<8>{});
-    else if (units <= 16)
-        heads(Int<16>{});
-    else if constexpr (sizeof(T) == 4)
-        heads(Int<32>{});
+    if (group % 4 == 0)
+        lanes_of(units, Int<4>{}, Int<1>{});
+    else if (group % 2 == 0)
+        lanes_of(units, Int<2>{}, Int<1>{});
+    else if (units % 2 == 0)
+        lanes_of(units / 2, Int<1>{}, Int<2>{});
+    else
+        lanes_of(units, Int<1>{}, Int<1>{});
 }
 
 // Lanes of a slot: those of its units, a power of two, at most a wave.
@@ -417,13 +426,14 @@ int tnr_neighbor_forward(const tnr_neighbor_attention* req, void* stream, char* 
     NeighborArgs a = neighbor_args(r);
     with_type(r.dtype, [&](auto t) {
         using T = decltype(t);
-        with_lanes<T>(r.dim, a.group, r.softcap > 0.f, [&](auto l, auto g, auto c) {
-            constexpr int LPH = decltype(l)::value, GH = decltype(g)::value;
+        with_lanes<T>(r.dim, a.group, r.softcap > 0.f, [&](auto l, auto g, auto p, auto c) {
+            constexpr int LPH = decltype(l)::value, GH = decltype(g)::value,
+                          R = decltype(p)::value;
             constexpr bool CAP = decltype(c)::value;
             const int units = r.heads / GH;
             a.slot = slot_of(LPH, units);
             const int block = a.slot / LPH;
-            k_neighbor_forward<T, LPH, GH, CAP>
+            k_neighbor_forward<T, LPH, GH, R, CAP>
                 <<<dim3((unsigned)((r.list.n_sources + 3) / 4), (units + block - 1) / block), 256, 0,
                    (hipStream_t)stream>>>(a);
         });
@@ -452,17 +462,18 @@ int tnr_neighbor_backward(const tnr_neighbor_attention* req, void* workspace,
                       padded((size_t)r.list.n_sources * r.heads * sizeof(float2)));
     with_type(r.dtype, [&](auto t) {
         using T = decltype(t);
-        with_lanes<T>(r.dim, a.group, r.softcap > 0.f, [&](auto l, auto g, auto c) {
-            constexpr int LPH = decltype(l)::value, GH = decltype(g)::value;
+        with_lanes<T>(r.dim, a.group, r.softcap > 0.f, [&](auto l, auto g, auto p, auto c) {
+            constexpr int LPH = decltype(l)::value, GH = decltype(g)::value,
+                          R = decltype(p)::value;
             constexpr bool CAP = decltype(c)::value;
             a.slot = slot_of(LPH, r.heads / GH);
             if (r.list.n_sources > 0)
-                k_neighbor_dq<T, LPH, GH, CAP>
+                k_neighbor_dq<T, LPH, GH, R, CAP>
                     <<<(unsigned)((r.list.n_sources + 3) / 4), 256, 0, st>>>(a);
             a.slot = slot_of(LPH, r.kv_heads);
             const int block = a.slot / LPH;
             if (r.list.n_targets > 0)
-                k_neighbor_dkv<T, LPH, GH, CAP><<<dim3((unsigned)((r.list.n_targets + 3) / 4),
+                k_neighbor_dkv<T, LPH, GH, R, CAP><<<dim3((unsigned)((r.list.n_targets + 3) / 4),
                                                   (r.kv_heads + block - 1) / block),
                                              256, 0, st>>>(a);
         });
