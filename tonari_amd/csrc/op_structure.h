@@ -485,7 +485,7 @@ constexpr int waves_held(int dp) {
     return sizeof(T) == 4 ? (dp <= 32 ? 3 : dp <= 64 ? 2 : 1) : (dp <= 32 ? 4 : dp <= 64 ? 3 : 2);
 }
 
-// grid: (tiles, kv_heads * splits); NW waves of 32 query rows each.
+// grid: (tiles * kv_heads, splits); NW waves of 32 query rows each.
 template <typename T, int DP, int NW, bool CAP>
 __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP)) void k_structure_forward(
     const StructureArgs a) {
@@ -498,10 +498,11 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP)) void k_structure_forw
     __shared__ alignas(16) T v_tile[kTiles * kValues];
     __shared__ TilePositions<kTiles> x_k;
 
-    const int64_t block = xcd_order(blockIdx.x, gridDim.x);
+    // a tile's key heads lie next to each other in memory: they follow one another
+    const int64_t order = xcd_order(blockIdx.x, gridDim.x), block = order / a.kv_heads;
     const StructureTile t = a.q_tiles[block];
     const int lane = lane_of(), half = lane / 32, wave = threadIdx.x / kWave;
-    const int kv = blockIdx.y % a.kv_heads, split = blockIdx.y / a.kv_heads;
+    const int kv = (int)(order - block * a.kv_heads), split = blockIdx.y;
     const int g = a.group;
     if (t.n_q < 0) {  // NaN for the rows that lie here in the batch
         const int64_t all = (int64_t)a.n_queries * g;

@@ -50,7 +50,7 @@ __device__ __forceinline__ void finish_row(const StructureArgs& a, int head, int
     if (a.turn) a.turn[at] = -(w[7] - w[0] * w[8]);
 }
 
-// grid: (query tiles, kv_heads * splits).
+// grid: (query tiles * kv_heads, splits).
 template <typename T, int DP, int NW, bool CAP>
 __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP <= 32 ? 64 : 2 * DP)) void k_structure_dq(
     const StructureArgs a) {
@@ -63,10 +63,10 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP <= 32 ? 64 : 2 * DP)) v
     __shared__ alignas(16) T v_rows[kTiles * Pair::kRows];
     __shared__ TilePositions<kTiles> x_k;
 
-    const int64_t block = xcd_order(blockIdx.x, gridDim.x);
+    const int64_t order = xcd_order(blockIdx.x, gridDim.x), block = order / a.kv_heads;
     const StructureTile t = a.q_tiles[block];
     const int lane = lane_of(), half = lane / 32, wave = threadIdx.x / kWave;
-    const int kv = blockIdx.y % a.kv_heads, split = blockIdx.y / a.kv_heads;
+    const int kv = (int)(order - block * a.kv_heads), split = blockIdx.y;
     const int g = a.group;
     if (t.n_q < 0) {
         const int64_t row = block * (NW * kTile) + wave * kTile + lane % 32;
@@ -296,7 +296,7 @@ __global__ __launch_bounds__(256) void k_structure_join_dq(const StructureArgs a
     if (lane == 0) finish_row(a, head, query, delta, top, a.slopes[head], w);
 }
 
-// grid: (key tiles, kv_heads * k_splits); NW waves of 32 keys each.
+// grid: (key tiles * kv_heads, k_splits); NW waves of 32 keys each.
 template <typename T, int DP, int NW, bool CAP>
 __global__ __launch_bounds__(NW* kWave, DP > 64 ? 1 : DP > 32 || CAP || sizeof(T) == 4 ? 2 : 3) void
 k_structure_dkv(const StructureArgs a) {
@@ -313,10 +313,10 @@ k_structure_dkv(const StructureArgs a) {
     __shared__ TilePositions<kTiles> x_q;
     __shared__ alignas(16) float stat[3][kQueries];  // log-sum, delta, largest |grad_out|
 
-    const int64_t block = xcd_order(blockIdx.x, gridDim.x);
+    const int64_t order = xcd_order(blockIdx.x, gridDim.x), block = order / a.kv_heads;
     const StructureTile t = a.k_tiles[block];
     const int lane = lane_of(), half = lane / 32, wave = threadIdx.x / kWave;
-    const int kv = blockIdx.y % a.kv_heads, split = blockIdx.y / a.kv_heads;
+    const int kv = (int)(order - block * a.kv_heads), split = blockIdx.y;
     if (t.n_q < 0) {
         const int64_t key = block * (NW * kTile) + wave * kTile + lane % 32;
         if (key >= a.n_keys || half) return;

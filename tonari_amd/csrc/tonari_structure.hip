@@ -62,8 +62,8 @@ int check_structure(const tnr_structure_attention* r, bool backward, char* err, 
         r->n_structures >= INT32_MAX)
         return refuse(err, len, "too many atoms");
     const StructurePlan p = structure_plan(*r);
-    if (p.q_tiles * p.q_waves * kWave > kMostThreads || p.k_tiles * p.k_waves * kWave > kMostThreads ||
-        (int64_t)r->kv_heads * p.splits > 65535)
+    if (p.q_tiles * r->kv_heads * p.q_waves * kWave > kMostThreads ||
+        p.k_tiles * r->kv_heads * p.k_waves * kWave > kMostThreads)
         return refuse(err, len, "too many atoms");
     if (r->n_structures > 0 && (!r->query_ptr || !r->key_ptr))
         return refuse(err, len, "required pointers are null");
@@ -233,7 +233,7 @@ int tnr_structure_forward(const tnr_structure_attention* req, void* workspace,
                 constexpr int NW = decltype(w)::value;
                 constexpr bool CAP = decltype(c)::value;
                 k_structure_forward<T, DP, NW, CAP>
-                    <<<dim3((unsigned)p.q_tiles, r.kv_heads * p.splits), NW * kWave, 0, st>>>(a);
+                    <<<dim3((unsigned)(p.q_tiles * r.kv_heads), p.splits), NW * kWave, 0, st>>>(a);
             });
         });
         if (p.splits > 1)
@@ -274,7 +274,7 @@ int tnr_structure_backward(const tnr_structure_attention* req, void* workspace,
                     constexpr int NW = decltype(w)::value;
                 constexpr bool CAP = decltype(c)::value;
                     k_structure_dq<T, DP, NW, CAP>
-                        <<<dim3((unsigned)p.q_tiles, r.kv_heads * p.splits), NW * kWave, 0, st>>>(
+                        <<<dim3((unsigned)(p.q_tiles * r.kv_heads), p.splits), NW * kWave, 0, st>>>(
                             a);
                 });
             if (r.n_queries > 0 && p.splits > 1)
@@ -285,7 +285,7 @@ int tnr_structure_backward(const tnr_structure_attention* req, void* workspace,
                     constexpr int NW = decltype(w)::value;
                 constexpr bool CAP = decltype(c)::value;
                     k_structure_dkv<T, DP, NW, CAP>
-                        <<<dim3((unsigned)p.k_tiles, r.kv_heads * p.k_splits), NW * kWave, 0,
+                        <<<dim3((unsigned)(p.k_tiles * r.kv_heads), p.k_splits), NW * kWave, 0,
                            st>>>(a);
                 });
             if (r.n_keys > 0 && p.k_splits > 1)
