@@ -44,9 +44,9 @@ int tnr_operators_version(void);
 typedef struct tnr_embedding {
     int32_t dtype;          /* of weight, out and their gradients */
     int32_t index_bytes;    /* 4 or 8: species are int32 or int64 */
-    int64_t n_atoms;
-    int64_t n_species;      /* rows of the table */
-    int64_t channels;
+    int64_t n_atoms;        /* below 2^31 - 1 */
+    int64_t n_species;      /* rows of the table, below 2^24 */
+    int64_t channels;       /* up to 2^18 */
     const void* species;    /* [n_atoms]; outside [0, n_species): a row of NaN, no gradient */
     const void* weight;     /* T[n_species][channels] */
     float scale;
@@ -76,7 +76,7 @@ int tnr_embedding_backward(const tnr_embedding* req, void* workspace, size_t wor
 typedef struct tnr_structure_attention {
     int32_t dtype;                  /* of q, k, v, out and their gradients */
     int32_t heads, kv_heads, dim;   /* dim: a multiple of 8, 8 to 128 */
-    int64_t n_structures, n_queries, n_keys;
+    int64_t n_structures, n_queries, n_keys;  /* below 2^30; rows of all heads below 2^31 */
     const int64_t* query_ptr;       /* [n_structures + 1] */
     const int64_t* key_ptr;         /* [n_structures + 1] (may be query_ptr) */
     const void* q;                  /* T[n_queries][heads][dim] */
@@ -116,7 +116,8 @@ int tnr_structure_backward(const tnr_structure_attention* req, void* workspace,
 /* A neighbor list laid out for neighbor attention.  `rows` holds
  * tnr_neighbor_rows_size() bytes written by tnr_neighbor_rows. */
 typedef struct tnr_neighbor_list {
-    int64_t n_pairs, n_sources, n_targets;  /* each below 2^31 */
+    int64_t n_pairs;                        /* up to 2^31 - 4097 */
+    int64_t n_sources, n_targets;           /* below 2^26 */
     const int64_t* sources;                 /* i: int64[n_pairs], not falling */
     const int64_t* targets;                 /* j: int64[n_pairs] */
     int32_t transpose;                      /* 1: also by target, which the backward needs */

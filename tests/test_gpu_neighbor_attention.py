@@ -139,6 +139,12 @@ def test_forces_and_stress():
         assert err <= 1e-4 * max(1.0, float(e.abs().max()))
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_negative_scale_under_the_cap(dtype):
+    i, j = random_list(40, 40, 20, seed=13)
+    check(make(i, j, 40, 40, 4, 1, 32, dtype, seed=2), 0.5, scale=-0.5)
+
+
 def test_pairs_that_weigh_nothing():
     i, j = random_list(40, 40, 15, seed=2)
     c = make(i, j, 40, 40, 2, 2, 16, torch.float32, grad=False)

@@ -128,6 +128,12 @@ def test_large_scores_and_negative_scale():
     check(c, 50.0)
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_negative_scale_under_the_cap(dtype):
+    # products far beyond the cap on either side
+    check(make([70, 33], 2, 1, 32, dtype, seed=24, spread=4.0), 2.0, scale=-0.5)
+
+
 def test_far_atoms():
     # far atoms weigh nothing; a lone far atom still attends to itself
     c = make([60], 2, 2, 32, torch.float32, grad=False)

@@ -239,3 +239,16 @@ def test_neighbor_requests(lib):  # noqa: F811
         assert code == ext.TNR_INPUT_ERROR and message in said
     code, said = refused(lib.tnr_neighbor_backward, neighbor(), PTR, 64)
     assert code == ext.TNR_INPUT_ERROR and "workspace" in said
+
+
+def test_sizes_beyond_a_launch(lib):  # noqa: F811
+    for req in (embedding(n_species=1 << 24), embedding(channels=1 << 19),
+                embedding(n_atoms=(1 << 31) - 1)):
+        code, said = refused(lib.tnr_embedding_backward, req, PTR, 1 << 40)
+        assert code == ext.TNR_INPUT_ERROR and "too many" in said
+    code, said = refused(lib.tnr_neighbor_rows, listing(n_pairs=(1 << 31) - 100), PTR, 1 << 40)
+    assert code == ext.TNR_INPUT_ERROR and "too many" in said
+    code, said = refused(lib.tnr_structure_forward,
+                         structure(heads=1, kv_heads=1, n_queries=1 << 30, n_keys=1 << 30), PTR,
+                         1 << 40)
+    assert code == ext.TNR_INPUT_ERROR and "too many atoms" in said

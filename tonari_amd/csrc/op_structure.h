@@ -440,7 +440,7 @@ __device__ __forceinline__ bool all_near(const f32x16& dot, const ScoreRule& rul
     float top = 0.f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(dot[i]));
-    return __builtin_amdgcn_ballot_w64(!(top * rule.inv <= kTanhNear)) == 0;
+    return __builtin_amdgcn_ballot_w64(!(top * fabsf(rule.inv) <= kTanhNear)) == 0;
 }
 // u log2(e) + shift of the products of run `run`, and what their gradients are
 // multiplied by.

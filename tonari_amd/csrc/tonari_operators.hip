@@ -23,9 +23,11 @@ int check_embedding(const tnr_embedding* r, bool backward, char* err, size_t len
     if (!is_type(r->dtype)) return refuse(err, len, "dtype must be float32, bfloat16 or float16");
     if (r->index_bytes != 4 && r->index_bytes != 8)
         return refuse(err, len, "species must be int32 or int64");
-    if (r->n_atoms < 0 || r->n_species < 0 || r->channels < 1 || r->n_atoms >= INT32_MAX ||
-        r->n_species >= INT32_MAX || r->channels > (1 << 20))
+    if (r->n_atoms < 0 || r->n_species < 0 || r->channels < 1)
         return refuse(err, len, "invalid sizes");
+    // a workgroup for each species, and at most 65,535 side by side for its channels
+    if (r->n_atoms >= INT32_MAX || r->n_species * 256 > kMostThreads || r->channels > (1 << 18))
+        return refuse(err, len, "too many atoms, species or channels");
     const bool rows = r->n_atoms > 0, table = r->n_species > 0;
     if ((rows && (!r->species || !(backward ? r->grad_out : r->out))) ||
         (table && !(backward ? r->grad_weight : r->weight)))
@@ -135,7 +137,8 @@ int check_list(const tnr_neighbor_list* l, char* err, size_t len) {
     if (!l) return refuse(err, len, "list is null");
     if (l->n_pairs < 0 || l->n_sources < 0 || l->n_targets < 0)
         return refuse(err, len, "invalid sizes");
-    if (l->n_pairs >= INT32_MAX || l->n_sources >= kMostAtoms || l->n_targets >= kMostAtoms)
+    // (kernels look 64 pairs ahead with 32-bit numbers)
+    if (l->n_pairs > INT32_MAX - 4096 || l->n_sources >= kMostAtoms || l->n_targets >= kMostAtoms)
         return refuse(err, len, "too many pairs or atoms");
     if (l->n_pairs > 0 && (l->n_sources == 0 || l->n_targets == 0))
         return refuse(err, len, "a list with pairs needs sources and targets");

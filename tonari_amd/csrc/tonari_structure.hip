@@ -23,7 +23,8 @@ struct StructurePlan {
     int64_t q_tiles, k_tiles;
 };
 
-constexpr int64_t kSplitWaves = 3072;
+constexpr int64_t kMostAtoms = int64_t(1) << 30;
+constexpr int64_t kSplitWaves = 3072;  // three to each SIMD
 
 StructurePlan structure_plan(const tnr_structure_attention& r) {
     StructurePlan p{};
@@ -59,7 +60,7 @@ int check_structure(const tnr_structure_attention* r, bool backward, char* err, 
     if (!r->query_positions && r->n_queries != r->n_keys)
         return refuse(err, len, "queries of their own need positions of their own");
     if (r->n_queries >= INT32_MAX / r->heads || r->n_keys >= INT32_MAX / r->kv_heads ||
-        r->n_structures >= INT32_MAX)
+        r->n_queries >= kMostAtoms || r->n_keys >= kMostAtoms || r->n_structures >= kMostAtoms)
         return refuse(err, len, "too many atoms");
     const StructurePlan p = structure_plan(*r);
     if (p.q_tiles * r->kv_heads * p.q_waves * kWave > kMostThreads ||
