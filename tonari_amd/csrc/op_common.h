@@ -52,8 +52,8 @@ __device__ __forceinline__ float max_halves(float x) {
 // Workgroups go to the 8 XCDs in turn; in this order each XCD takes a run of
 // the work, so that what neighbours share, or write next to each other, meets
 // in one L2.
-__device__ __forceinline__ int64_t xcd_order(int64_t block, int64_t blocks) {
-    const int64_t each = blocks / 8, left = blocks % 8, xcd = block % 8, at = block / 8;
+__device__ __forceinline__ uint32_t xcd_order(uint32_t block, uint32_t blocks) {
+    const uint32_t each = blocks / 8, left = blocks % 8, xcd = block % 8, at = block / 8;
     return xcd * each + (xcd < left ? xcd : left) + at;
 }
 

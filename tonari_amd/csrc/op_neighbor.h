@@ -340,7 +340,7 @@ struct PairChunk {
 template <typename T, int LPH, int GH, int R, bool CAP>
 __global__ __launch_bounds__(256, kHeld) void k_neighbor_forward(const NeighborArgs a) {
     constexpr int VEC = Raw<T, R>::kVec, kAhead = GH == 1 && R == 1 ? 4 : 2;
-    const int64_t i = xcd_order(blockIdx.x, gridDim.x) * 4 + threadIdx.x / kWave;
+    const int64_t i = (int64_t)xcd_order(blockIdx.x, gridDim.x) * 4 + threadIdx.x / kWave;
     if (i >= a.n_sources) return;
     const Lane<T, LPH, GH, R> l(a, blockIdx.y * (a.slot / LPH));
     const int64_t row = i * a.heads + l.head;
@@ -472,7 +472,7 @@ __global__ __launch_bounds__(256, kHeld) void k_neighbor_forward(const NeighborA
 template <typename T, int LPH, int GH, int R, bool CAP>
 __global__ __launch_bounds__(256, kHeldBack) void k_neighbor_dq(const NeighborArgs a) {
     constexpr int VEC = Raw<T, R>::kVec, kAhead = GH == 4 ? 1 : GH == 2 || R == 2 ? 2 : 4;
-    const int64_t i = xcd_order(blockIdx.x, gridDim.x) * 4 + threadIdx.x / kWave;
+    const int64_t i = (int64_t)xcd_order(blockIdx.x, gridDim.x) * 4 + threadIdx.x / kWave;
     if (i >= a.n_sources) return;
     if (*a.rows.status != 0) {
         const int lane = lane_of();
@@ -583,7 +583,7 @@ __global__ __launch_bounds__(256, kHeldBack) void k_neighbor_dq(const NeighborAr
 template <typename T, int LPH, int GH, int R, bool CAP>
 __global__ __launch_bounds__(256, kHeldBack) void k_neighbor_dkv(const NeighborArgs a) {
     constexpr int VEC = Raw<T, R>::kVec, kAhead = GH == 4 ? 1 : GH == 2 || R == 2 ? 2 : 4;
-    const int64_t j = xcd_order(blockIdx.x, gridDim.x) * 4 + threadIdx.x / kWave;
+    const int64_t j = (int64_t)xcd_order(blockIdx.x, gridDim.x) * 4 + threadIdx.x / kWave;
     if (j >= a.n_targets) return;
     const int lane = lane_of(), slot = lane / a.slot, in_slot = lane % a.slot;
     const int slots = kWave / a.slot;

@@ -53,6 +53,13 @@ struct SortKeys {
     __device__ __forceinline__ int operator()(int64_t i) const { return key[i]; }
 };
 
+// Clears `words` that a later kernel wants zero.
+__device__ __forceinline__ void sort_clear(int32_t* clear, int64_t words) {
+    for (int64_t w = (int64_t)blockIdx.x * kSortThreads + threadIdx.x; w < words;
+         w += (int64_t)gridDim.x * kSortThreads)
+        clear[w] = 0;
+}
+
 // counts[digit * stride + tile]; and `clear`, which a later kernel wants zero.
 template <typename Keys>
 __global__ __launch_bounds__(kSortThreads) void k_sort_count(Keys keys, int64_t n, SortPass pass,
@@ -60,9 +67,7 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_count(Keys keys, int64_t 
                                                              int64_t clear_words) {
     __shared__ int32_t hist[kSortRadix];
     const int radix = 1 << pass.bits;
-    for (int64_t w = (int64_t)blockIdx.x * kSortThreads + threadIdx.x; w < clear_words;
-         w += (int64_t)gridDim.x * kSortThreads)
-        clear[w] = 0;
+    sort_clear(clear, clear_words);
     for (int d = threadIdx.x; d < radix; d += kSortThreads) hist[d] = 0;
     __syncthreads();
     const int64_t tile = xcd_order(blockIdx.x, gridDim.x), base = tile * kSortTile;
@@ -111,14 +116,18 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_scan(int32_t* counts, int
     if (lane_of() == 0) totals[digit] = before;
 }
 
-// Moves the items of a tile.  `put(place, index, key)` writes an item.
+// Moves the items of a tile.  `put(place, index, key)` writes an item.  Where there
+// is one tile it counts for itself (counts null), and clears what the counting
+// kernel else does.
 template <typename Keys, typename Put>
 __global__ __launch_bounds__(kSortThreads) void k_sort_move(Keys keys, int64_t n, SortPass pass,
                                                             const int32_t* counts,
-                                                            const int32_t* totals, Put put) {
+                                                            const int32_t* totals, Put put,
+                                                            int32_t* clear, int64_t clear_words) {
     __shared__ int32_t seen[kSortWaves][kSortRadix];
     __shared__ int32_t wave_sum[kSortWaves];
     const int radix = 1 << pass.bits, lane = lane_of(), wave = threadIdx.x / kWave;
+    if (!counts) sort_clear(clear, clear_words);
     for (int d = threadIdx.x; d < radix; d += kSortThreads)
 #pragma unroll
         for (int w = 0; w < kSortWaves; ++w) seen[w][d] = 0;
@@ -156,7 +165,14 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_move(Keys keys, int64_t n
     int carry = 0;
     for (int d0 = 0; d0 < radix; d0 += kSortThreads) {
         const int d = d0 + threadIdx.x;
-        const int x = d < radix ? totals[d] : 0;
+        int x = 0;
+        if (d < radix) {
+            if (counts)
+                x = totals[d];
+            else
+#pragma unroll
+                for (int w = 0; w < kSortWaves; ++w) x += seen[w][d];
+        }
         const int up = sort_wave_scan(x);
         if (lane == kWave - 1) wave_sum[wave] = up;
         __syncthreads();
@@ -167,7 +183,8 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_move(Keys keys, int64_t n
             all += wave_sum[w];
         }
         if (d < radix) {
-            int at = before + up - x + counts[(int64_t)d * sort_stride(gridDim.x) + tile];
+            int at = before + up - x;
+            if (counts) at += counts[(int64_t)d * sort_stride(gridDim.x) + tile];
 #pragma unroll
             for (int w = 0; w < kSortWaves; ++w) {
                 const int c = seen[w][d];

@@ -499,14 +499,14 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP)) void k_structure_forw
     __shared__ TilePositions<kTiles> x_k;
 
     // a tile's key heads lie next to each other in memory: they follow one another
-    const int64_t order = xcd_order(blockIdx.x, gridDim.x), block = order / a.kv_heads;
+    const uint32_t order = xcd_order(blockIdx.x, gridDim.x), block = order / (uint32_t)a.kv_heads;
     const StructureTile t = a.q_tiles[block];
     const int lane = lane_of(), half = lane / 32, wave = threadIdx.x / kWave;
     const int kv = (int)(order - block * a.kv_heads), split = blockIdx.y;
     const int g = a.group;
     if (t.n_q < 0) {  // NaN for the rows that lie here in the batch
         const int64_t all = (int64_t)a.n_queries * g;
-        const int64_t row = block * (NW * kTile) + wave * kTile + lane % 32;
+        const int64_t row = (int64_t)block * (NW * kTile) + wave * kTile + lane % 32;
         if (row >= all || split > 0 || half) return;
         const int query = (int)(row / g), head = kv * g + (int)(row % g);
         T* out = (T*)a.out + ((int64_t)query * a.heads + head) * a.dim;
@@ -528,7 +528,9 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP)) void k_structure_forw
     const int row = t.first + wave * kTile + lane % 32;
     const bool valid = row < rows;
     const bool busy = t.first + wave * kTile < rows;  // a wave without rows only helps to stage
-    const int query = t.q_lo + (valid ? row / g : 0), head = kv * g + (valid ? row % g : 0);
+    // (a division costs as much as a short row's tile does)
+    const int nth = !valid ? 0 : g == 1 ? row : (int)((uint32_t)row / (uint32_t)g);
+    const int query = t.q_lo + nth, head = kv * g + (valid ? row - nth * g : 0);
     Row qr;
     qr.load(valid ? (const T*)a.q + (int64_t)query * a.q_stride[0] + head * a.q_stride[1] : nullptr,
             a.dim);

@@ -63,13 +63,13 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP <= 32 ? 64 : 2 * DP)) v
     __shared__ alignas(16) T v_rows[kTiles * Pair::kRows];
     __shared__ TilePositions<kTiles> x_k;
 
-    const int64_t order = xcd_order(blockIdx.x, gridDim.x), block = order / a.kv_heads;
+    const uint32_t order = xcd_order(blockIdx.x, gridDim.x), block = order / (uint32_t)a.kv_heads;
     const StructureTile t = a.q_tiles[block];
     const int lane = lane_of(), half = lane / 32, wave = threadIdx.x / kWave;
     const int kv = (int)(order - block * a.kv_heads), split = blockIdx.y;
     const int g = a.group;
     if (t.n_q < 0) {
-        const int64_t row = block * (NW * kTile) + wave * kTile + lane % 32;
+        const int64_t row = (int64_t)block * (NW * kTile) + wave * kTile + lane % 32;
         if (row >= (int64_t)a.n_queries * g || half) return;
         const int query = (int)(row / g), head = kv * g + (int)(row % g);
         const int64_t at = (int64_t)head * a.n_queries + query;
@@ -90,7 +90,9 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP <= 32 ? 64 : 2 * DP)) v
     const int row = t.first + wave * kTile + lane % 32;
     const bool valid = row < rows;
     const bool busy = t.first + wave * kTile < rows;  // a wave without rows only helps to stage
-    const int query = t.q_lo + (valid ? row / g : 0), head = kv * g + (valid ? row % g : 0);
+    // (a division costs as much as a short row's tile does)
+    const int nth = !valid ? 0 : g == 1 ? row : (int)((uint32_t)row / (uint32_t)g);
+    const int query = t.q_lo + nth, head = kv * g + (valid ? row - nth * g : 0);
     const int64_t at = (int64_t)head * a.n_queries + query;
     const int64_t flat = ((int64_t)query * a.heads + head) * a.dim;
     Row qr, dor;
@@ -313,12 +315,12 @@ k_structure_dkv(const StructureArgs a) {
     __shared__ TilePositions<kTiles> x_q;
     __shared__ alignas(16) float stat[3][kQueries];  // log-sum, delta, largest |grad_out|
 
-    const int64_t order = xcd_order(blockIdx.x, gridDim.x), block = order / a.kv_heads;
+    const uint32_t order = xcd_order(blockIdx.x, gridDim.x), block = order / (uint32_t)a.kv_heads;
     const StructureTile t = a.k_tiles[block];
     const int lane = lane_of(), half = lane / 32, wave = threadIdx.x / kWave;
     const int kv = (int)(order - block * a.kv_heads), split = blockIdx.y;
     if (t.n_q < 0) {
-        const int64_t key = block * (NW * kTile) + wave * kTile + lane % 32;
+        const int64_t key = (int64_t)block * (NW * kTile) + wave * kTile + lane % 32;
         if (key >= a.n_keys || half) return;
         if (a.k_splits > 1) {
             float* part = a.part_k + (((int64_t)split * a.kv_heads + kv) * a.n_keys + key) *

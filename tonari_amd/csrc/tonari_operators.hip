@@ -103,10 +103,16 @@ void sort_pass(Keys keys, int64_t n, SortPass pass, int32_t* counts, int32_t* to
                hipStream_t stream, int32_t* clear = nullptr, int64_t clear_words = 0) {
     const unsigned tiles = (unsigned)sort_tiles(n);
     const int radix = 1 << pass.bits;
+    if (tiles == 1) {
+        k_sort_move<<<1, kSortThreads, 0, stream>>>(keys, n, pass, (const int32_t*)nullptr,
+                                                    (const int32_t*)nullptr, put, clear,
+                                                    clear_words);
+        return;
+    }
     k_sort_count<<<tiles, kSortThreads, 0, stream>>>(keys, n, pass, counts, clear, clear_words);
     k_sort_scan<<<(radix + kSortWaves - 1) / kSortWaves, kSortThreads, 0, stream>>>(
         counts, tiles, radix, totals);
-    k_sort_move<<<tiles, kSortThreads, 0, stream>>>(keys, n, pass, counts, totals, put);
+    k_sort_move<<<tiles, kSortThreads, 0, stream>>>(keys, n, pass, counts, totals, put, nullptr, 0);
 }
 
 template <typename I>
