@@ -19,12 +19,13 @@ int waves_for(int64_t rows, int64_t structures) {
 }
 
 struct StructurePlan {
-    int group, q_waves, k_waves, splits, k_splits;
+    int group, q_waves, k_waves;
+    int f_splits, splits, k_splits;  // of the forward, the queries' pass back, the keys'
     int64_t q_tiles, k_tiles;
 };
 
 constexpr int64_t kMostAtoms = int64_t(1) << 30;
-constexpr int64_t kSplitWaves = 3072;  // three to each SIMD
+constexpr int64_t kSimds = 1024;
 
 StructurePlan structure_plan(const tnr_structure_attention& r) {
     StructurePlan p{};
@@ -34,18 +35,21 @@ StructurePlan structure_plan(const tnr_structure_attention& r) {
     p.q_tiles = tile_start(r.n_queries, p.group, p.q_waves * kTile, r.n_structures);
     p.k_tiles = tile_start(r.n_keys, 1, p.k_waves * kTile, r.n_structures);
     // Few rows: the keys (or, for the keys' gradients, the rows) are split over
-    // workgroups, at least 8 tiles each, until there are waves enough for the
-    // device.
-    const auto split = [&](int64_t rows, int64_t others) {
+    // workgroups, at least 8 tiles each, into as many waves as the device holds of
+    // the kernel at once (`held` to a SIMD): a cluster of 4,001 atoms at three
+    // waves for all kernels took a second round of half the workgroups back.
+    const auto split = [&](int64_t rows, int64_t others, int held) {
         const int64_t waves = (rows / kTile + r.n_structures) * r.kv_heads;
         const int64_t most = r.n_structures > 0 ? others / r.n_structures / (8 * kTile) : 0;
-        int64_t n = waves > 0 ? kSplitWaves / waves : 1;
+        int64_t n = waves > 0 ? kSimds * held / waves : 1;
         if (n > most) n = most;
         if (n > 64) n = 64;
         return n < 2 ? 1 : (int)n;
     };
-    p.splits = split(r.n_queries * p.group, r.n_keys);
-    p.k_splits = split(r.n_keys, r.n_queries * p.group);
+    const bool wide = r.dtype == TNR_FLOAT32;
+    p.f_splits = split(r.n_queries * p.group, r.n_keys, r.dim <= 64 ? 3 : 2);
+    p.splits = split(r.n_queries * p.group, r.n_keys, wide && r.dim > 96 ? 1 : 2);
+    p.k_splits = split(r.n_keys, r.n_queries * p.group, r.dim > 64 ? 1 : 2);
     return p;
 }
 
@@ -144,8 +148,9 @@ StructureSpace structure_space(const tnr_structure_attention& r, const Structure
     };
     const size_t rows = (size_t)r.heads * r.n_queries;
     StructureSpace s{};
-    if (p.splits > 1)
-        s.part = (float*)part(rows * p.splits * (r.dim + (backward ? kRowSums : 2)) * 4);
+    const int splits = backward ? p.splits : p.f_splits;
+    if (splits > 1)
+        s.part = (float*)part(rows * splits * (r.dim + (backward ? kRowSums : 2)) * 4);
     if (backward) {
         if (p.k_splits > 1)
             s.part_k = (float*)part((size_t)r.kv_heads * r.n_keys * p.k_splits *
@@ -224,6 +229,7 @@ int tnr_structure_forward(const tnr_structure_attention* req, void* workspace,
     const hipStream_t st = (hipStream_t)stream;
     StructureArgs a = structure_args(r, p);
     a.part = s.part;
+    a.splits = p.f_splits;
     lay_tiles(r, p, a, r.lse != nullptr, st);
     if (r.n_queries == 0) return launched(err, err_len);
     with_type(r.dtype, [&](auto t) {
@@ -234,10 +240,10 @@ int tnr_structure_forward(const tnr_structure_attention* req, void* workspace,
                 constexpr int NW = decltype(w)::value;
                 constexpr bool CAP = decltype(c)::value;
                 k_structure_forward<T, DP, NW, CAP>
-                    <<<dim3((unsigned)(p.q_tiles * r.kv_heads), p.splits), NW * kWave, 0, st>>>(a);
+                    <<<dim3((unsigned)(p.q_tiles * r.kv_heads), p.f_splits), NW * kWave, 0, st>>>(a);
             });
         });
-        if (p.splits > 1)
+        if (p.f_splits > 1)
             k_structure_join<T>
                 <<<(unsigned)((r.n_queries * r.heads + 3) / 4), 256, 0, st>>>(a);
     });
