@@ -23,8 +23,6 @@ using f16 = _Float16;
 template <typename T, int N>
 using Vec = T __attribute__((ext_vector_type(N)));
 using f32x16 = Vec<float, 16>;
-using u32x4 = Vec<uint32_t, 4>;
-using u32x2 = Vec<uint32_t, 2>;
 
 __device__ __forceinline__ int lane_of() { return (int)__lane_id(); }
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }

@@ -6,6 +6,10 @@
 //
 // A digit has up to 10 bits (1,024 counters for each of a workgroup's 4 waves
 // in LDS), so that keys below 1,024 take one pass and below 2^20 two.
+//
+// A pass over 2.9 M pairs (8-byte payloads) takes 6 + 5 + 41 us: the move writes
+// runs of a few items, and what lies next to them comes from the next tiles.  With
+// tiles dealt to the XCDs in turn it took 64, since each wrote parts of all lines.
 #pragma once
 
 #include "op_common.h"

@@ -11,6 +11,12 @@
 // e = sum p (dp - do.o), which is what the rounding of o left out, and
 // corrects by it: sum p (dp - delta) f = sum p (dp - do.o) f - e sum p f.
 //
+// Both recompute a tile's scores, which costs seven products of matrices in place
+// of five but needs no sums across workgroups.  As the forward they are bound by
+// vector instructions: 4,001 atoms, 8 capped heads of 64 on 2, bfloat16: 251 us by
+// queries (726 instructions a tile) and 244 by keys, at two waves to a SIMD, whose
+// accumulators and rows fill its registers.
+//
 // float16: dx is scaled by a power of two that follows |do| (of the row, or the
 // largest so far of the rows that a key has met), and p by 2^12, so that
 // neither small upstream gradients nor the small weights of long rows fall out
