@@ -143,8 +143,8 @@ def main() -> None:
     print(f"loss: {losses[0]:.4f} -> {losses[-1]:.4f} in {len(losses)} steps")
     data = crystals(4, 1000, "cuda")
     energy, forces = predict(model, data, training=False)
-    print("energies of new crystals:", [round(float(e), 3) for e in energy])
-    print(f"largest force: {float(forces.norm(dim=1).max()):.3f}")
+    print("energies of new crystals:", [round(e, 3) for e in energy.detach().tolist()])
+    print(f"largest force: {float(forces.detach().norm(dim=1).max()):.3f}")
 
 
 if __name__ == "__main__":
