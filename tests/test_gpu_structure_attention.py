@@ -10,7 +10,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from tests._operators import assert_near, attend, distances, double, pointer, structure_pairs
+from tests._operators import HALF_SPACING, assert_near, attend, distances, double, pointer, structure_pairs
 from tonari_amd.attention import structure_attention
 
 pytestmark = pytest.mark.gpu
@@ -106,6 +106,25 @@ def test_queries_of_their_own(dtype, lengths, queries, heads, kv_heads, dim):
         if n == 0:
             rows = out[c["query_ptr"][b]:c["query_ptr"][b + 1]]
             assert bool((rows == 0).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES[1:], ids=IDS[1:])
+@pytest.mark.parametrize("lengths,queries,heads,kv_heads,dim", [
+    ([4000, 3973, 4500], [1, 1, 1], 2, 2, 40),  # keys split over workgroups
+    ([700, 40], [7, 3], 4, 1, 64),
+    ([550, 600, 3], [2, 2, 2], 8, 1, 128),
+    ([20, 5, 1, 32], None, 3, 3, 32),
+])
+def test_few_rows_round_once(dtype, lengths, queries, heads, kv_heads, dim):
+    # Few rows: the output's rounding, u |out|, is the only one to its type.  The weights' remainder
+    # after their rounding is rounded itself, u^2 of the weights, and 32-bit sums and scores add 2e-5
+    # of them, each times the values' magnitude.
+    c = make(lengths, heads, kv_heads, dim, dtype, queries=queries, grad=False)
+    out = call(c, 8.0).double().cpu()
+    ref, _ = expected(c, 8.0)
+    size, _ = expected({**c, "v": c["v"].abs()}, 8.0)
+    u = HALF_SPACING[dtype]
+    assert bool(((out - ref).abs() <= u * ref.abs() + (2e-5 + u * u) * size).all())
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)

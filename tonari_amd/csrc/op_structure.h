@@ -23,7 +23,11 @@
 //
 // The distance is computed in the tile from the positions, 32 bits.  Scores,
 // statistics and sums are 32 bits; the weights p and dx are rounded to the
-// inputs' 16-bit type for the second products.
+// inputs' 16-bit type for the second products.  With many rows that adds as much
+// error as the output's own rounding (together 1.4 times it, over all values).
+// With few, where one or two keys may make most of a row, it does not average
+// out; there the keys' rows bound the kernel, and the weights' remainder passes a
+// second product, which leaves the output's rounding alone (FINE).
 //
 // What bounds it: vector instructions, not the matrix cores.  A tile of 32 x 32
 // and one head takes about 25 instructions for each of a lane's 16 products
@@ -495,8 +499,9 @@ constexpr int waves_held(int dp) {
     return sizeof(T) == 4 ? (dp <= 32 ? 3 : dp <= 64 ? 2 : 1) : (dp <= 32 ? 4 : dp <= 64 ? 3 : 2);
 }
 
-// grid: (tiles * kv_heads, splits); NW waves of 32 query rows each.
-template <typename T, int DP, int NW, bool CAP>
+// grid: (tiles * kv_heads, splits); NW waves of 32 query rows each.  FINE: what
+// rounding took from the weights goes through a product of its own.
+template <typename T, int DP, int NW, bool CAP, bool FINE>
 __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP)) void k_structure_forward(
     const StructureArgs a) {
     using M = Mat<T>;
@@ -634,15 +639,17 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP)) void k_structure_forw
             for (int i = 0; i < 16; ++i) s[i] -= up;
         }
         float part[4] = {};
-        typename M::Weights p;
+        typename M::Weights p, rest;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const float w = exp2_of(s[i]);
             part[i % 4] += w;
             p.set(i, w);
+            if constexpr (FINE) rest.set(i, w - p.get(i));
         }
         sum += (part[0] + part[1]) + (part[2] + part[3]);
         M::template cols<DP>(acc, v_tile + sub * kValues, p);
+        if constexpr (FINE) M::template cols<DP>(acc, v_tile + sub * kValues, rest);
     };
     if (from < to) fetch(from);
     for (int tile = from; tile < to; tile += kTiles) {
