@@ -22,14 +22,11 @@
 // and one moved atom with 4 query heads to a key head fills 4 rows.
 //
 // The distance is computed in the tile from the positions, 32 bits.  Scores,
-// statistics and sums are 32 bits; the weights p and dx are rounded to the
-// inputs' 16-bit type for the second products.  With many rows that adds as much
-// error as the output's own rounding (together 1.4 times it, over all values).
-// With few, where one or two keys may make most of a row, it does not average
-// out; there the keys' rows bound the kernel, and the weights' remainder passes a
-// second product, which leaves the output's rounding alone (FINE).  One query in
-// each of 64 structures, 8 heads of 64 on 2 key heads, bfloat16: 132 us, and 127
-// without; in 6 structures of 4,000 atoms, float16, an error of 2.0e-4 for 3.2e-4.
+// statistics and sums are 32 bits.  The matrix products with 16-bit values take
+// 16-bit weights: these go in two pieces, rounded and rest, so that the output
+// is rounded once, at the end.  (One piece adds as much error as the output's own
+// rounding.)  float16 weights are lifted by 2^7, so that those of keys far below
+// the largest keep digits down to 2^-31 of it.
 //
 // What bounds it: vector instructions, not the matrix cores.  A tile of 32 x 32
 // and one head takes about 25 instructions for each of a lane's 16 products
@@ -501,9 +498,12 @@ constexpr int waves_held(int dp) {
     return sizeof(T) == 4 ? (dp <= 32 ? 3 : dp <= 64 ? 2 : 1) : (dp <= 32 ? 4 : dp <= 64 ? 3 : 2);
 }
 
-// grid: (tiles * kv_heads, splits); NW waves of 32 query rows each.  FINE: what
-// rounding took from the weights goes through a product of its own.
-template <typename T, int DP, int NW, bool CAP, bool FINE>
+// float16 has small values down to 2^-24 and large ones below 2^16.
+template <typename T>
+constexpr bool kNarrow = std::is_same_v<T, f16>;
+
+// grid: (tiles * kv_heads, splits); NW waves of 32 query rows each.
+template <typename T, int DP, int NW, bool CAP>
 __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP)) void k_structure_forward(
     const StructureArgs a) {
     using M = Mat<T>;
@@ -597,6 +597,8 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP)) void k_structure_forw
     // Weights are taken relative to `top`, the maximum when it was last set: it
     // is set anew only where a score passes it by more than 2^8 (the row's sums
     // then change their unit), so that most tiles neither subtract nor rescale.
+    // A lift lowers `top` below that maximum: weights reach up to 2^(8 + kLift).
+    constexpr float kLift = kNarrow<T> ? 7.f : 0.f;
     const auto weigh = [&](int sub, int left) {
         f32x16 dot{};
         M::template rows<DP>(dot, k_rows + sub * Pair::kRows, qr, a.dim);
@@ -629,11 +631,11 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP)) void k_structure_forw
             __builtin_amdgcn_sched_barrier(kLoadsPass);
         }
         high = max_halves(high);
-        const bool anew = high > 8.f || (top == -inf_of() && high > -inf_of());
+        const bool anew = high > 8.f + kLift || (top == -inf_of() && high > -inf_of());
         if (__builtin_amdgcn_ballot_w64(anew) != 0) {
-            const float up = anew ? high : 0.f;
+            const float up = anew ? high - kLift : 0.f;
             const float fade = exp2_of(-up);
-            top = anew ? ref + high : top;
+            top = anew ? ref + up : top;
             sum *= fade;
 #pragma unroll
             for (int d = 0; d < DP / 32; ++d) acc[d] *= fade;
@@ -647,11 +649,11 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP)) void k_structure_forw
             const float w = exp2_of(s[i]);
             part[i % 4] += w;
             p.set(i, w);
-            if constexpr (FINE) rest.set(i, w - p.get(i));
+            if constexpr (sizeof(T) == 2) rest.set(i, w - p.get(i));
         }
         sum += (part[0] + part[1]) + (part[2] + part[3]);
         M::template cols<DP>(acc, v_tile + sub * kValues, p);
-        if constexpr (FINE) M::template cols<DP>(acc, v_tile + sub * kValues, rest);
+        if constexpr (sizeof(T) == 2) M::template cols<DP>(acc, v_tile + sub * kValues, rest);
     };
     if (from < to) fetch(from);
     for (int tile = from; tile < to; tile += kTiles) {

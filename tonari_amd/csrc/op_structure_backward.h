@@ -28,11 +28,6 @@
 namespace tnr {
 namespace op {
 
-template <typename T>
-constexpr bool kNarrow = false;
-template <>
-constexpr bool kNarrow<f16> = true;
-
 constexpr int kNoScale = -1000;
 
 // Sums of a query row besides grad_q: e, sum (ds u, p u) for the unit vectors

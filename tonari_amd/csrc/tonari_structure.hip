@@ -20,7 +20,6 @@ int waves_for(int64_t rows, int64_t structures) {
 
 struct StructurePlan {
     int group, q_waves, k_waves;
-    bool fine;                       // the weights' remainder too, in the forward
     int f_splits, splits, k_splits;  // of the forward, the queries' pass back, the keys'
     int64_t q_tiles, k_tiles;
 };
@@ -35,8 +34,6 @@ StructurePlan structure_plan(const tnr_structure_attention& r) {
     p.k_waves = waves_for(r.n_keys, r.n_structures);
     p.q_tiles = tile_start(r.n_queries, p.group, p.q_waves * kTile, r.n_structures);
     p.k_tiles = tile_start(r.n_keys, 1, p.k_waves * kTile, r.n_structures);
-    // A structure's rows fill one wave at most: the keys' rows bound the forward.
-    p.fine = r.n_queries * p.group <= kTile * r.n_structures;
     // Few rows: the keys (or, for the keys' gradients, the rows) are split over
     // workgroups, at least 8 tiles each, into as many waves as the device holds of
     // the kernel at once (`held` to a SIMD): a cluster of 4,001 atoms at three
@@ -243,12 +240,7 @@ int tnr_structure_forward(const tnr_structure_attention* req, void* workspace,
                 constexpr int NW = decltype(w)::value;
                 constexpr bool CAP = decltype(c)::value;
                 const dim3 grid((unsigned)(p.q_tiles * r.kv_heads), p.f_splits);
-                if constexpr (NW == 2 && sizeof(T) == 2)
-                    if (p.fine) {
-                        k_structure_forward<T, DP, NW, CAP, true><<<grid, NW * kWave, 0, st>>>(a);
-                        return;
-                    }
-                k_structure_forward<T, DP, NW, CAP, false><<<grid, NW * kWave, 0, st>>>(a);
+                k_structure_forward<T, DP, NW, CAP><<<grid, NW * kWave, 0, st>>>(a);
             });
         });
         if (p.f_splits > 1)
