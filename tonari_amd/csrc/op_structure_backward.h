@@ -17,6 +17,9 @@
 // queries (726 instructions a tile) and 244 by keys, at two waves to a SIMD, whose
 // accumulators and rows fill its registers.
 //
+// 16-bit types: dx and p go through two products, rounded and rest, so that each
+// gradient is rounded once, at the end.
+//
 // float16: dx is scaled by a power of two that follows |do| (of the row, or the
 // largest so far of the rows that a key has met), and p by 2^12, so that
 // neither small upstream gradients nor the small weights of long rows fall out
@@ -382,7 +385,7 @@ k_structure_dkv(const StructureArgs a) {
         f32x16 dot{}, dp{};
         M::template rows<DP>(dot, q_rows + sub * Pair::kRows, kr, a.dim);
         M::template rows<DP>(dp, o_rows + sub * Pair::kRows, vr, a.dim);
-        typename M::Weights p, dx;
+        typename M::Weights p, p_rest, dx, dx_rest;
         const bool near = all_near<CAP>(dot, a.rule);
         float unit = 1.f;
         if (kNarrow<T>) {
@@ -426,8 +429,13 @@ k_structure_dkv(const StructureArgs a) {
                 const float w = exp2_of(fmaf(-slope2, r[e], u[e]) - lse[e]);
                 ds[e] = (kNarrow<T> ? w * kLower : w) * (dp[i] - delta[e]);
                 p.set(i, w);
-                const float dx_i = CAP ? ds[e] * bend[e] : ds[e];
-                dx.set(i, kNarrow<T> ? dx_i * unit : dx_i);
+                float dx_i = CAP ? ds[e] * bend[e] : ds[e];
+                if (kNarrow<T>) dx_i *= unit;
+                dx.set(i, dx_i);
+                if constexpr (sizeof(T) == 2) {  // what the rounding leaves out
+                    p_rest.set(i, w - p.get(i));
+                    dx_rest.set(i, dx_i - dx.get(i));
+                }
             }
             if (a.push_k) {
                 asm volatile("");  // one branch for the run
@@ -444,10 +452,12 @@ k_structure_dkv(const StructureArgs a) {
         px = fmaf(slope, ux, px);
         py = fmaf(slope, uy, py);
         pz = fmaf(slope, uz, pz);
-        M::template cols<DP>(
-            dv, M::kSeparateCols ? o_cols + sub * Pair::kCols : o_rows + sub * Pair::kRows, p);
-        M::template cols<DP>(
-            dk, M::kSeparateCols ? q_cols + sub * Pair::kCols : q_rows + sub * Pair::kRows, dx);
+        const T* oc = M::kSeparateCols ? o_cols + sub * Pair::kCols : o_rows + sub * Pair::kRows;
+        const T* qc = M::kSeparateCols ? q_cols + sub * Pair::kCols : q_rows + sub * Pair::kRows;
+        M::template cols<DP>(dv, oc, p);
+        if constexpr (sizeof(T) == 2) M::template cols<DP>(dv, oc, p_rest);
+        M::template cols<DP>(dk, qc, dx);
+        if constexpr (sizeof(T) == 2) M::template cols<DP>(dk, qc, dx_rest);
     };
     const bool busy = t.first + wave * kTile < t.n_k;  // a wave without keys only helps to stage
     const int each = (stages + a.k_splits - 1) / a.k_splits;
