@@ -30,7 +30,7 @@ extern "C" {
 #endif
 
 /* Version of this header's structs and functions. */
-#define TNR_OPERATORS_VERSION 1
+#define TNR_OPERATORS_VERSION 2
 
 /* Types besides TNR_FLOAT32. */
 #define TNR_BFLOAT16 2
@@ -91,8 +91,10 @@ typedef struct tnr_structure_attention {
     void* tiles;                    /* tnr_structure_tiles_size() bytes, 256-byte aligned: the batch
                                        as the forward cuts it up; the backward reads it */
     void* out;                      /* T[n_queries][heads][dim] */
+    float* out32;                   /* the same in 32 bits for the backward; NULL: not wanted
+                                       (with TNR_FLOAT32 the backward reads out) */
     float* lse;                     /* [heads][n_queries]: what the backward needs; NULL: not wanted */
-    /* backward: tiles, out and lse of the forward, and */
+    /* backward: tiles, out, out32 and lse of the forward, and */
     const void* grad_out;           /* T[n_queries][heads][dim] */
     void* grad_q;                   /* contiguous, like q, k and v; written whole */
     void* grad_k;

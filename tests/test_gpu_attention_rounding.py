@@ -104,6 +104,13 @@ def test_gradients_of_keys_and_values(dtype, lengths, queries, heads, kv_heads, 
     assert_rounded_once(case_of(lengths, queries, heads, kv_heads, dim, dtype, 0.0), 8.0, "kv")
 
 
+@pytest.mark.parametrize("dtype", DTYPES[1:], ids=IDS[1:])
+@pytest.mark.parametrize("mean", [0.0, 3.0])
+@pytest.mark.parametrize("lengths,queries,heads,kv_heads,dim", CASES)
+def test_gradient_of_queries(dtype, mean, lengths, queries, heads, kv_heads, dim):
+    assert_rounded_once(case_of(lengths, queries, heads, kv_heads, dim, dtype, mean), None, "q")
+
+
 def test_many_keys_that_weigh_little():
     # one near key and 20,000 far ones, whose weights of 2^-26 add up to 3e-4 of the row
     n, dim = 20_000, 16

@@ -252,3 +252,11 @@ def test_sizes_beyond_a_launch(lib):  # noqa: F811
                          structure(heads=1, kv_heads=1, n_queries=1 << 30, n_keys=1 << 30), PTR,
                          1 << 40)
     assert code == ext.TNR_INPUT_ERROR and "too many atoms" in said
+
+
+def test_structure_backward_needs_the_wide_output(lib):  # noqa: F811
+    need = lib.tnr_structure_backward_workspace_size(ctypes.byref(structure()))
+    code, said = refused(lib.tnr_structure_backward, structure(out32=None), PTR, need)
+    assert code == ext.TNR_INPUT_ERROR and "pointers are null" in said
+    code, said = refused(lib.tnr_structure_backward, structure(out32=PTR + 4), PTR, need)
+    assert code == ext.TNR_INPUT_ERROR and "aligned" in said

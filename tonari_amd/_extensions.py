@@ -115,7 +115,7 @@ class SkinList(ctypes.Structure):
 
 
 # include/tonari_operators.h: the operators beside the search.
-OPERATORS_VERSION = 1
+OPERATORS_VERSION = 2
 OPERATOR_EXPORTS = (
     "tnr_operators_version",
     "tnr_embedding_forward",
@@ -179,6 +179,7 @@ class StructureAttention(ctypes.Structure):
         ("softcap", ctypes.c_float),
         ("tiles", ctypes.c_void_p),
         ("out", ctypes.c_void_p),
+        ("out32", ctypes.c_void_p),
         ("lse", ctypes.c_void_p),
         ("grad_out", ctypes.c_void_p),
         ("grad_q", ctypes.c_void_p),

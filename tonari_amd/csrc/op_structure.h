@@ -63,6 +63,7 @@ struct StructureArgs {
     int n_queries, n_keys;
     int splits, k_splits;
     void* out;
+    float* out32;  // out before its rounding to 16 bits, NULL: not wanted
     float* lse;   // [heads][n_queries], base 2
     float* part;    // splits of a row: [split][heads][n_queries][dim + 2], or dim + kRowSums
     float* part_k;  // splits of a key: [split][kv_heads][n_keys][2 dim + 3]
@@ -175,13 +176,42 @@ struct Mat16 {
                 if (p && c < dim) x[s] = *(const Frag*)(p + c);
             }
         }
-        // Row for row, by the matrix product that also makes a query's product
-        // with a value: equal rows give equal bits.
-        __device__ __forceinline__ float dot(const Row& o) const {
-            f32x16 all{};
+        // With a row of 32 bits, in three pieces of T (float16's are lifted by
+        // 2^11 each, which its range would else cut off), by the matrix product
+        // that also makes a query's product with a value: a row that T holds gives
+        // the same bits as that product.
+        __device__ __forceinline__ float dot32(const float* p, int dim) const {
+            constexpr float kLift = std::is_same_v<T, f16> ? 2048.f : 1.f;
+            const int half = lane_of() / 32;
+            float rest[DP / 16][8], sum = 0.f, by = 1.f;
 #pragma unroll
-            for (int s = 0; s < DP / 16; ++s) all = F::mma(o.x[s], x[s], all);
-            return diagonal(all);
+            for (int s = 0; s < DP / 16; ++s) {
+                const int c = 16 * s + 8 * half;
+                Vec<float, 4> lo{}, hi{};
+                if (p && c < dim) {
+                    lo = *(const Vec<float, 4>*)(p + c);
+                    hi = *(const Vec<float, 4>*)(p + c + 4);
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) rest[s][e] = e < 4 ? lo[e % 4] : hi[e % 4];
+            }
+#pragma unroll
+            for (int piece = 0; piece < 3; ++piece) {
+                f32x16 all{};
+#pragma unroll
+                for (int s = 0; s < DP / 16; ++s) {
+                    Frag o;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        o[e] = rounded<T>(rest[s][e]);
+                        rest[s][e] = (rest[s][e] - (float)o[e]) * kLift;
+                    }
+                    all = F::mma(o, x[s], all);
+                }
+                sum = fmaf(diagonal(all), by, sum);
+                by *= 1.f / kLift;
+            }
+            return sum;
         }
         __device__ __forceinline__ float largest() const {
             float top = 0.f;
@@ -296,7 +326,9 @@ struct Mat<float> {
                     x[s] = *(const Vec<float, 4>*)(p + half * (dim / 2) + 4 * s);
             }
         }
-        __device__ __forceinline__ float dot(const Row& o) const {
+        __device__ __forceinline__ float dot32(const float* p, int dim) const {
+            Row o;
+            o.load(p, dim);
             f32x16 all{};
 #pragma unroll
             for (int s = 0; s < DP / 8; ++s)
@@ -528,6 +560,9 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP)) void k_structure_forw
         const int query = (int)(row / g), head = kv * g + (int)(row % g);
         T* out = (T*)a.out + ((int64_t)query * a.heads + head) * a.dim;
         for (int c = 0; c < a.dim; ++c) out[c] = rounded<T>(nan_of());
+        if (a.out32)
+            for (int c = 0; c < a.dim; ++c)
+                a.out32[((int64_t)query * a.heads + head) * a.dim + c] = nan_of();
         if (a.lse) a.lse[(int64_t)head * a.n_queries + query] = nan_of();
         if (a.splits > 1)
             for (int s = 0; s < a.splits; ++s) {
@@ -682,7 +717,9 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP)) void k_structure_forw
         return;
     }
     const float by = sum == 0.f ? 0.f : 1.f / sum;
-    store_channels<T, DP>((T*)a.out + ((int64_t)query * a.heads + head) * a.dim, a.dim, acc, by);
+    const int64_t flat = ((int64_t)query * a.heads + head) * a.dim;
+    store_channels<T, DP>((T*)a.out + flat, a.dim, acc, by);
+    if (a.out32) store_channels<float, DP>(a.out32 + flat, a.dim, acc, by);
     if (a.lse && half == 0)
         a.lse[(int64_t)head * a.n_queries + query] =
             sum == 0.f ? -inf_of() : top + __builtin_amdgcn_logf(sum);
@@ -714,9 +751,14 @@ __global__ __launch_bounds__(256) void k_structure_join(const StructureArgs a) {
     }
     const int head = (int)(at / a.n_queries), query = (int)(at % a.n_queries);
     const float by = sum == 0.f ? 0.f : 1.f / sum;
-    T* out = (T*)a.out + ((int64_t)query * a.heads + head) * a.dim;
+    const int64_t flat = ((int64_t)query * a.heads + head) * a.dim;
+    T* out = (T*)a.out + flat;
     if (lane < a.dim) out[lane] = rounded<T>(x0 * by);
     if (lane + kWave < a.dim) out[lane + kWave] = rounded<T>(x1 * by);
+    if (a.out32) {
+        if (lane < a.dim) a.out32[flat + lane] = x0 * by;
+        if (lane + kWave < a.dim) a.out32[flat + lane + kWave] = x1 * by;
+    }
     if (a.lse && lane == 0)
         a.lse[at] = sum == 0.f ? -inf_of() : top + __builtin_amdgcn_logf(sum);
 }

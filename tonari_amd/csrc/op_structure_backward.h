@@ -5,11 +5,12 @@
 // keys' share of the positions' gradient).  Neither needs an atomic, so the
 // sums' order is fixed by the sizes.
 //
-// delta = do.o from the rounded output is good enough for grad_q, grad_k and
-// grad_v, which are rounded to the same type, but not for the gradients of
-// positions and slopes, which are 32-bit: the queries' pass also sums
-// e = sum p (dp - do.o), which is what the rounding of o left out, and
-// corrects by it: sum p (dp - delta) f = sum p (dp - do.o) f - e sum p f.
+// delta = do.o is taken from the forward's output in 32 bits.  The rounding of a
+// 16-bit output, times sum p k, would show in grad_q where keys have a component
+// in common: 200 keys of mean 3, bfloat16, 32 channels, a tenth of it.  What is
+// left, e = sum p (dp - do.o) of the weights' own rounding, is summed by the
+// queries' pass and taken out of the gradients of positions and slopes, which are
+// 32-bit: sum p (dp - delta) f = sum p (dp - do.o) f - e sum p f.
 //
 // Both recompute a tile's scores, which costs seven products of matrices in place
 // of five but needs no sums across workgroups.  As the forward they are bound by
@@ -80,6 +81,10 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP <= 32 ? 64 : 2 * DP)) v
         if (a.splits > 1) {
             float* part = a.part + ((int64_t)split * a.heads * a.n_queries + at) * (a.dim + kRowSums);
             for (int c = 0; c < a.dim + kRowSums; ++c) part[c] = nan_of();
+            if (split == 0) {
+                a.row[2 * at] = nan_of();
+                a.row[2 * at + 1] = 1.f;
+            }
             return;
         }
         T* dq = (T*)a.grad_q + ((int64_t)query * a.heads + head) * a.dim;
@@ -103,13 +108,9 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP <= 32 ? 64 : 2 * DP)) v
     qr.load(valid ? (const T*)a.q + (int64_t)query * a.q_stride[0] + head * a.q_stride[1] : nullptr,
             a.dim);
     dor.load(valid ? (const T*)a.grad_out + flat : nullptr, a.dim);
-    float delta, largest = 1.f;
-    {
-        Row o;
-        o.load(valid ? (const T*)a.out + flat : nullptr, a.dim);
-        delta = dor.dot(o);
-    }
-    float unit = 1.f;
+    const float* full = sizeof(T) == 4 ? (const float*)a.out : a.out32;
+    const float delta = dor.dot32(valid ? full + flat : nullptr, a.dim);
+    float unit = 1.f, largest = 1.f;
     if (kNarrow<T>) {
         largest = dor.largest();
         unit = power_of(-exponent_of(largest));
@@ -258,16 +259,22 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP <= 32 ? 64 : 2 * DP)) v
                 const int c = 32 * d + row_of(i, half);
                 if (c < a.dim) part[c] = acc[d][i] * by;
             }
-        if (half == 0)
+        if (half == 0) {
 #pragma unroll
             for (int i = 0; i < kRowSums; ++i) part[a.dim + i] = w[i];
+            if (split == 0) {
+                a.row[2 * at] = delta;
+                a.row[2 * at + 1] = largest;
+            }
+        }
         return;
     }
     store_channels<T, DP>((T*)a.grad_q + flat, a.dim, acc, a.rule.scale / unit);
     if (half == 0) finish_row(a, head, query, delta, largest, slope, w);
 }
 
-// Joins the splits of a row of the queries' pass: one wave each.
+// Joins the splits of a row of the queries' pass: one wave each.  (The first
+// split has put the row's delta down.)
 template <typename T>
 __global__ __launch_bounds__(256) void k_structure_join_dq(const StructureArgs a) {
     const int64_t at = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
@@ -286,20 +293,11 @@ __global__ __launch_bounds__(256) void k_structure_join_dq(const StructureArgs a
         if (lane + kWave < a.dim) x1 += p[lane + kWave];
         for (int i = 0; i < kRowSums; ++i) w[i] += p[a.dim + i];
     }
-    float delta = 0.f, top = 0.f;
-    for (int c = lane; c < a.dim; c += kWave) {
-        const float go = (float)((const T*)a.grad_out)[flat + c];
-        delta = fmaf(go, (float)((const T*)a.out)[flat + c], delta);
-        top = fmaxf(top, fabsf(go));
-    }
-    for (int d = 32; d > 0; d >>= 1) {
-        delta += __shfl_xor(delta, d);
-        top = fmaxf(top, __shfl_xor(top, d));
-    }
     T* dq = (T*)a.grad_q + flat;
     if (lane < a.dim) dq[lane] = rounded<T>(x0 * a.rule.scale);
     if (lane + kWave < a.dim) dq[lane + kWave] = rounded<T>(x1 * a.rule.scale);
-    if (lane == 0) finish_row(a, head, query, delta, top, a.slopes[head], w);
+    if (lane == 0)
+        finish_row(a, head, query, a.row[2 * at], a.row[2 * at + 1], a.slopes[head], w);
 }
 
 // grid: (key tiles * kv_heads, k_splits); NW waves of 32 keys each.

@@ -78,7 +78,8 @@ int check_structure(const tnr_structure_attention* r, bool backward, char* err, 
         (r->n_keys > 0 && (!r->k || !r->v || !r->positions)))
         return refuse(err, len, "required pointers are null");
     if (!aligned(r->q, r->q_stride, r->dtype) || !aligned(r->k, r->k_stride, r->dtype) ||
-        !aligned(r->v, r->v_stride, r->dtype) || (uintptr_t)r->out % 16 != 0)
+        !aligned(r->v, r->v_stride, r->dtype) || (uintptr_t)r->out % 16 != 0 ||
+        (uintptr_t)r->out32 % 16 != 0)
         return refuse(err, len, "q, k, v and out must be aligned to 16 bytes, with strides up to 2^24");
     if (backward) {
         if ((r->n_queries > 0 && (!r->grad_out || !r->grad_q || !r->lse)) ||
@@ -126,6 +127,7 @@ StructureArgs structure_args(const tnr_structure_attention& r, const StructurePl
     a.splits = p.splits;
     a.k_splits = p.k_splits;
     a.out = r.out;
+    a.out32 = r.out32;
     a.lse = r.lse;
     a.grad_out = r.grad_out;
     a.grad_q = r.grad_q;
@@ -264,6 +266,8 @@ int tnr_structure_backward(const tnr_structure_attention* req, void* workspace,
     const StructureSpace s = structure_space(r, p, true, workspace);
     if (s.bytes > 0 && (!workspace || (uintptr_t)workspace % 256 != 0 || workspace_bytes < s.bytes))
         return refuse(err, err_len, "workspace is too small or not aligned to 256 bytes");
+    if (r.dtype != TNR_FLOAT32 && r.n_queries > 0 && !r.out32)
+        return refuse(err, err_len, "required pointers are null");
     const hipStream_t st = (hipStream_t)stream;
     StructureArgs a = structure_args(r, p);
     a.part = s.part;

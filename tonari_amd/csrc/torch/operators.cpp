@@ -237,9 +237,14 @@ struct StructureCall {
     }
 };
 
-Tensor structure_forward(StructureCall& c, Tensor* lse) {
+// `lse` and `full`: what the backward reads, NULL where there is none.
+Tensor structure_forward(StructureCall& c, Tensor* lse, Tensor* full) {
     const Tensor out = at::empty(c.q.sizes(), c.q.options());
     c.r.out = out.data_ptr();
+    if (full && c.r.dtype != TNR_FLOAT32) {
+        *full = at::empty(c.q.sizes(), c.slopes.options());
+        c.r.out32 = (float*)full->data_ptr();
+    }
     if (lse) {
         *lse = at::empty({c.q.size(1), c.q.size(0)}, c.slopes.options());
         c.r.lse = (float*)lse->data_ptr();
@@ -260,10 +265,10 @@ struct StructureAttention : torch::autograd::Function<StructureAttention> {
         const Tensor x_q = query_positions.value_or(Tensor());
         const Tensor query_ptr = query_ptr_.value_or(Tensor());
         StructureCall c(q, k, v, x, slopes, x_q, batch_ptr, query_ptr, scale, softcap);
-        Tensor lse;
-        const Tensor out = structure_forward(c, &lse);
+        Tensor lse, full;
+        const Tensor out = structure_forward(c, &lse, &full);
         ctx->save_for_backward(
-            {q, k, v, x, slopes, x_q, batch_ptr, query_ptr, out, lse, c.tiles});
+            {q, k, v, x, slopes, x_q, batch_ptr, query_ptr, out, lse, c.tiles, full});
         ctx->saved_data["scale"] = scale;
         ctx->saved_data["softcap"] = softcap;
         return out;
@@ -302,9 +307,10 @@ struct StructureAttention : torch::autograd::Function<StructureAttention> {
             return all;
         }
         StructureCall c(s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], scale, softcap, s[10]);
-        const Tensor &out = s[8], &lse = s[9];
+        const Tensor &out = s[8], &lse = s[9], &full = s[11];
         const Tensor go = flat(grads[0]);
         c.r.out = out.data_ptr();
+        c.r.out32 = full.defined() ? (float*)full.data_ptr() : nullptr;
         c.r.lse = (float*)lse.data_ptr();
         c.r.grad_out = go.data_ptr();
         all[0] = at::empty(c.q.sizes(), c.q.options());
@@ -344,7 +350,7 @@ Tensor structure_attention(const Tensor& q, const Tensor& k, const Tensor& v, co
                                          scale, softcap);
     c10::DeviceGuard guard(q.device());
     StructureCall c(q, k, v, x, slopes, x_q, batch_ptr, q_ptr, scale, softcap);
-    return structure_forward(c, nullptr);
+    return structure_forward(c, nullptr, nullptr);
 }
 
 // ------------------------------------------------------- neighbor attention
