@@ -126,3 +126,31 @@ def test_many_keys_that_weigh_little():
     want = 2.0 * (n - 1) * 2.0**-26 / (1 + (n - 1) * 2.0**-26)
     out = call(c)
     assert bool(((out.double() - want).abs() <= (2.0**-11 + 2e-5) * want + 2.0**-24).all())
+
+
+@pytest.mark.parametrize("opposite", [False, True])
+@pytest.mark.parametrize("scale", [0.9, 0.9e-3])
+@pytest.mark.parametrize("lengths,queries", [([2], None), ([40], None), ([2], [600]), ([600], [2])])
+def test_large_values(lengths, queries, scale, opposite):
+    # sums over 64 channels of values of 3,000 lie far beyond float16, the gradients within it
+    c = make(lengths, 1, 1, 64, torch.float16, queries=queries, seed=28)
+    sign = torch.where(torch.arange(sum(lengths), device="cuda") % 2 == 0, 1.0, -1.0)
+    with torch.no_grad():
+        c["v"].copy_(3000.0 * sign[:, None, None].expand_as(c["v"]))
+        c["q"].mul_(0.01)
+        c["k"].mul_(0.01)
+        c["slopes"].zero_()
+        c["upstream"] = torch.full_like(c["upstream"], scale)
+        if opposite:
+            c["upstream"][1::2] *= -1
+    assert_rounded_once(c, None, "qkv")
+
+
+def test_small_gradients_beside_large_ones():
+    # rows whose upstream gradient is 2^-12 of the others', and scores that spread over 2^20
+    c = make([70], 2, 2, 32, torch.float16, seed=29)
+    with torch.no_grad():
+        c["upstream"][::3] *= 2.0**-12
+        c["v"].mul_(64.0)
+        c["q"].mul_(4.0)
+    assert_rounded_once(c, None, "qkv")

@@ -69,7 +69,7 @@ struct StructureArgs {
     float* part_k;  // splits of a key: [split][kv_heads][n_keys][2 dim + 3]
     const void* grad_out;
     void *grad_q, *grad_k, *grad_v;
-    float* row;     // [heads][n_queries][2]: delta, largest |grad_out|
+    float* row;     // [heads][n_queries]: delta
     float* push_q;  // [heads][n_queries][3], NULL: not wanted
     float* push_k;  // [kv_heads][n_keys][3]
     float* turn;    // [heads][n_queries]: the slope's gradient by rows, NULL: not wanted
@@ -213,14 +213,6 @@ struct Mat16 {
             }
             return sum;
         }
-        __device__ __forceinline__ float largest() const {
-            float top = 0.f;
-#pragma unroll
-            for (int s = 0; s < DP / 16; ++s)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf((float)x[s][e]));
-            return max_halves(top);
-        }
     };
 
     // acc += tile . row^T over the first `dim` channels
@@ -337,7 +329,6 @@ struct Mat<float> {
                     all = __builtin_amdgcn_mfma_f32_32x32x2f32(o.x[s][e], x[s][e], all, 0, 0, 0);
             return diagonal(all);
         }
-        __device__ __forceinline__ float largest() const { return 1.f; }
     };
 
     template <int DP>

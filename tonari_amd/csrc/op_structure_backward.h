@@ -21,10 +21,10 @@
 // 16-bit types: dx and p go through two products, rounded and rest, so that each
 // gradient is rounded once, at the end.
 //
-// float16: dx is scaled by a power of two that follows |do| (of the row, or the
-// largest so far of the rows that a key has met), and p by 2^12, so that
-// neither small upstream gradients nor the small weights of long rows fall out
-// of the type's range.  bfloat16 has the range of 32 bits.
+// float16: dx is scaled by a power of two that follows the largest |dx| that a
+// row (or, in the keys' pass, a key) has met so far, to below 2^14, and p by 2^12, so
+// that neither large values nor small upstream gradients nor the small weights
+// of long rows fall out of the type's range.  bfloat16 has the range of 32 bits.
 #pragma once
 
 #include "op_structure.h"
@@ -32,24 +32,40 @@
 namespace tnr {
 namespace op {
 
-constexpr int kNoScale = -1000;
-
 // Sums of a query row besides grad_q: e, sum (ds u, p u) for the unit vectors
 // u, sum (ds (r - r'), p (r - r')) for one r' of the row.
 constexpr int kRowSums = 9;
 
 __device__ __forceinline__ float power_of(int e) { return __builtin_amdgcn_ldexpf(1.f, e); }
-__device__ __forceinline__ int exponent_of(float x) {
-    return x > 0.f && x < inf_of() ? __builtin_amdgcn_frexp_expf(x) : 0;
-}
+
+// The scale of a lane's dx: 2^kMost / 2^e, where 2^e is above all of them so far.
+struct Unit {
+    static constexpr int kMost = 14;
+    int e = -100;
+    __device__ __forceinline__ float by() const { return power_of(kMost - e); }
+    __device__ __forceinline__ float back() const { return power_of(e - kMost); }
+    // Takes the 16 of a tile; sums of earlier ones change their unit with it.
+    template <int N>
+    __device__ __forceinline__ void meet(const f32x16& dx, f32x16 (&sums)[N]) {
+        float top = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(dx[i]));
+        top = max_halves(top);
+        const int next = top > 0.f && top < inf_of() ? __builtin_amdgcn_frexp_expf(top) : e;
+        if (next <= e) return;
+        const float fade = power_of(e - next);
+#pragma unroll
+        for (int d = 0; d < N; ++d) sums[d] *= fade;
+        e = next;
+    }
+};
 
 // What a row's sums make, for its own lane.
 __device__ __forceinline__ void finish_row(const StructureArgs& a, int head, int query,
-                                           float delta, float largest, float slope,
+                                           float delta, float slope,
                                            const float (&w)[kRowSums]) {
     const int64_t at = (int64_t)head * a.n_queries + query;
-    a.row[2 * at] = delta + w[0];
-    a.row[2 * at + 1] = largest;
+    a.row[at] = delta + w[0];
     if (a.push_q)
         for (int c = 0; c < 3; ++c) a.push_q[3 * at + c] = -slope * (w[1 + c] - w[0] * w[4 + c]);
     if (a.turn) a.turn[at] = -(w[7] - w[0] * w[8]);
@@ -81,16 +97,13 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP <= 32 ? 64 : 2 * DP)) v
         if (a.splits > 1) {
             float* part = a.part + ((int64_t)split * a.heads * a.n_queries + at) * (a.dim + kRowSums);
             for (int c = 0; c < a.dim + kRowSums; ++c) part[c] = nan_of();
-            if (split == 0) {
-                a.row[2 * at] = nan_of();
-                a.row[2 * at + 1] = 1.f;
-            }
+            if (split == 0) a.row[at] = nan_of();
             return;
         }
         T* dq = (T*)a.grad_q + ((int64_t)query * a.heads + head) * a.dim;
         for (int c = 0; c < a.dim; ++c) dq[c] = rounded<T>(nan_of());
         const float w[kRowSums] = {nan_of()};
-        finish_row(a, head, query, 0.f, 1.f, 1.f, w);
+        finish_row(a, head, query, 0.f, 1.f, w);
         return;
     }
     const int rows = t.n_q * g;
@@ -110,11 +123,7 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP <= 32 ? 64 : 2 * DP)) v
     dor.load(valid ? (const T*)a.grad_out + flat : nullptr, a.dim);
     const float* full = sizeof(T) == 4 ? (const float*)a.out : a.out32;
     const float delta = dor.dot32(valid ? full + flat : nullptr, a.dim);
-    float unit = 1.f, largest = 1.f;
-    if (kNarrow<T>) {
-        largest = dor.largest();
-        unit = power_of(-exponent_of(largest));
-    }
+    Unit unit;
     float xq = 0.f, yq = 0.f, zq = 0.f, slope = 0.f, lse = inf_of();
     if (valid) {
         xq = a.x_q[3 * (int64_t)query];
@@ -207,10 +216,13 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP <= 32 ? 64 : 2 * DP)) v
                 const int i = 4 * run + e;
                 ds[e] = s[e] * (dp[i] - delta);
                 tw[0] += ds[e];
-                float dx_i = CAP ? ds[e] * bend[e] : ds[e];
-                if (kNarrow<T>) dx_i *= unit;
-                p.set(i, dx_i);
-                if (sizeof(T) == 2) rest.set(i, dx_i - p.get(i));
+                const float dx_i = CAP ? ds[e] * bend[e] : ds[e];
+                if constexpr (kNarrow<T>) {
+                    dot[i] = dx_i;  // (its product is done with)
+                } else {
+                    p.set(i, dx_i);
+                    if (sizeof(T) == 2) rest.set(i, dx_i - p.get(i));
+                }
             }
             if (geometry) {
                 asm volatile("");  // one branch for the run
@@ -232,6 +244,15 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP <= 32 ? 64 : 2 * DP)) v
         }
 #pragma unroll
         for (int i = 0; i < kRowSums; ++i) w[i] += tw[i];
+        if constexpr (kNarrow<T>) {
+            unit.meet(dot, acc);
+            const float by = unit.by();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                p.set(i, dot[i] * by);
+                rest.set(i, dot[i] * by - p.get(i));
+            }
+        }
         // Their sum over a row is 0, so grad_q is a difference: what the rounding of
         // dx leaves out goes through a second product.
         const T* cols = M::kSeparateCols ? k_cols + sub * Pair::kCols : k_rows + sub * Pair::kRows;
@@ -251,7 +272,7 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP <= 32 ? 64 : 2 * DP)) v
     if (!valid) return;
     if (a.splits > 1) {
         float* part = a.part + ((int64_t)split * a.heads * a.n_queries + at) * (a.dim + kRowSums);
-        const float by = 1.f / unit;
+        const float by = kNarrow<T> ? unit.back() : 1.f;
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
@@ -262,15 +283,13 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP <= 32 ? 64 : 2 * DP)) v
         if (half == 0) {
 #pragma unroll
             for (int i = 0; i < kRowSums; ++i) part[a.dim + i] = w[i];
-            if (split == 0) {
-                a.row[2 * at] = delta;
-                a.row[2 * at + 1] = largest;
-            }
+            if (split == 0) a.row[at] = delta;
         }
         return;
     }
-    store_channels<T, DP>((T*)a.grad_q + flat, a.dim, acc, a.rule.scale / unit);
-    if (half == 0) finish_row(a, head, query, delta, largest, slope, w);
+    store_channels<T, DP>((T*)a.grad_q + flat, a.dim, acc,
+                          kNarrow<T> ? a.rule.scale * unit.back() : a.rule.scale);
+    if (half == 0) finish_row(a, head, query, delta, slope, w);
 }
 
 // Joins the splits of a row of the queries' pass: one wave each.  (The first
@@ -296,8 +315,7 @@ __global__ __launch_bounds__(256) void k_structure_join_dq(const StructureArgs a
     T* dq = (T*)a.grad_q + flat;
     if (lane < a.dim) dq[lane] = rounded<T>(x0 * a.rule.scale);
     if (lane + kWave < a.dim) dq[lane + kWave] = rounded<T>(x1 * a.rule.scale);
-    if (lane == 0)
-        finish_row(a, head, query, a.row[2 * at], a.row[2 * at + 1], a.slopes[head], w);
+    if (lane == 0) finish_row(a, head, query, a.row[at], a.slopes[head], w);
 }
 
 // grid: (key tiles * kv_heads, k_splits); NW waves of 32 keys each.
@@ -315,7 +333,7 @@ k_structure_dkv(const StructureArgs a) {
     __shared__ alignas(16) T q_cols[M::kSeparateCols ? kTiles * Pair::kCols : 8];
     __shared__ alignas(16) T o_cols[M::kSeparateCols ? kTiles * Pair::kCols : 8];
     __shared__ TilePositions<kTiles> x_q;
-    __shared__ alignas(16) float stat[3][kQueries];  // log-sum, delta, largest |grad_out|
+    __shared__ alignas(16) float stat[2][kQueries];  // log-sum, delta
 
     const uint32_t order = xcd_order(blockIdx.x, gridDim.x), block = order / (uint32_t)a.kv_heads;
     const StructureTile t = a.k_tiles[block];
@@ -353,12 +371,12 @@ k_structure_dkv(const StructureArgs a) {
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d) dk[d] = dv[d] = f32x16{};
     float px = 0.f, py = 0.f, pz = 0.f;
-    int scale_e = kNoScale;  // exponent of what dk is held in
+    Unit unit;  // what dk is held in
 
     // stages of kTiles tiles, of one head after the other
     const int per_head = (t.n_q + kQueries - 1) / kQueries, stages = per_head * a.group;
     Pair stage;
-    float xs[3], ss[3];
+    float xs[3], ss[2];
     const auto fetch = [&](int at_stage) {
         const int head = kv * a.group + at_stage / per_head;
         const int q0 = (at_stage % per_head) * kQueries, n = t.n_q - q0;
@@ -374,8 +392,7 @@ k_structure_dkv(const StructureArgs a) {
             for (int c = 0; c < 3; ++c) xs[c] = a.x_q[3 * query + c];
             ss[0] = in ? a.lse[at] : inf_of();  // no weight beyond the rows
             if (ss[0] == -inf_of()) ss[0] = inf_of();
-            ss[1] = a.row[2 * at];
-            ss[2] = in ? a.row[2 * at + 1] : 0.f;
+            ss[1] = a.row[at];
         }
     };
     const auto pull = [&](int sub, float slope) {
@@ -385,25 +402,6 @@ k_structure_dkv(const StructureArgs a) {
         M::template rows<DP>(dp, o_rows + sub * Pair::kRows, vr, a.dim);
         typename M::Weights p, p_rest, dx, dx_rest;
         const bool near = all_near<CAP>(dot, a.rule);
-        float unit = 1.f;
-        if (kNarrow<T>) {
-            float tile_top = 0.f;
-#pragma unroll
-            for (int run = 0; run < 4; ++run) {
-                const Vec<float, 4> largest = four_of(stat[2] + sub * kTile, run, half);
-                tile_top = fmaxf(fmaxf(fmaxf(tile_top, largest[0]), largest[1]),
-                                 fmaxf(largest[2], largest[3]));
-            }
-            tile_top = max_halves(tile_top);
-            const int e = exponent_of(tile_top);
-            if (tile_top > 0.f && e > scale_e) {  // (all zeros: dx is zero whatever the scale)
-                const float by = scale_e == kNoScale ? 1.f : power_of(scale_e - e);
-#pragma unroll
-                for (int d = 0; d < DP / 32; ++d) dk[d] *= by;
-                scale_e = e;
-            }
-            unit = scale_e == kNoScale ? 1.f : power_of(-scale_e);
-        }
         float ux = 0.f, uy = 0.f, uz = 0.f;
 #pragma unroll
         for (int run = 0; run < 4; ++run) {
@@ -427,12 +425,14 @@ k_structure_dkv(const StructureArgs a) {
                 const float w = exp2_of(fmaf(-slope2, r[e], u[e]) - lse[e]);
                 ds[e] = (kNarrow<T> ? w * kLower : w) * (dp[i] - delta[e]);
                 p.set(i, w);
-                float dx_i = CAP ? ds[e] * bend[e] : ds[e];
-                if (kNarrow<T>) dx_i *= unit;
-                dx.set(i, dx_i);
-                if constexpr (sizeof(T) == 2) {  // what the rounding leaves out
-                    p_rest.set(i, w - p.get(i));
-                    dx_rest.set(i, dx_i - dx.get(i));
+                // (the rests are what the rounding leaves out)
+                if constexpr (sizeof(T) == 2) p_rest.set(i, w - p.get(i));
+                const float dx_i = CAP ? ds[e] * bend[e] : ds[e];
+                if constexpr (kNarrow<T>) {
+                    dot[i] = dx_i;  // (its product is done with)
+                } else {
+                    dx.set(i, dx_i);
+                    if constexpr (sizeof(T) == 2) dx_rest.set(i, dx_i - dx.get(i));
                 }
             }
             if (a.push_k) {
@@ -454,6 +454,15 @@ k_structure_dkv(const StructureArgs a) {
         const T* qc = M::kSeparateCols ? q_cols + sub * Pair::kCols : q_rows + sub * Pair::kRows;
         M::template cols<DP>(dv, oc, p);
         if constexpr (sizeof(T) == 2) M::template cols<DP>(dv, oc, p_rest);
+        if constexpr (kNarrow<T>) {
+            unit.meet(dot, dk);
+            const float by = unit.by();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                dx.set(i, dot[i] * by);
+                dx_rest.set(i, dot[i] * by - dx.get(i));
+            }
+        }
         M::template cols<DP>(dk, qc, dx);
         if constexpr (sizeof(T) == 2) M::template cols<DP>(dk, qc, dx_rest);
     };
@@ -469,7 +478,7 @@ k_structure_dkv(const StructureArgs a) {
 #pragma unroll
             for (int c = 0; c < 3; ++c) {
                 x_q.x[c][threadIdx.x] = xs[c];
-                stat[c][threadIdx.x] = ss[c];
+                if (c < 2) stat[c][threadIdx.x] = ss[c];
             }
         __syncthreads();
         if (i + 1 < to) fetch(i + 1);
@@ -483,7 +492,7 @@ k_structure_dkv(const StructureArgs a) {
     pz = sum_halves(pz);
     if (!valid) return;
     const int64_t flat = (key * a.kv_heads + kv) * a.dim;
-    const float back = kNarrow<T> && scale_e != kNoScale ? power_of(scale_e) : 1.f;
+    const float back = kNarrow<T> ? unit.back() : 1.f;
     if (a.k_splits > 1) {
         float* part =
             a.part_k + (((int64_t)split * a.kv_heads + kv) * a.n_keys + key) * (2 * a.dim + 3);

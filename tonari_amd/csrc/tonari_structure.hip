@@ -157,7 +157,7 @@ StructureSpace structure_space(const tnr_structure_attention& r, const Structure
         if (p.k_splits > 1)
             s.part_k = (float*)part((size_t)r.kv_heads * r.n_keys * p.k_splits *
                                     (2 * r.dim + 3) * 4);
-        s.row = (float*)part(rows * 8);
+        s.row = (float*)part(rows * 4);
         if (r.grad_positions || r.grad_query_positions) {
             s.push_q = (float*)part(rows * 12);
             s.push_k = (float*)part((size_t)r.kv_heads * r.n_keys * 12);
