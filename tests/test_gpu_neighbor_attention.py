@@ -298,3 +298,23 @@ def test_in_a_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, call(dict(c, **{n: other[n] for n in fixed})))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("heads,kv_heads,dim", [(1, 1, 8), (4, 4, 16), (4, 1, 32), (2, 1, 128)])
+def test_first_pairs_far_below_the_rest(dtype, heads, kv_heads, dim):
+    # the first 20 pairs of a row score below -200, where exp has nothing left
+    i, j = random_list(30, 30, 40, seed=14)
+    c = make(i, j, 30, 30, heads, kv_heads, dim, dtype, seed=4)
+    with torch.no_grad():
+        c["slopes"].fill_(1.0)
+        first = torch.searchsorted(c["i"], torch.arange(30, device=DEV))
+        place = torch.arange(len(i), device=DEV) - first[c["i"]]
+        c["d"] += torch.where(place < 20, 250.0, 0.0)
+    out = call(c)
+    ref, leaves = expected(c)
+    assert_near(out, ref, "out")
+    grads = torch.autograd.grad(out, [c[n] for n in LEAVES], c["upstream"])
+    refs = torch.autograd.grad(ref, leaves, c["upstream"].double().cpu())
+    for name, a, e in list(zip(LEAVES, grads, refs))[:4]:
+        assert_near(a, e, f"gradient of {name}")

@@ -10,7 +10,8 @@ from __future__ import annotations
 import pytest
 import torch
 
-from tests._operators import HALF_SPACING, assert_near, attend, distances, double, pointer, structure_pairs
+from tests._operators import (HALF_SPACING, assert_near, attend, distances, double, pointer,
+                              structure_pairs, tolerance)
 from tonari_amd.attention import structure_attention
 
 pytestmark = pytest.mark.gpu
@@ -401,3 +402,39 @@ def test_in_a_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, call(dict(c, **{n: other[n] for n in ("q", "k", "v")})))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("where", [40, 70, 250])
+def test_lone_atom_of_a_later_tile(dtype, where):
+    # every key of the first tiles scores far below what exp holds; the atom's own key comes later
+    c = make([256], 2, 1, 32, dtype, seed=25)
+    with torch.no_grad():
+        c["positions"][where] += 300.0
+        c["slopes"].copy_(torch.tensor([0.5, 2.0]))
+    check(c)
+
+
+def check_scores(c, score):
+    """check() where the scores that carry weight go up to `score`: 32 bits hold these to 2^-24 of it,
+    so that the tolerance of scores up to 2^6 grows with it."""
+    out = call(c)
+    ref, leaves = expected(c)
+    given = [n for n in LEAVES if c[n] is not None]
+    grads = torch.autograd.grad(out, [c[n] for n in given], c["upstream"])
+    refs = torch.autograd.grad(ref, leaves, c["upstream"].double().cpu())
+    for name, a, e in zip(["out", *given], (out, *grads), (ref, *refs)):
+        a, most = a.detach().double().cpu(), max(tolerance(a.dtype), 2e-5 * score / 64)
+        assert bool(((a - e).abs() <= most * e.abs().max()).all()), name
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_far_keys_before_near_ones(dtype):
+    # an ordered slab, split over workgroups: whole splits lie hundreds of lengths away, and the
+    # nearest key of the last query 1,100
+    c = make([5000], 2, 2, 16, dtype, queries=[3], seed=26)
+    with torch.no_grad():
+        c["positions"][:, 0] = torch.linspace(-900.0, 900.0, 5000, device=DEV)
+        c["query_positions"][:, 0] = torch.tensor([890.0, 0.0, -2000.0], device=DEV)
+        c["slopes"].fill_(1.0)
+    check_scores(c, 1100.0)

@@ -423,7 +423,8 @@ __global__ __launch_bounds__(256, kHeld) void k_neighbor_forward(const NeighborA
                 for (int g = 0; g < GH; ++g) {
                     const bool first = top[g] == -inf_of();
                     const bool move = first ? high[g] > -inf_of() : high[g] > 0.f;
-                    const float up = move ? high[g] : 0.f, fade = exp2_of(-up);
+                    // (the first maximum has no sums to fade, and may lie far below 0)
+                    const float up = move ? high[g] : 0.f, fade = exp2_of(fminf(-up, 0.f));
                     if (move) top[g] = (first ? 0.f : top[g]) + high[g];
                     sum[g] *= fade;
 #pragma unroll

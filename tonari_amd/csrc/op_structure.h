@@ -660,7 +660,8 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP)) void k_structure_forw
         const bool anew = high > 8.f + kLift || (top == -inf_of() && high > -inf_of());
         if (__builtin_amdgcn_ballot_w64(anew) != 0) {
             const float up = anew ? high - kLift : 0.f;
-            const float fade = exp2_of(-up);
+            // (the first maximum has no sums to fade, and may lie far below 0)
+            const float fade = exp2_of(fminf(-up, 0.f));
             top = anew ? ref + up : top;
             sum *= fade;
 #pragma unroll
