@@ -438,3 +438,13 @@ def test_far_keys_before_near_ones(dtype):
         c["query_positions"][:, 0] = torch.tensor([890.0, 0.0, -2000.0], device=DEV)
         c["slopes"].fill_(1.0)
     check_scores(c, 1100.0)
+
+
+def test_scores_far_below_zero():
+    # q.k of -8 8 32 / sqrt(32)
+    c = make([150], 2, 2, 32, torch.float32, seed=27)
+    g = torch.Generator().manual_seed(3)
+    with torch.no_grad():
+        c["q"].fill_(8.0)
+        c["k"].copy_(-8.0 + 0.05 * torch.randn(c["k"].shape, generator=g))
+    check_scores(c, 362.0)

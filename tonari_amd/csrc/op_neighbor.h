@@ -235,14 +235,15 @@ __device__ __forceinline__ float slot_sum(float x, int slot) {
     return x;
 }
 
-// u log2(e) + shift of N products, and what their gradients are multiplied by.
+// u log2(e) of N products, and what their gradients are multiplied by.  (As in
+// structure attention nothing is subtracted before a score is whole.)
 template <bool CAP, int N>
-__device__ __forceinline__ void capped_few(float (&u)[N], const ScoreRule& rule, float shift,
+__device__ __forceinline__ void capped_few(float (&u)[N], const ScoreRule& rule,
                                            float (&bend)[N]) {
     if (!CAP) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            u[i] = fmaf(u[i], rule.scale2, shift);
+            u[i] *= rule.scale2;
             bend[i] = 1.f;
         }
         return;
@@ -266,7 +267,7 @@ __device__ __forceinline__ void capped_few(float (&u)[N], const ScoreRule& rule,
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         bend[i] = fmaf(-u[i], u[i], 1.f);
-        u[i] = fmaf(u[i], rule.cap2, shift);
+        u[i] *= rule.cap2;
     }
 }
 
@@ -407,11 +408,11 @@ __global__ __launch_bounds__(256, kHeld) void k_neighbor_forward(const NeighborA
 #pragma unroll
                 for (int u = 0; u < kAhead; ++u) s[g][u] = head_sum<LPH>(q[g].dot(kx[u], 0.f));
                 const float ref = top[g] == -inf_of() ? 0.f : top[g];
-                capped_few<CAP>(s[g], a.rule, -ref, unused);
+                capped_few<CAP>(s[g], a.rule, unused);
                 high[g] = -inf_of();
 #pragma unroll
                 for (int u = 0; u < kAhead; ++u) {
-                    s[g][u] = fmaf(-slope2[g], d[u], s[g][u]);
+                    s[g][u] = fmaf(-slope2[g], d[u], s[g][u]) - ref;
                     if (!whole && !in[u]) s[g][u] = -inf_of();
                     high[g] = fmaxf(high[g], s[g][u]);
                 }
@@ -552,7 +553,7 @@ __global__ __launch_bounds__(256, kHeldBack) void k_neighbor_dq(const NeighborAr
                     s[g] = head_sum<LPH>(q[g].dot(kx[u], 0.f));
                     dp[g] = head_sum<LPH>(go[g].dot(vx[u], 0.f));
                 }
-                capped_few<CAP>(s, a.rule, 0.f, bend);
+                capped_few<CAP>(s, a.rule, bend);
 #pragma unroll
                 for (int g = 0; g < GH; ++g) {
                     s[g] = fmaf(-slope[g] * kLog2e, d[u], s[g]);
@@ -667,7 +668,7 @@ __global__ __launch_bounds__(256, kHeldBack) void k_neighbor_dkv(const NeighborA
                             s[g] = head_sum<LPH>(qx[u][g].dot(k, 0.f));
                             dp[g] = head_sum<LPH>(ox[u][g].dot(v, 0.f));
                         }
-                        capped_few<CAP>(s, a.rule, 0.f, bend);
+                        capped_few<CAP>(s, a.rule, bend);
 #pragma unroll
                         for (int g = 0; g < GH; ++g) {
                             float p = exp2_of(fmaf(-slope2[g], d[u], s[g]) - st[u][g].x);

@@ -478,14 +478,16 @@ __device__ __forceinline__ bool all_near(const f32x16& dot, const ScoreRule& rul
     for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(dot[i]));
     return __builtin_amdgcn_ballot_w64(!(top * fabsf(rule.inv) <= kTanhNear)) == 0;
 }
-// u log2(e) + shift of the products of run `run`, and what their gradients are
-// multiplied by.
+// u log2(e) of the products of run `run`, and what their gradients are multiplied
+// by.  (What is subtracted from a score comes after the score is whole, in every pass:
+// its rounding is then the same bits in all of them, and delta is the mean of dp
+// under the weights that the backward finds.)
 template <bool CAP>
 __device__ __forceinline__ void capped(const f32x16& dot, int run, const ScoreRule& rule, bool near,
-                                       float shift, float (&u)[4], float (&bend)[4]) {
+                                       float (&u)[4], float (&bend)[4]) {
     if (!CAP) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) u[e] = fmaf(dot[4 * run + e], rule.scale2, shift);
+        for (int e = 0; e < 4; ++e) u[e] = dot[4 * run + e] * rule.scale2;
         return;
     }
     // (the empty asm keeps this a branch of the wave: one side only is computed)
@@ -501,7 +503,7 @@ __device__ __forceinline__ void capped(const f32x16& dot, int run, const ScoreRu
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         bend[e] = fmaf(-u[e], u[e], 1.f);
-        u[e] = fmaf(u[e], rule.cap2, shift);
+        u[e] *= rule.cap2;
     }
 }
 
@@ -639,12 +641,12 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP)) void k_structure_forw
                                 y = four_of(x_k.x[1] + first, run, half),
                                 z = four_of(x_k.x[2] + first, run, half);
             float u[4];
-            capped<CAP>(dot, run, a.rule, near, -ref, u, unused);
+            capped<CAP>(dot, run, a.rule, near, u, unused);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const float dx = xq - x[e], dy = yq - y[e], dz = zq - z[e];
                 const float r = __builtin_amdgcn_sqrtf(fmaf(dx, dx, fmaf(dy, dy, dz * dz)));
-                s[4 * run + e] = fmaf(-slope2, r, u[e]);
+                s[4 * run + e] = fmaf(-slope2, r, u[e]) - ref;
             }
             if (left < kTile) {
                 asm volatile("");  // a branch: only a structure's last tile pays for the selects

@@ -194,7 +194,7 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP <= 32 ? 64 : 2 * DP)) v
                                 y = four_of(x_k.x[1] + first, run, half),
                                 z = four_of(x_k.x[2] + first, run, half);
             float dx[4], dy[4], dz[4], r[4], s[4], u[4], bend[4];
-            capped<CAP>(dot, run, a.rule, near, -lse, u, bend);
+            capped<CAP>(dot, run, a.rule, near, u, bend);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 dx[e] = xq - x[e];
@@ -202,7 +202,7 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP <= 32 ? 64 : 2 * DP)) v
                 dz[e] = zq - z[e];
                 r[e] = __builtin_amdgcn_sqrtf(
                     fmaf(dx[e], dx[e], fmaf(dy[e], dy[e], dz[e] * dz[e])));
-                s[e] = exp2_of(fmaf(-slope2, r[e], u[e]));
+                s[e] = exp2_of(fmaf(-slope2, r[e], u[e]) - lse);
             }
             if (left < kTile) {
                 asm volatile("");  // a branch: only a structure's last tile pays for the selects
@@ -392,6 +392,7 @@ k_structure_dkv(const StructureArgs a) {
             for (int c = 0; c < 3; ++c) xs[c] = a.x_q[3 * query + c];
             ss[0] = in ? a.lse[at] : inf_of();  // no weight beyond the rows
             if (ss[0] == -inf_of()) ss[0] = inf_of();
+            ss[0] -= kLift;
             ss[1] = a.row[at];
         }
     };
@@ -412,7 +413,7 @@ k_structure_dkv(const StructureArgs a) {
                                 lse = four_of(stat[0] + first, run, half),
                                 delta = four_of(stat[1] + first, run, half);
             float u[4], bend[4];
-            capped<CAP>(dot, run, a.rule, near, kLift, u, bend);
+            capped<CAP>(dot, run, a.rule, near, u, bend);
             float ex[4], ey[4], ez[4], r[4], ds[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
