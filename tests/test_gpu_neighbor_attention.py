@@ -318,3 +318,14 @@ def test_first_pairs_far_below_the_rest(dtype, heads, kv_heads, dim):
     refs = torch.autograd.grad(ref, leaves, c["upstream"].double().cpu())
     for name, a, e in list(zip(LEAVES, grads, refs))[:4]:
         assert_near(a, e, f"gradient of {name}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("heads,kv_heads,dim", [(1, 1, 8), (1, 1, 16), (2, 2, 8), (2, 1, 8),
+                                                (4, 1, 8)])
+@pytest.mark.parametrize("pairs", [64, 65, 90, 128, 150, 300])
+def test_long_rows_of_narrow_heads(dtype, heads, kv_heads, dim, pairs):
+    # a pair takes a lane or two, so that a wave takes all 64 pairs of a chunk in a step or less
+    i = torch.arange(3).repeat_interleave(torch.tensor([pairs, 0, pairs + 1]))
+    j = torch.randint(0, 40, (len(i),), generator=torch.Generator().manual_seed(pairs))
+    check(make(i, j, 3, 40, heads, kv_heads, dim, dtype, seed=3), 4.0)

@@ -382,14 +382,16 @@ __global__ __launch_bounds__(256, kHeld) void k_neighbor_forward(const NeighborA
         // 64 pairs ahead.  A pair beyond the run's end repeats its last one, with
         // weight 0.
         PairChunk chunk(a, run);
-        const auto step = [&](int p0, auto whole) {
+        // `n` of the chunk's 64 places hold pairs; a step reaches beyond them, and
+        // beyond 64 where a slot is a lane or two
+        const auto step = [&](int p0, int n, auto whole) {
             Raw<T, R> kx[kAhead], vx[kAhead];
             float d[kAhead];
             bool in[kAhead];
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
                 const int p = p0 + u * l.slots + l.slot;
-                in[u] = whole || p < chunk.left;
+                in[u] = whole || p < n;
                 const int j = __shfl(chunk.target, p);
                 d[u] = __shfl(chunk.distance, p);
                 kx[u] = Raw<T, R>::at(row_at<T>(k, j, k_row));
@@ -446,8 +448,8 @@ __global__ __launch_bounds__(256, kHeld) void k_neighbor_forward(const NeighborA
         for (; chunk.left > 0; chunk.next(a, run)) {
             const int n = min(chunk.left, kWave), stride = l.slots * kAhead;
             int p0 = 0;
-            for (; p0 + stride <= n; p0 += stride) step(p0, std::true_type{});
-            if (p0 < n) step(p0, std::false_type{});
+            for (; p0 + stride <= n; p0 += stride) step(p0, n, std::true_type{});
+            if (p0 < n) step(p0, n, std::false_type{});
         }
         // the slots' sums, in the largest maximum's terms
 #pragma unroll
@@ -530,7 +532,7 @@ __global__ __launch_bounds__(256, kHeldBack) void k_neighbor_dq(const NeighborAr
         // The sum of ds over a row is 0, so the slope's gradient may count
         // distances from any one of them: what they share cancels exactly.
         const float near = __shfl(chunk.distance, 0);
-        const auto step = [&](int p0, auto whole) {
+        const auto step = [&](int p0, int n, auto whole) {
             Raw<T, R> kx[kAhead], vx[kAhead];
             float d[kAhead];
 #pragma unroll
@@ -544,7 +546,7 @@ __global__ __launch_bounds__(256, kHeldBack) void k_neighbor_dq(const NeighborAr
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
                 const int p = p0 + u * l.slots + l.slot;
-                const bool in = whole || p < chunk.left;
+                const bool in = whole || p < n;
                 const int e = chunk.first + p;
                 if (!whole && !in) kx[u] = Raw<T, R>{};
                 float push = 0.f, s[GH], dp[GH], bend[GH];
@@ -571,8 +573,8 @@ __global__ __launch_bounds__(256, kHeldBack) void k_neighbor_dq(const NeighborAr
         for (; chunk.left > 0; chunk.next(a, run)) {
             const int n = min(chunk.left, kWave), stride = l.slots * kAhead;
             int p0 = 0;
-            for (; p0 + stride <= n; p0 += stride) step(p0, std::true_type{});
-            if (p0 < n) step(p0, std::false_type{});
+            for (; p0 + stride <= n; p0 += stride) step(p0, n, std::true_type{});
+            if (p0 < n) step(p0, n, std::false_type{});
         }
 #pragma unroll
         for (int g = 0; g < GH; ++g) {
