@@ -329,3 +329,17 @@ def test_long_rows_of_narrow_heads(dtype, heads, kv_heads, dim, pairs):
     i = torch.arange(3).repeat_interleave(torch.tensor([pairs, 0, pairs + 1]))
     j = torch.randint(0, 40, (len(i),), generator=torch.Generator().manual_seed(pairs))
     check(make(i, j, 3, 40, heads, kv_heads, dim, dtype, seed=3), 4.0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("heads,kv_heads,dim", [(1, 1, 8), (4, 4, 16), (4, 1, 32), (2, 1, 128)])
+def test_slopes_of_rows_whose_first_pairs_are_far(dtype, heads, kv_heads, dim):
+    # distances near 250, which weigh nothing, before those that carry the row
+    i, j = random_list(30, 30, 40, seed=14)
+    c = make(i, j, 30, 30, heads, kv_heads, dim, dtype, seed=4)
+    with torch.no_grad():
+        c["slopes"].fill_(1.0)
+        first = torch.searchsorted(c["i"], torch.arange(30, device=DEV))
+        place = torch.arange(len(i), device=DEV) - first[c["i"]]
+        c["d"] += torch.where(place < 20, 250.0, 0.0)
+    check(c)

@@ -500,11 +500,11 @@ __global__ __launch_bounds__(256, kHeldBack) void k_neighbor_dq(const NeighborAr
         const Lane<T, LPH, GH, R> l(a, first);
         const int64_t row = i * a.heads + l.head;
         Raw<T, R> q[GH], go[GH];
-        float acc[GH][VEC], delta[GH], turn[GH], lse[GH], slope[GH];
+        float acc[GH][VEC], delta[GH], turn[GH], over[GH], mean[GH], lse[GH], slope[GH];
 #pragma unroll
         for (int g = 0; g < GH; ++g) {
             q[g] = go[g] = Raw<T, R>{};
-            delta[g] = turn[g] = slope[g] = 0.f;
+            delta[g] = turn[g] = over[g] = mean[g] = slope[g] = 0.f;
             lse[g] = inf_of();
             if (l.mine) {
                 const int64_t at = (row + g) * a.dim + l.c;
@@ -529,9 +529,8 @@ __global__ __launch_bounds__(256, kHeldBack) void k_neighbor_dq(const NeighborAr
         const char* k = (const char*)((const T*)a.k + l.kv * a.k_stride[1] + l.c);
         const char* v = (const char*)((const T*)a.v + l.kv * a.v_stride[1] + l.c);
         PairChunk chunk(a, run);
-        // The sum of ds over a row is 0, so the slope's gradient may count
-        // distances from any one of them: what they share cancels exactly.
-        const float near = __shfl(chunk.distance, 0);
+        // The slope's gradient is sum ds d, where ds sums to 0: what rounding leaves of
+        // that sum, `over`, is taken out times the mean distance.
         const auto step = [&](int p0, int n, auto whole) {
             Raw<T, R> kx[kAhead], vx[kAhead];
             float d[kAhead];
@@ -559,10 +558,12 @@ __global__ __launch_bounds__(256, kHeldBack) void k_neighbor_dq(const NeighborAr
 #pragma unroll
                 for (int g = 0; g < GH; ++g) {
                     s[g] = fmaf(-slope[g] * kLog2e, d[u], s[g]);
-                    float ds = exp2_of(s[g] - lse[g]) * (dp[g] - delta[g]);
-                    if (!l.there || (!whole && !in)) ds = 0.f;
+                    float w = exp2_of(s[g] - lse[g]), ds = w * (dp[g] - delta[g]);
+                    if (!l.there || (!whole && !in)) w = ds = 0.f;
                     kx[u].add(CAP ? ds * bend[g] : ds, acc[g]);
-                    turn[g] = fmaf(-ds, d[u] - near, turn[g]);
+                    turn[g] = fmaf(-ds, d[u], turn[g]);
+                    over[g] += ds;
+                    mean[g] = fmaf(w, d[u], mean[g]);
                     push = fmaf(-slope[g], ds, push);
                 }
                 push = slot_sum<LPH>(push, a.slot);
@@ -579,12 +580,16 @@ __global__ __launch_bounds__(256, kHeldBack) void k_neighbor_dq(const NeighborAr
 #pragma unroll
         for (int g = 0; g < GH; ++g) {
             turn[g] = join_lanes<sum_of>(turn[g], a.slot);
+            over[g] = join_lanes<sum_of>(over[g], a.slot);
+            mean[g] = join_lanes<sum_of>(mean[g], a.slot);
 #pragma unroll
             for (int x = 0; x < VEC; ++x)
                 acc[g][x] = join_lanes<sum_of>(acc[g][x], a.slot) * a.rule.scale;
             if (l.mine && l.slot == 0) {
                 store_wide<T, VEC>((T*)a.grad_q + (row + g) * a.dim + l.c, acc[g]);
-                if (l.c == 0) a.turn[(int64_t)(l.head + g) * a.n_sources + i] = turn[g];
+                if (l.c == 0)
+                    a.turn[(int64_t)(l.head + g) * a.n_sources + i] =
+                        fmaf(over[g], mean[g], turn[g]);
             }
         }
     }
