@@ -448,3 +448,13 @@ def test_scores_far_below_zero():
         c["q"].fill_(8.0)
         c["k"].copy_(-8.0 + 0.05 * torch.randn(c["k"].shape, generator=g))
     check_scores(c, 362.0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 4, 16), (4, 1, 32), (2, 1, 128)])
+def test_slopes_where_the_middle_atom_is_far(dtype, heads, kv_heads, dim):
+    c = make([200], heads, kv_heads, dim, dtype, seed=31)
+    with torch.no_grad():
+        c["positions"][100] += 300.0
+        c["slopes"].fill_(1.0)
+    check(c)

@@ -33,7 +33,7 @@ namespace tnr {
 namespace op {
 
 // Sums of a query row besides grad_q: e, sum (ds u, p u) for the unit vectors
-// u, sum (ds (r - r'), p (r - r')) for one r' of the row.
+// u, sum (ds r, p r).
 constexpr int kRowSums = 9;
 
 __device__ __forceinline__ float power_of(int e) { return __builtin_amdgcn_ldexpf(1.f, e); }
@@ -139,15 +139,6 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP <= 32 ? 64 : 2 * DP)) v
     const T* vb = (const T*)a.v + (int64_t)t.k_lo * a.v_stride[0] + kv * a.v_stride[1];
     const float* xb = a.x_k + 3 * (int64_t)t.k_lo;
 
-    // distances in the slope's sums count from that of one key: what they share
-    // cancels (sum ds = 0), exactly
-    float r_mid = 0.f;
-    if (valid && t.n_k > 0) {
-        const float* p = xb + 3 * (int64_t)(t.n_k / 2);
-        const float ex = xq - p[0], ey = yq - p[1], ez = zq - p[2];
-        r_mid = __builtin_amdgcn_sqrtf(fmaf(ex, ex, fmaf(ey, ey, ez * ez)));
-    }
-
     const int tiles = (t.n_k + kTile - 1) / kTile;
     const int each = (tiles + a.splits - 1) / a.splits;
     const int from = min(tiles, split * each), to = min(tiles, from + each);
@@ -236,8 +227,8 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP <= 32 ? 64 : 2 * DP)) v
                     tw[4] = fmaf(wp, dx[e], tw[4]);
                     tw[5] = fmaf(wp, dy[e], tw[5]);
                     tw[6] = fmaf(wp, dz[e], tw[6]);
-                    tw[7] = fmaf(ds[e], r[e] - r_mid, tw[7]);
-                    tw[8] = fmaf(s[e], r[e] - r_mid, tw[8]);
+                    tw[7] = fmaf(ds[e], r[e], tw[7]);
+                    tw[8] = fmaf(s[e], r[e], tw[8]);
                 }
             }
             __builtin_amdgcn_sched_barrier(kLoadsPass);
