@@ -84,7 +84,7 @@ typedef struct tnr_structure_attention {
     const void* v;
     int64_t q_stride[2], k_stride[2], v_stride[2];  /* atom, head */
     const float* query_positions;   /* [n_queries][3]; NULL: the queries are the keys' atoms, at
-                                       positions (n_queries == n_keys) */
+                                       positions (n_queries == n_keys), or there are none */
     const float* positions;         /* [n_keys][3] */
     const float* slopes;            /* [heads] */
     float scale, softcap;

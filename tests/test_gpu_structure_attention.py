@@ -458,3 +458,13 @@ def test_slopes_where_the_middle_atom_is_far(dtype, heads, kv_heads, dim):
         c["positions"][100] += 300.0
         c["slopes"].fill_(1.0)
     check(c)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_no_queries_at_all(dtype):
+    # keys that nobody asks: an empty output, and gradients of 0
+    c = make([5, 40, 0], 4, 2, 16, dtype, queries=[0, 0, 0], seed=32)
+    out = call(c)
+    assert out.shape == (0, 4, 16)
+    for t in torch.autograd.grad(out, [c[n] for n in LEAVES], c["upstream"]):
+        assert bool((t == 0).all())

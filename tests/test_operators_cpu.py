@@ -260,3 +260,9 @@ def test_structure_backward_needs_the_wide_output(lib):  # noqa: F811
     assert code == ext.TNR_INPUT_ERROR and "pointers are null" in said
     code, said = refused(lib.tnr_structure_backward, structure(out32=PTR + 4), PTR, need)
     assert code == ext.TNR_INPUT_ERROR and "aligned" in said
+
+
+def test_no_queries_need_no_positions(lib):  # noqa: F811
+    # (the workspace is refused, which comes after the sizes)
+    code, said = refused(lib.tnr_structure_backward, structure(n_queries=0), None, 0)
+    assert code == ext.TNR_INPUT_ERROR and "workspace" in said

@@ -61,7 +61,7 @@ int check_structure(const tnr_structure_attention* r, bool backward, char* err, 
     if (r->n_structures < 0 || r->n_queries < 0 || r->n_keys < 0 ||
         (r->n_structures == 0 && (r->n_queries > 0 || r->n_keys > 0)))
         return refuse(err, len, "invalid sizes");
-    if (!r->query_positions && r->n_queries != r->n_keys)
+    if (!r->query_positions && r->n_queries > 0 && r->n_queries != r->n_keys)
         return refuse(err, len, "queries of their own need positions of their own");
     if (r->n_queries >= INT32_MAX / r->heads || r->n_keys >= INT32_MAX / r->kv_heads ||
         r->n_queries >= kMostAtoms || r->n_keys >= kMostAtoms || r->n_structures >= kMostAtoms)
@@ -232,7 +232,8 @@ int tnr_structure_forward(const tnr_structure_attention* req, void* workspace,
     StructureArgs a = structure_args(r, p);
     a.part = s.part;
     a.splits = p.f_splits;
-    lay_tiles(r, p, a, r.lse != nullptr, st);
+    // (no queries have no log-sums, and their backward reads the keys' tiles all the same)
+    lay_tiles(r, p, a, r.lse != nullptr || r.n_queries == 0, st);
     if (r.n_queries == 0) return launched(err, err_len);
     with_type(r.dtype, [&](auto t) {
         using T = decltype(t);
@@ -305,7 +306,7 @@ int tnr_structure_backward(const tnr_structure_attention* req, void* workspace,
                        st>>>(a);
         });
     });
-    const int shared = !r.query_positions;
+    const int shared = !r.query_positions && r.n_queries > 0;
     const int64_t items = (r.grad_positions ? 3 * r.n_keys : 0) +
                           (r.grad_query_positions ? 3 * r.n_queries : 0);
     const int64_t blocks = (items + 1023) / 1024 + (r.grad_slopes ? r.heads : 0);
