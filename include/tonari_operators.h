@@ -11,8 +11,8 @@
  * TNR_OK, TNR_INPUT_ERROR and TNR_DEVICE_ERROR with a message in `err`.
  *
  * What only the device can see (a species outside the table, a batch_ptr
- * that does not rise from 0 to the number of atoms, a list that is not sorted
- * or names atoms that do not exist) is not refused, since a call does not
+ * that does not rise from 0 to the number of atoms, a list whose sources do not
+ * lie together or that names atoms that do not exist) is not refused, since a call does not
  * wait for the device: the results that it touches are NaN, and no access
  * goes by it.
  *
@@ -116,11 +116,12 @@ int tnr_structure_backward(const tnr_structure_attention* req, void* workspace,
 /* ---------------------------------------------------- neighbor attention */
 
 /* A neighbor list laid out for neighbor attention.  `rows` holds
- * tnr_neighbor_rows_size() bytes written by tnr_neighbor_rows. */
+ * tnr_neighbor_rows_size() bytes written by tnr_neighbor_rows; rows of a list of
+ * other sizes give NaN.  The first 32-bit word is 0 for a valid list. */
 typedef struct tnr_neighbor_list {
     int64_t n_pairs;                        /* up to 2^31 - 4097 */
     int64_t n_sources, n_targets;           /* below 2^26 */
-    const int64_t* sources;                 /* i: int64[n_pairs], not falling */
+    const int64_t* sources;                 /* i: int64[n_pairs], those of an atom together */
     const int64_t* targets;                 /* j: int64[n_pairs] */
     int32_t transpose;                      /* 1: also by target, which the backward needs */
     void* rows;

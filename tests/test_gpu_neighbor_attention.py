@@ -343,3 +343,32 @@ def test_slopes_of_rows_whose_first_pairs_are_far(dtype, heads, kv_heads, dim):
         place = torch.arange(len(i), device=DEV) - first[c["i"]]
         c["d"] += torch.where(place < 20, 250.0, 0.0)
     check(c)
+
+
+def test_rows_of_another_list():
+    # a tuple altered by hand is refused by its size, or read no further than its head
+    def given(i, j, n, m):
+        c = make(i, j, n, m, 2, 1, 16, torch.float32)
+        return c, neighbor_rows(c["i"], c["j"], n, m)
+
+    def attend_along(c, rows):
+        return neighbor_attention(c["q"], c["k"], c["v"], c["d"], rows, c["slopes"])
+
+    c, rows = given(*random_list(10, 12, 4, seed=1), 10, 12)
+    plain = neighbor_rows(c["i"], c["j"], 10, 12, transpose=False)
+    with pytest.raises(ValueError, match="not those of this list"):
+        attend_along(c, plain._replace(transpose=True))
+    with pytest.raises(ValueError, match="not those of this list"):
+        attend_along(c, rows._replace(rows=rows.rows[:256]))
+    fewer = make(c["i"].cpu()[:-1], c["j"].cpu()[:-1], 10, 12, 2, 1, 16, torch.float32)
+    for other, altered in (
+            (dict(c, k=c["k"][:11], v=c["v"][:11]), rows._replace(n_targets=11)),
+            (dict(c, q=c["q"][:9], upstream=c["upstream"][:9]), rows._replace(n_sources=9)),
+            (dict(fewer), rows._replace(i=fewer["i"], j=fewer["j"]))):
+        for n in ("q", "k", "v"):
+            other[n] = other[n].detach().requires_grad_()
+        out = attend_along(other, altered)
+        assert bool(torch.isnan(out).all())
+        for t in torch.autograd.grad(out, [other[n] for n in LEAVES], other["upstream"]):
+            assert bool(torch.isnan(t).all())
+    assert bool(torch.isfinite(attend_along(c, rows)).all())

@@ -200,13 +200,15 @@ def neighbor_attention(
     _check_tensors(q=q, k=k, v=v, d=d, slopes=slopes)
     if not isinstance(rows, NeighborRows):
         raise TypeError("rows must come from neighbor_rows")
+    _check_tensors(i=rows.i, j=rows.j, rows=rows.rows)
     _check_heads(q, k, v, slopes)
     if q.shape[0] != rows.n_sources or k.shape[0] != rows.n_targets:
         raise ValueError("q needs a row for each source of the list, k and v one for each target")
-    if d.shape != rows.i.shape or d.dtype not in (torch.float32, torch.float64):
+    if rows.j.shape != rows.i.shape or d.shape != rows.i.shape or d.dtype not in (torch.float32, torch.float64):
         raise ValueError("d must be float32 or float64 with one value for each pair")
     scale, softcap = _score_rule(q, scale, softcap)
-    _check_place("neighbor_attention", q, k=k, v=v, d=d, slopes=slopes, rows=rows.rows)
+    _check_place("neighbor_attention", q, k=k, v=v, d=d, slopes=slopes, rows=rows.rows, i=rows.i,
+                 j=rows.j)
     if not rows.transpose and torch.is_grad_enabled() and any(
             t.requires_grad for t in (q, k, v, d, slopes)):
         raise ValueError("gradients need rows with transpose=True")

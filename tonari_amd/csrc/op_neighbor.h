@@ -29,9 +29,20 @@
 namespace tnr {
 namespace op {
 
+// What the rows are of.  Rows whose head does not say what a call says are not read
+// further, so that no call goes by the runs of another list.
+struct RowsHead {
+    int32_t status;  // not 0: the list is not valid (every result is NaN)
+    int32_t pairs, sources, targets;
+    __host__ __device__ bool holds(const RowsHead& o) const {
+        return status == 0 && pairs == o.pairs && sources == o.sources && targets == o.targets;
+    }
+};
+constexpr int kHeadWords = sizeof(RowsHead) / 4;
+
 // What tnr_neighbor_rows writes, in this order (each part 256-byte aligned).
 struct NeighborRows {
-    int32_t* status;   // not 0: the list is not valid (every result is NaN)
+    RowsHead* head;
     int2* sources;     // [n_sources]: pairs [x, y)
     int32_t* target;   // [n_pairs]
     int2* targets;     // [n_targets]: places [x, y) of `order`
@@ -48,7 +59,7 @@ inline NeighborRows neighbor_rows(void* base, int64_t pairs, int64_t sources, in
         return p + here;
     };
     NeighborRows r{};
-    r.status = (int32_t*)part(4);
+    r.head = (RowsHead*)part(sizeof(RowsHead));
     r.sources = (int2*)part((size_t)sources * 8);
     if (transpose) r.targets = (int2*)part((size_t)targets * 8);
     r.target = (int32_t*)part((size_t)pairs * 4);
@@ -57,7 +68,20 @@ inline NeighborRows neighbor_rows(void* base, int64_t pairs, int64_t sources, in
     return r;
 }
 
-// status and the runs are cleared before.  A source whose pairs do not lie
+// Clears `words` from the head on: the runs, but for what the head says.
+__global__ __launch_bounds__(256) void k_neighbor_clear(RowsHead* at, RowsHead head, int64_t words) {
+    const int32_t says[kHeadWords] = {head.status, head.pairs, head.sources, head.targets};
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < words;
+         i += (int64_t)gridDim.x * 256) {
+        int32_t x = 0;
+#pragma unroll
+        for (int w = 0; w < kHeadWords; ++w)
+            if (i == w) x = says[w];
+        ((int32_t*)at)[i] = x;
+    }
+}
+
+// The runs are cleared before.  A source whose pairs do not lie
 // together finds its run taken.
 constexpr int kRowsEach = 4, kRowsBlock = 256 * kRowsEach;
 __global__ __launch_bounds__(256) void k_neighbor_rows(const int64_t* sources,
@@ -98,7 +122,7 @@ __global__ __launch_bounds__(256) void k_neighbor_rows(const int64_t* sources,
             bad |= atomicExch(&r.sources[i[u]].x, (int)e + 1) != 0;  // 0: none yet
         if (e + 1 == n_pairs || after != i[u]) r.sources[i[u]].y = (int)e + 1;
     }
-    if (__builtin_amdgcn_ballot_w64(bad != 0) != 0 && lane == 0) atomicOr(r.status, 1);
+    if (__builtin_amdgcn_ballot_w64(bad != 0) != 0 && lane == 0) atomicOr(&r.head->status, 1);
 }
 
 struct PairKeys {
@@ -140,6 +164,7 @@ __device__ __forceinline__ int2 run_of(const int2* runs, int64_t i) {
 
 struct NeighborArgs {
     NeighborRows rows;
+    RowsHead head;  // what the rows have to be of
     int n_pairs, n_sources, n_targets;
     const void *q, *k, *v;
     int64_t q_stride[2], k_stride[2], v_stride[2];
@@ -361,7 +386,7 @@ __global__ __launch_bounds__(256, kHeld) void k_neighbor_forward(const NeighborA
 #pragma unroll
         for (int x = 0; x < VEC; ++x) acc[g][x] = 0.f;
     }
-    const bool valid = *a.rows.status == 0;
+    const bool valid = a.rows.head->holds(a.head);
     if (valid) {
         Raw<T, R> q[GH];
         float slope2[GH];
@@ -486,7 +511,7 @@ __global__ __launch_bounds__(256, kHeldBack) void k_neighbor_dq(const NeighborAr
     constexpr int VEC = Raw<T, R>::kVec, kAhead = GH == 4 ? 1 : GH == 2 || R == 2 ? 2 : 4;
     const int64_t i = (int64_t)xcd_order(blockIdx.x, gridDim.x) * 4 + threadIdx.x / kWave;
     if (i >= a.n_sources) return;
-    if (*a.rows.status != 0) {
+    if (!a.rows.head->holds(a.head)) {
         const int lane = lane_of();
         fill_nan((T*)a.grad_q + i * a.heads * a.dim, (int64_t)a.heads * a.dim, lane, kWave);
         fill_nan(a.grad_distances, a.n_pairs, i * kWave + lane, (int64_t)a.n_sources * kWave);
@@ -610,7 +635,7 @@ __global__ __launch_bounds__(256, kHeldBack) void k_neighbor_dkv(const NeighborA
     if (!mine) c = 0;
     const int64_t flat = (j * a.kv_heads + kv) * a.dim + c;
     float dk[VEC], dv[VEC];
-    const bool valid = *a.rows.status == 0;
+    const bool valid = a.rows.head->holds(a.head);
 #pragma unroll
     for (int x = 0; x < VEC; ++x) dk[x] = dv[x] = valid ? 0.f : nan_of();
     if (valid) {

@@ -182,6 +182,10 @@ NeighborRows rows_of(const tnr_neighbor_list& l) {
     return neighbor_rows(l.rows, l.n_pairs, l.n_sources, l.n_targets, l.transpose != 0);
 }
 
+RowsHead head_of(const tnr_neighbor_list& l) {
+    return {0, (int32_t)l.n_pairs, (int32_t)l.n_sources, (int32_t)l.n_targets};
+}
+
 int check_neighbor(const tnr_neighbor_attention* r, bool backward, char* err, size_t len) {
     if (!r) return refuse(err, len, "request is null");
     int code = check_heads(r->dtype, r->heads, r->kv_heads, r->dim, r->scale, r->softcap, err, len);
@@ -212,6 +216,7 @@ int check_neighbor(const tnr_neighbor_attention* r, bool backward, char* err, si
 NeighborArgs neighbor_args(const tnr_neighbor_attention& r) {
     NeighborArgs a{};
     a.rows = rows_of(r.list);
+    a.head = head_of(r.list);
     a.n_pairs = (int)r.list.n_pairs;
     a.n_sources = (int)r.list.n_sources;
     a.n_targets = (int)r.list.n_targets;
@@ -398,8 +403,11 @@ int tnr_neighbor_rows(const tnr_neighbor_list* list, void* workspace, size_t wor
         return refuse(err, err_len, "workspace is too small or not aligned to 256 bytes");
     const hipStream_t st = (hipStream_t)stream;
     const NeighborRows rows = rows_of(l);
-    // status and the runs, which lie at the front
-    zero(rows.status, (char*)rows.target - (char*)rows.status, st);
+    // the head and the runs, which lie at the front
+    const int64_t words = ((char*)rows.target - (char*)rows.head) / 4;
+    const int64_t blocks = (words + 1023) / 1024;
+    k_neighbor_clear<<<(unsigned)(blocks < 1024 ? blocks : 1024), 256, 0, st>>>(rows.head,
+                                                                                head_of(l), words);
     if (l.n_pairs > 0) {
         k_neighbor_rows<<<(unsigned)((l.n_pairs + kRowsBlock - 1) / kRowsBlock), 256, 0, st>>>(
             l.sources, l.targets, l.n_pairs, l.n_sources, l.n_targets, rows);

@@ -480,6 +480,10 @@ struct NeighborAttention : torch::autograd::Function<NeighborAttention> {
 Tensor neighbor_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& d,
                           const Tensor& slopes, const Tensor& rows, const Tensor& i,
                           const Tensor& j, bool transpose, double scale, double softcap) {
+    const tnr_neighbor_list l = list_of(d.numel(), q.size(0), k.size(0), transpose);
+    TORCH_CHECK_VALUE(rows.scalar_type() == at::kByte && rows.dim() == 1 && rows.is_contiguous() &&
+                          rows.numel() == (int64_t)tnr_neighbor_rows_size(&l),
+                      "rows are not those of this list");
     if (wants({q, k, v, d, slopes}))
         return NeighborAttention::apply(q, k, v, d, slopes, rows, i, j, transpose, scale, softcap);
     c10::DeviceGuard guard(q.device());
