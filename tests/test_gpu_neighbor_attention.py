@@ -372,3 +372,15 @@ def test_rows_of_another_list():
         for t in torch.autograd.grad(out, [other[n] for n in LEAVES], other["upstream"]):
             assert bool(torch.isnan(t).all())
     assert bool(torch.isfinite(attend_along(c, rows)).all())
+
+
+@pytest.mark.parametrize("i,j", [
+    ([0, 1, 0], [1, 0, 2]), ([0, 0, 3], [1, 2, 0]), ([0, -1, 1], [1, 2, 0]), ([0, 0, 1], [1, 3, 0]),
+    ([0, 0, 1], [1, -2, 0]), ([0, 0, 1], [1, 1 << 40, 0]),
+])
+def test_graphs_of_wrong_lists_are_nan(i, j):
+    c = make(torch.tensor(i), torch.tensor(j), 3, 3, 2, 2, 16, torch.float32)
+    grads = torch.autograd.grad(call(c), [c[n] for n in LEAVES], c["upstream"], create_graph=True)
+    again = torch.autograd.grad(sum(t.sum() for t in grads), [c[n] for n in LEAVES])
+    for t in (*grads, *again):
+        assert bool(torch.isnan(t).all())

@@ -468,3 +468,23 @@ def test_no_queries_at_all(dtype):
     assert out.shape == (0, 4, 16)
     for t in torch.autograd.grad(out, [c[n] for n in LEAVES], c["upstream"]):
         assert bool((t == 0).all())
+
+
+@pytest.mark.parametrize("ptr", [[0, 5, 3, 10], [1, 5, 7, 10], [0, 5, 7, 9], [0, 5, 7, 11],
+                                 [0, -5, 1 << 40, 10]])
+def test_graphs_of_wrong_pointers_are_nan(ptr):
+    c = make([10], 2, 2, 16, torch.float32)
+    c["batch_ptr"] = torch.tensor(ptr, dtype=torch.int64, device=DEV)
+    leaves = [c[n] for n in LEAVES if c[n] is not None]
+    grads = torch.autograd.grad(call(c), leaves, c["upstream"], create_graph=True)
+    again = torch.autograd.grad(sum(t.sum() for t in grads), leaves)
+    for t in (*grads, *again):
+        assert bool(torch.isnan(t).all())
+
+
+def test_graphs_without_pairs():
+    for lengths, queries in (([], None), ([0, 0], None), ([0, 3], [2, 0]), ([3], [0])):
+        c = make(lengths, 2, 1, 16, torch.float32, queries=queries, seed=33)
+        leaves = [c[n] for n in LEAVES if c[n] is not None]
+        for t in torch.autograd.grad(call(c), leaves, c["upstream"], create_graph=True):
+            assert bool((t == 0).all())

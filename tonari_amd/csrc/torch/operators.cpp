@@ -12,6 +12,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <limits>
 #include <optional>
 #include <vector>
@@ -175,6 +176,38 @@ Tensor pair_attention(const Tensor& q, const Tensor& k, const Tensor& v, const T
         .to(q.scalar_type());
 }
 
+// 1 or, where `ok` (a truth value on the device) does not hold, NaN: inputs are
+// multiplied by it, so that all that follows from them is NaN, as in the kernels.
+Tensor nan_unless(const Tensor& ok) {
+    return at::where(ok, at::ones({}, ok.options().dtype(at::kFloat)),
+                     at::full({}, std::numeric_limits<double>::quiet_NaN(),
+                              ok.options().dtype(at::kFloat)));
+}
+variable_list times(const variable_list& nodes, const Tensor& factor) {
+    variable_list all;
+    for (const Tensor& t : nodes) all.push_back(t.defined() ? t * factor : t);
+    return all;
+}
+
+// Whether pointers rise from 0 to n.
+Tensor rising(const Tensor& ptr, int64_t n) {
+    return (ptr.slice(0, 1) - ptr.slice(0, 0, -1))
+        .ge(0)
+        .all()
+        .logical_and(ptr.select(0, 0).eq(0))
+        .logical_and(ptr.select(0, -1).eq(n));
+}
+
+// Whether the rows are of a valid list of these sizes (their head says both).
+Tensor rows_hold(const Tensor& rows, int64_t pairs, int64_t sources, int64_t targets) {
+    const Tensor head = rows.slice(0, 0, 16).view(at::kInt);
+    return head.select(0, 0)
+        .eq(0)
+        .logical_and(head.select(0, 1).eq(pairs))
+        .logical_and(head.select(0, 2).eq(sources))
+        .logical_and(head.select(0, 3).eq(targets));
+}
+
 // The inputs as nodes of their own: the gradient for one of them then takes no
 // path through another (q may well depend on the positions).
 variable_list own_nodes(const variable_list& saved, size_t n) {
@@ -284,10 +317,14 @@ struct StructureAttention : torch::autograd::Function<StructureAttention> {
         std::vector<bool> needed;
         for (size_t i = 0; i < 6; ++i) needed.push_back(s[i].defined() && ctx->needs_input_grad(i));
         if (at::GradMode::is_enabled()) {
-            const variable_list n = own_nodes(s, 6);
-            const Tensor &x = n[3], &x_q = n[5], &kp = s[6], &qp = s[7].defined() ? s[7] : s[6];
-            const Tensor nq = qp.slice(0, 1) - qp.slice(0, 0, -1);
-            const Tensor nk = kp.slice(0, 1) - kp.slice(0, 0, -1);
+            const variable_list nodes = own_nodes(s, 6);
+            const Tensor &kp = s[6], &qp = s[7].defined() ? s[7] : s[6];
+            const Tensor ok = rising(kp, s[1].size(0)).logical_and(rising(qp, s[0].size(0)));
+            const variable_list n = times(nodes, nan_unless(ok));
+            const Tensor &x = n[3], &x_q = n[5];
+            // (pointers that are wrong make no pairs, so that nothing goes by them)
+            const Tensor nq = (qp.slice(0, 1) - qp.slice(0, 0, -1)) * ok;
+            const Tensor nk = (kp.slice(0, 1) - kp.slice(0, 0, -1)) * ok;
             const Tensor pairs = nq * nk;
             const Tensor b = at::repeat_interleave(pairs);
             const Tensor place = at::arange(b.numel(), b.options()) -
@@ -302,7 +339,7 @@ struct StructureAttention : torch::autograd::Function<StructureAttention> {
             const Tensor r = at::where(apart, at::where(apart, r2, one).sqrt(), one * 0);
             const Tensor out =
                 pair_attention(n[0], n[1], n[2], r, n[4], source, target, scale, softcap);
-            const variable_list found = graph_of(out, grads[0], n, needed);
+            const variable_list found = graph_of(out, grads[0], nodes, needed);
             for (size_t i = 0; i < 6; ++i) all[i] = found[i];
             return all;
         }
@@ -443,10 +480,16 @@ struct NeighborAttention : torch::autograd::Function<NeighborAttention> {
         if (at::GradMode::is_enabled()) {
             std::vector<bool> needed;
             for (size_t i = 0; i < 5; ++i) needed.push_back(ctx->needs_input_grad(i));
-            const variable_list n = own_nodes(s, 5);
-            const Tensor out =
-                pair_attention(n[0], n[1], n[2], n[3], n[4], s[6], s[7], scale, softcap);
-            const variable_list found = graph_of(out, grads[0], n, needed);
+            const variable_list nodes = own_nodes(s, 5);
+            const int64_t sources = s[0].size(0), targets = s[1].size(0);
+            const variable_list n =
+                times(nodes, nan_unless(rows_hold(s[5], s[3].numel(), sources, targets)));
+            // (a list may name atoms that do not exist)
+            const Tensor out = pair_attention(n[0], n[1], n[2], n[3], n[4],
+                                              s[6].clamp(0, std::max<int64_t>(sources - 1, 0)),
+                                              s[7].clamp(0, std::max<int64_t>(targets - 1, 0)),
+                                              scale, softcap);
+            const variable_list found = graph_of(out, grads[0], nodes, needed);
             for (size_t i = 0; i < 5; ++i) all[i] = found[i];
             return all;
         }
