@@ -384,3 +384,19 @@ def test_graphs_of_wrong_lists_are_nan(i, j):
     again = torch.autograd.grad(sum(t.sum() for t in grads), [c[n] for n in LEAVES])
     for t in (*grads, *again):
         assert bool(torch.isnan(t).all())
+
+
+def test_graph_of_pairs_that_weigh_nothing():
+    i, j = random_list(40, 40, 15, seed=2)
+    c = make(i, j, 40, 40, 2, 2, 16, torch.float32, grad=False)
+    c["slopes"] = torch.ones(2, device=DEV)
+    c["d"] = torch.where(c["i"] == c["i"][0], float("inf"), c["d"])     # a row, and a pair of another
+    c["d"][-1] = float("inf")
+    leaves = [c[n].requires_grad_() for n in ("q", "k", "v")]
+    out = call(c)
+    plain = torch.autograd.grad(out, leaves, c["upstream"], retain_graph=True)
+    graph = torch.autograd.grad(out, leaves, c["upstream"], create_graph=True)
+    for a, e in zip(graph, plain):
+        assert_near(a, e)
+    for t in torch.autograd.grad(sum((t * t).sum() for t in graph), leaves):
+        assert bool(torch.isfinite(t).all())

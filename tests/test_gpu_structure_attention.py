@@ -488,3 +488,17 @@ def test_graphs_without_pairs():
         leaves = [c[n] for n in LEAVES if c[n] is not None]
         for t in torch.autograd.grad(call(c), leaves, c["upstream"], create_graph=True):
             assert bool((t == 0).all())
+
+
+def test_graph_of_a_row_without_weight():
+    c = make([4], 2, 2, 16, torch.float32, queries=[2], grad=False)
+    c["query_positions"][1] = float("inf")
+    c["slopes"] = torch.ones(2, device=DEV)
+    leaves = [c[n].requires_grad_() for n in ("q", "k", "v")]
+    out = call(c)
+    plain = torch.autograd.grad(out, leaves, c["upstream"], retain_graph=True)
+    graph = torch.autograd.grad(out, leaves, c["upstream"], create_graph=True)
+    for a, e in zip(graph, plain):
+        assert_near(a, e)
+    for t in torch.autograd.grad(sum((t * t).sum() for t in graph), leaves):
+        assert bool(torch.isfinite(t).all())

@@ -170,7 +170,8 @@ Tensor pair_attention(const Tensor& q, const Tensor& k, const Tensor& v, const T
     top = at::where(top.isinf(), at::zeros_like(top), top);
     const Tensor e = at::exp(score - top.index_select(0, source));
     const Tensor sum = at::zeros({n, heads}, e.options()).index_add(0, source, e);
-    const Tensor p = e / sum.index_select(0, source);
+    // (a row that no key weighs in on is 0)
+    const Tensor p = e / at::where(sum.eq(0), at::ones_like(sum), sum).index_select(0, source);
     return at::zeros({n, heads, dim}, e.options())
         .index_add(0, source, p.unsqueeze(-1) * wide(v))
         .to(q.scalar_type());
