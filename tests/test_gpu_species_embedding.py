@@ -133,3 +133,29 @@ def test_gradient_of_the_gradient():
     want = 2 * 3.0 * gw.detach()[z.clamp(min=0)]
     want[4] = 0
     assert torch.allclose(gu, want, rtol=1e-5, atol=1e-5)
+
+
+def test_graph_has_the_same_bits():
+    z, w, up = make((40_000,), 119, 64, torch.bfloat16)
+    z[7], z[40] = -1, 119
+    out = species_embedding(z, w, scale=0.5)
+    (want,) = torch.autograd.grad(out, w, up, retain_graph=True)
+    up.requires_grad_()
+    for _ in range(2):
+        (got,) = torch.autograd.grad(out, w, up, create_graph=True)
+        assert torch.equal(got, want)
+    # and on: a sum of cubes of the gradient, twice in the upstream gradient
+    (first,) = torch.autograd.grad((got.float() ** 3).sum(), up, create_graph=True)
+    assert bool((first[[7, 40]] == 0).all())
+    (second,) = torch.autograd.grad(first.float().sum(), up)
+    assert bool(torch.isfinite(second).all()) and bool((second[[7, 40]] == 0).all())
+
+
+def test_graph_of_an_empty_table():
+    z, w, up = make((9,), 0, 8, torch.float32)
+    up.requires_grad_()
+    out = species_embedding(z, w)
+    assert bool(torch.isnan(out).all())
+    (got,) = torch.autograd.grad(out, w, up, create_graph=True)
+    assert got.shape == (0, 8)
+    assert bool((torch.autograd.grad(got.sum(), up)[0] == 0).all())

@@ -2,8 +2,9 @@
 // outputs and workspaces, the calls on torch's current stream, and autograd.
 // Arguments come checked from tonari_amd/embedding.py and attention.py.
 //
-// A gradient's own graph (create_graph, for training on forces) comes from
-// the operator's expression in torch operations, as for the list's d and D.
+// A gradient's own graph (create_graph, for training on forces) comes, for the
+// attentions, from the operator's expression in torch operations, as for the
+// list's d and D; the embedding's is the embedding again.
 
 #include "../../../include/tonari_operators.h"
 
@@ -105,6 +106,44 @@ Tensor embedding_forward(const Tensor& species, const Tensor& weight, double sca
     return out;
 }
 
+Tensor embedding_gradient(const Tensor& grad_out, const Tensor& species, int64_t rows,
+                          double scale) {
+    c10::DeviceGuard guard(grad_out.device());
+    const Tensor z = species.contiguous(), go = flat(grad_out);
+    const Tensor grad = at::empty({rows, go.size(-1)}, go.options());
+    tnr_embedding r = embedding_request(z, go, rows, scale);
+    r.grad_out = go.data_ptr();
+    r.grad_weight = grad.data_ptr();
+    const Tensor space = bytes_on(go, tnr_embedding_workspace_size(&r));
+    char err[kErrLen] = {0};
+    require(tnr_embedding_backward(&r, space.data_ptr(), (size_t)space.numel(), stream_of(go), err,
+                                   kErrLen),
+            err);
+    return grad;
+}
+
+Tensor species_embedding(const Tensor& species, const Tensor& weight, double scale);
+
+// The table's gradient as a function of the output's: linear, and its own gradient
+// is the embedding of the table's (0 for a species outside it).
+struct EmbeddingGradient : torch::autograd::Function<EmbeddingGradient> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& grad_out, const Tensor& species,
+                          int64_t rows, double scale) {
+        ctx->save_for_backward({species});
+        ctx->saved_data["scale"] = scale;
+        return embedding_gradient(grad_out, species, rows, scale);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        variable_list all(4);
+        const Tensor &g = grads[0], species = ctx->get_saved_variables()[0];
+        if (!g.defined()) return all;
+        const Tensor out = species_embedding(species, g, ctx->saved_data["scale"].toDouble());
+        const Tensor in = species.ge(0).logical_and(species.lt(g.size(0))).unsqueeze(-1);
+        all[0] = at::where(in, out, at::zeros({}, out.options()));
+        return all;
+    }
+};
+
 struct Embedding : torch::autograd::Function<Embedding> {
     static Tensor forward(AutogradContext* ctx, const Tensor& weight, const Tensor& species,
                           double scale) {
@@ -119,28 +158,9 @@ struct Embedding : torch::autograd::Function<Embedding> {
         const int64_t rows = ctx->saved_data["rows"].toInt();
         const Tensor& g = grads[0];
         if (!g.defined()) return {Tensor(), Tensor(), Tensor()};
-        c10::DeviceGuard guard(g.device());
-        if (at::GradMode::is_enabled() && g.requires_grad()) {
-            const Tensor z = species.reshape({-1}).to(at::kLong);
-            const Tensor in = z.ge(0).logical_and(z.lt(rows));
-            const Tensor rowed = g.reshape({z.numel(), g.size(-1)}).to(at::kFloat) * scale;
-            const Tensor masked = at::where(in.unsqueeze(1), rowed, at::zeros({}, rowed.options()));
-            const Tensor sum = at::zeros({rows, g.size(-1)}, rowed.options())
-                                   .index_add(0, at::where(in, z, at::zeros_like(z)),
-                                              rows > 0 ? masked : masked.slice(0, 0, 0));
-            return {sum.to(g.scalar_type()), Tensor(), Tensor()};
-        }
-        const Tensor z = species.contiguous(), go = flat(g);
-        const Tensor grad = at::empty({rows, go.size(-1)}, go.options());
-        tnr_embedding r = embedding_request(z, go, rows, scale);
-        r.grad_out = go.data_ptr();
-        r.grad_weight = grad.data_ptr();
-        const Tensor space = bytes_on(go, tnr_embedding_workspace_size(&r));
-        char err[kErrLen] = {0};
-        require(tnr_embedding_backward(&r, space.data_ptr(), (size_t)space.numel(), stream_of(go),
-                                       err, kErrLen),
-                err);
-        return {grad, Tensor(), Tensor()};
+        return {wants({g}) ? EmbeddingGradient::apply(g, species, rows, scale)
+                           : embedding_gradient(g, species, rows, scale),
+                Tensor(), Tensor()};
     }
 };
 
