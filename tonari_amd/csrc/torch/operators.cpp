@@ -11,6 +11,7 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <algorithm>
@@ -65,7 +66,18 @@ Tensor flat(const Tensor& x) {
                : t.clone(at::MemoryFormat::Contiguous);
 }
 
+// What these calls would lose without a word: tangents of forward-mode
+// derivatives, and themselves in a trace (which would record outputs that nothing fills).
+void refuse_untracked(std::initializer_list<Tensor> inputs) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing(),
+                                "the operators cannot be traced (torch.jit.trace)");
+    for (const Tensor& t : inputs)
+        TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(),
+                                    "the operators have no forward-mode derivatives");
+}
+
 bool wants(std::initializer_list<Tensor> inputs) {
+    refuse_untracked(inputs);
     if (!at::GradMode::is_enabled()) return false;
     for (const Tensor& t : inputs)
         if (t.defined() && t.requires_grad()) return true;
@@ -158,6 +170,7 @@ struct Embedding : torch::autograd::Function<Embedding> {
         const int64_t rows = ctx->saved_data["rows"].toInt();
         const Tensor& g = grads[0];
         if (!g.defined()) return {Tensor(), Tensor(), Tensor()};
+        // (wants refuses a tangent of g)
         return {wants({g}) ? EmbeddingGradient::apply(g, species, rows, scale)
                            : embedding_gradient(g, species, rows, scale),
                 Tensor(), Tensor()};
@@ -334,6 +347,7 @@ struct StructureAttention : torch::autograd::Function<StructureAttention> {
         const double softcap = ctx->saved_data["softcap"].toDouble();
         variable_list all(10);
         if (!grads[0].defined()) return all;
+        refuse_untracked({grads[0]});
         c10::DeviceGuard guard(s[0].device());
         std::vector<bool> needed;
         for (size_t i = 0; i < 6; ++i) needed.push_back(s[i].defined() && ctx->needs_input_grad(i));
@@ -424,6 +438,7 @@ tnr_neighbor_list list_of(int64_t pairs, int64_t sources, int64_t targets, bool 
 
 Tensor neighbor_rows(const Tensor& i, const Tensor& j, int64_t n_sources, int64_t n_targets,
                      bool transpose) {
+    refuse_untracked({});
     c10::DeviceGuard guard(i.device());
     const Tensor sources = i.contiguous(), targets = j.contiguous();
     tnr_neighbor_list l = list_of(i.numel(), n_sources, n_targets, transpose);
@@ -497,6 +512,7 @@ struct NeighborAttention : torch::autograd::Function<NeighborAttention> {
         const double softcap = ctx->saved_data["softcap"].toDouble();
         variable_list all(11);
         if (!grads[0].defined()) return all;
+        refuse_untracked({grads[0]});
         c10::DeviceGuard guard(s[0].device());
         if (at::GradMode::is_enabled()) {
             std::vector<bool> needed;
