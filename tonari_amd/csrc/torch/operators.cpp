@@ -416,11 +416,11 @@ Tensor structure_attention(const Tensor& q, const Tensor& k, const Tensor& v, co
                            const Tensor& batch_ptr, const Tensor& slopes,
                            const std::optional<Tensor>& query_positions,
                            const std::optional<Tensor>& query_ptr, double scale, double softcap) {
+    c10::DeviceGuard guard(q.device());  // (for both paths: launches go to the current device)
     const Tensor x_q = query_positions.value_or(Tensor()), q_ptr = query_ptr.value_or(Tensor());
     if (wants({q, k, v, x, slopes, x_q}))
         return StructureAttention::apply(q, k, v, x, slopes, query_positions, batch_ptr, query_ptr,
                                          scale, softcap);
-    c10::DeviceGuard guard(q.device());
     StructureCall c(q, k, v, x, slopes, x_q, batch_ptr, q_ptr, scale, softcap);
     return structure_forward(c, nullptr, nullptr);
 }
@@ -560,13 +560,13 @@ struct NeighborAttention : torch::autograd::Function<NeighborAttention> {
 Tensor neighbor_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& d,
                           const Tensor& slopes, const Tensor& rows, const Tensor& i,
                           const Tensor& j, bool transpose, double scale, double softcap) {
+    c10::DeviceGuard guard(q.device());
     const tnr_neighbor_list l = list_of(d.numel(), q.size(0), k.size(0), transpose);
     TORCH_CHECK_VALUE(rows.scalar_type() == at::kByte && rows.dim() == 1 && rows.is_contiguous() &&
                           rows.numel() == (int64_t)tnr_neighbor_rows_size(&l),
                       "rows are not those of this list");
     if (wants({q, k, v, d, slopes}))
         return NeighborAttention::apply(q, k, v, d, slopes, rows, i, j, transpose, scale, softcap);
-    c10::DeviceGuard guard(q.device());
     NeighborCall c(q, k, v, d, slopes, rows, transpose, scale, softcap);
     const Tensor out = at::empty(c.q.sizes(), c.q.options());
     c.r.out = out.data_ptr();
