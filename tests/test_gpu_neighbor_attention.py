@@ -400,3 +400,16 @@ def test_graph_of_pairs_that_weigh_nothing():
         assert_near(a, e)
     for t in torch.autograd.grad(sum((t * t).sum() for t in graph), leaves):
         assert bool(torch.isfinite(t).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("heads,kv_heads,dim", [(2, 2, 16), (2, 2, 24), (3, 1, 40), (4, 1, 48)])
+def test_keys_at_minus_infinity(dtype, heads, kv_heads, dim):
+    # keys that are masked by a channel of -inf leave their pairs without weight, also where a
+    # head's channels do not fill its lanes
+    i, j = random_list(30, 30, 12, seed=15)
+    c = make(i, j, 30, 30, heads, kv_heads, dim, dtype, seed=5, grad=False)
+    c["q"] = c["q"].abs() + 0.1
+    c["k"][7, :, 0] = c["k"][11, :, dim - 1] = float("-inf")
+    keep = (c["j"] != 7) & (c["j"] != 11)
+    assert_near(call(c), call(dict(c, i=c["i"][keep], j=c["j"][keep], d=c["d"][keep])))

@@ -314,8 +314,8 @@ __device__ __forceinline__ void load_wide(const float* p, float (&x)[N]) {
 
 // What a lane of a wave takes: R times 16 bytes of a key head's channels, for GH
 // query heads that share it (`head` is the first).  A slot holds `block` such units.
-// Lanes whose head or channels do not exist read those of others and add
-// nothing.
+// Lanes whose head or channels do not exist read those of others, which may be
+// infinite, and add nothing: their products are left out, not multiplied by 0.
 template <typename T, int LPH, int GH, int R>
 struct Lane {
     static constexpr int VEC = Raw<T, R>::kVec;
@@ -433,7 +433,8 @@ __global__ __launch_bounds__(256, kHeld) void k_neighbor_forward(const NeighborA
 #pragma unroll
             for (int g = 0; g < GH; ++g) {
 #pragma unroll
-                for (int u = 0; u < kAhead; ++u) s[g][u] = head_sum<LPH>(q[g].dot(kx[u], 0.f));
+                for (int u = 0; u < kAhead; ++u)
+                    s[g][u] = head_sum<LPH>(l.mine ? q[g].dot(kx[u], 0.f) : 0.f);
                 const float ref = top[g] == -inf_of() ? 0.f : top[g];
                 capped_few<CAP>(s[g], a.rule, unused);
                 high[g] = -inf_of();
@@ -576,8 +577,8 @@ __global__ __launch_bounds__(256, kHeldBack) void k_neighbor_dq(const NeighborAr
                 float push = 0.f, s[GH], dp[GH], bend[GH];
 #pragma unroll
                 for (int g = 0; g < GH; ++g) {
-                    s[g] = head_sum<LPH>(q[g].dot(kx[u], 0.f));
-                    dp[g] = head_sum<LPH>(go[g].dot(vx[u], 0.f));
+                    s[g] = head_sum<LPH>(l.mine ? q[g].dot(kx[u], 0.f) : 0.f);
+                    dp[g] = head_sum<LPH>(l.mine ? go[g].dot(vx[u], 0.f) : 0.f);
                 }
                 capped_few<CAP>(s, a.rule, bend);
 #pragma unroll
@@ -697,8 +698,8 @@ __global__ __launch_bounds__(256, kHeldBack) void k_neighbor_dkv(const NeighborA
 #pragma unroll
                         for (int g = 0; g < GH; ++g) {
                             if (!whole && !in) qx[u][g] = ox[u][g] = Raw<T, R>{};
-                            s[g] = head_sum<LPH>(qx[u][g].dot(k, 0.f));
-                            dp[g] = head_sum<LPH>(ox[u][g].dot(v, 0.f));
+                            s[g] = head_sum<LPH>(mine ? qx[u][g].dot(k, 0.f) : 0.f);
+                            dp[g] = head_sum<LPH>(mine ? ox[u][g].dot(v, 0.f) : 0.f);
                         }
                         capped_few<CAP>(s, a.rule, bend);
 #pragma unroll
