@@ -266,3 +266,24 @@ def test_no_queries_need_no_positions(lib):  # noqa: F811
     # (the workspace is refused, which comes after the sizes)
     code, said = refused(lib.tnr_structure_backward, structure(n_queries=0), None, 0)
     assert code == ext.TNR_INPUT_ERROR and "workspace" in said
+
+
+@pytest.mark.parametrize("changed,message", [
+    ({"softcap": 1e-46}, "softcap must be finite and positive"),
+    ({"softcap": 1e39}, "softcap must be finite and positive"),
+    ({"scale": -1e39}, "scale must be finite"),
+])
+def test_scores_beyond_32_bits(changed, message):
+    with pytest.raises(ValueError, match=message):
+        structure_attention(**attention_arguments(**changed))
+    if "scale" in changed:
+        with pytest.raises(ValueError, match=message):
+            species_embedding(torch.zeros(3, dtype=torch.int64), torch.zeros(4, 8), **changed)
+
+
+def test_score_rules_beyond_32_bits(lib):  # noqa: F811
+    for rule in (dict(scale=0.25, softcap=1e-40), dict(scale=3e38), dict(softcap=3e38)):
+        for req, forward in ((structure(**rule), lambda r: refused(lib.tnr_structure_forward, r, PTR, 1 << 40)),
+                             (neighbor(**rule), lambda r: refused(lib.tnr_neighbor_forward, r))):
+            code, said = forward(req)
+            assert code == ext.TNR_INPUT_ERROR and "too large for 32 bits" in said

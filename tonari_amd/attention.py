@@ -15,6 +15,7 @@ No counterpart in the reference, which ends at the neighbor list.
 
 from __future__ import annotations
 
+from ctypes import c_float
 from math import isfinite, sqrt
 from typing import NamedTuple
 
@@ -60,14 +61,15 @@ def _check_ptr(name: str, ptr: Tensor) -> None:
 
 
 def _score_rule(q: Tensor, scale: float | None, softcap: float | None) -> tuple[float, float]:
-    scale = 1.0 / sqrt(q.shape[2]) if scale is None else float(scale)
+    # as the kernels take them: a cap that 32 bits round to 0 would be none
+    scale = c_float(1.0 / sqrt(q.shape[2]) if scale is None else float(scale)).value
     if not isfinite(scale):
-        raise ValueError("scale must be finite")
+        raise ValueError("scale must be finite in 32 bits")
     if softcap is None:
         return scale, 0.0
-    softcap = float(softcap)
+    softcap = c_float(float(softcap)).value
     if not isfinite(softcap) or softcap <= 0.0:
-        raise ValueError("softcap must be finite and positive")
+        raise ValueError("softcap must be finite and positive in 32 bits")
     return scale, softcap
 
 

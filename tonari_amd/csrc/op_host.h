@@ -56,6 +56,9 @@ inline int check_heads(int32_t dtype, int32_t heads, int32_t kv_heads, int32_t d
     if (!std::isfinite(scale)) return refuse(err, len, "scale must be finite");
     if (!std::isfinite(softcap) || softcap < 0.f)
         return refuse(err, len, "softcap must be finite and positive");
+    const ScoreRule rule = ScoreRule::of(scale, softcap);
+    if (!std::isfinite(rule.scale2) || !std::isfinite(rule.inv) || !std::isfinite(rule.cap2))
+        return refuse(err, len, "scale, softcap or scale / softcap is too large for 32 bits");
     return TNR_OK;
 }
 

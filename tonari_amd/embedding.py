@@ -5,6 +5,7 @@ No counterpart in the reference, which ends at the neighbor list.
 
 from __future__ import annotations
 
+from ctypes import c_float
 from math import isfinite
 
 import torch
@@ -36,9 +37,9 @@ def species_embedding(species: Tensor, weight: Tensor, *, scale: float = 1.0) ->
         raise ValueError("weight must have dtype float32, bfloat16 or float16")
     if species.device != weight.device:
         raise ValueError("species and weight must be on the same device")
-    scale = float(scale)
+    scale = c_float(float(scale)).value  # as the kernels take it
     if not isfinite(scale):
-        raise ValueError("scale must be finite")
+        raise ValueError("scale must be finite in 32 bits")
     if not weight.is_cuda:
         raise RuntimeError("species_embedding runs on ROCm (HIP) devices; move the tensors to a GPU")
     check_device(weight.device.index)
