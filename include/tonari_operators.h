@@ -76,7 +76,8 @@ int tnr_embedding_backward(const tnr_embedding* req, void* workspace, size_t wor
 typedef struct tnr_structure_attention {
     int32_t dtype;                  /* of q, k, v, out and their gradients */
     int32_t heads, kv_heads, dim;   /* dim: a multiple of 8, 8 to 128 */
-    int64_t n_structures, n_queries, n_keys;  /* below 2^30; rows of all heads below 2^31 */
+    int64_t n_structures, n_queries, n_keys;  /* below 2^30 (backward: together below
+                                                 1.4 * 10^9); rows of all heads below 2^31 */
     const int64_t* query_ptr;       /* [n_structures + 1] */
     const int64_t* key_ptr;         /* [n_structures + 1] (may be query_ptr) */
     const void* q;                  /* T[n_queries][heads][dim] */
@@ -120,7 +121,7 @@ int tnr_structure_backward(const tnr_structure_attention* req, void* workspace,
  * other sizes give NaN.  The first 32-bit word is 0 for a valid list. */
 typedef struct tnr_neighbor_list {
     int64_t n_pairs;                        /* up to 2^31 - 4097 */
-    int64_t n_sources, n_targets;           /* below 2^26 */
+    int64_t n_sources, n_targets;           /* up to 2^26 - 4 */
     const int64_t* sources;                 /* i: int64[n_pairs], those of an atom together */
     const int64_t* targets;                 /* j: int64[n_pairs] */
     int32_t transpose;                      /* 1: also by target, which the backward needs */

@@ -287,3 +287,20 @@ def test_score_rules_beyond_32_bits(lib):  # noqa: F811
                              (neighbor(**rule), lambda r: refused(lib.tnr_neighbor_forward, r))):
             code, said = forward(req)
             assert code == ext.TNR_INPUT_ERROR and "too large for 32 bits" in said
+
+
+def test_sizes_at_the_edge_of_a_launch(lib):  # noqa: F811
+    # 2^32 threads are one too many; (the workspace is refused after the sizes)
+    most = (1 << 26) - 4
+    for n, word in ((most, "workspace"), (most + 1, "too many")):
+        code, said = refused(lib.tnr_neighbor_rows, listing(n_targets=n), None, 0)
+        assert code == ext.TNR_INPUT_ERROR and word in said
+        code, said = refused(lib.tnr_neighbor_backward,
+                             neighbor(listing(n_sources=n), heads=1, kv_heads=1), None, 0)
+        assert code == ext.TNR_INPUT_ERROR and word in said
+    code, said = refused(lib.tnr_embedding_backward, embedding(n_species=1 << 58), PTR, 1 << 40)
+    assert code == ext.TNR_INPUT_ERROR and "too many" in said
+    for n, word in ((700_000_000, "workspace"), (720_000_000, "too many")):
+        code, said = refused(lib.tnr_structure_backward,
+                             structure(heads=1, kv_heads=1, n_queries=n, n_keys=n), None, 0)
+        assert code == ext.TNR_INPUT_ERROR and word in said, said

@@ -26,7 +26,7 @@ int check_embedding(const tnr_embedding* r, bool backward, char* err, size_t len
     if (r->n_atoms < 0 || r->n_species < 0 || r->channels < 1)
         return refuse(err, len, "invalid sizes");
     // a workgroup for each species, and at most 65,535 side by side for its channels
-    if (r->n_atoms >= INT32_MAX || r->n_species * 256 > kMostThreads || r->channels > (1 << 18))
+    if (r->n_atoms >= INT32_MAX || r->n_species > kMostThreads / 256 || r->channels > (1 << 18))
         return refuse(err, len, "too many atoms, species or channels");
     const bool rows = r->n_atoms > 0, table = r->n_species > 0;
     if ((rows && (!r->species || !(backward ? r->grad_out : r->out))) ||
@@ -137,7 +137,7 @@ void sort_species(const tnr_embedding& r, const EmbeddingSpace& s, RunArgs& runs
 
 // -------------------------------------------------------- neighbor attention
 
-constexpr int64_t kMostAtoms = int64_t(1) << 26;  // a wave each
+constexpr int64_t kMostAtoms = kMostThreads / 256 * 4 + 1;  // a wave each, four to a workgroup
 
 int check_list(const tnr_neighbor_list* l, char* err, size_t len) {
     if (!l) return refuse(err, len, "list is null");

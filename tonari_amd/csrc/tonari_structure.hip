@@ -67,7 +67,10 @@ int check_structure(const tnr_structure_attention* r, bool backward, char* err, 
         r->n_queries >= kMostAtoms || r->n_keys >= kMostAtoms || r->n_structures >= kMostAtoms)
         return refuse(err, len, "too many atoms");
     const StructurePlan p = structure_plan(*r);
-    if (p.q_tiles * r->kv_heads * p.q_waves * kWave > kMostThreads ||
+    // (the last kernel back: a thread for each coordinate, a workgroup for each slope)
+    const int64_t coordinates = 3 * (r->n_queries + r->n_keys) + 1024 * (int64_t)(r->heads + 1);
+    if ((backward && coordinates > kMostThreads) ||
+        p.q_tiles * r->kv_heads * p.q_waves * kWave > kMostThreads ||
         p.k_tiles * r->kv_heads * p.k_waves * kWave > kMostThreads)
         return refuse(err, len, "too many atoms");
     if (r->n_structures > 0 && (!r->query_ptr || !r->key_ptr))
