@@ -502,3 +502,17 @@ def test_graph_of_a_row_without_weight():
         assert_near(a, e)
     for t in torch.autograd.grad(sum((t * t).sum() for t in graph), leaves):
         assert bool(torch.isfinite(t).all())
+
+
+def test_graph_beyond_the_memory():
+    c = make([1500], 8, 8, 64, torch.float32, seed=34)
+    out = call(c)
+    torch.cuda.empty_cache()
+    total = torch.cuda.get_device_properties(0).total_memory
+    torch.cuda.set_per_process_memory_fraction(2.0 * 2**30 / total)
+    try:
+        with pytest.raises(torch.OutOfMemoryError, match="create_graph holds .* fewer structures"):
+            torch.autograd.grad(out, c["positions"], c["upstream"], create_graph=True)
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+    assert bool(torch.isfinite(torch.autograd.grad(out, c["positions"], c["upstream"])[0]).all())

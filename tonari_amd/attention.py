@@ -10,6 +10,11 @@ layout of ``neighbor_list`` (positions and batch_ptr) and attends to all atoms o
 images.  Both are differentiable in everything that is real; the gradient of d goes on through the
 list to positions and cell.  Query heads may share key and value heads.
 
+A gradient's own graph (``create_graph=True``, as training on forces takes) is built of torch operations
+over all pairs of a query and a key: it holds several tensors of pairs x heads x dim floats (a structure
+of 1,000 atoms with 8 heads of 64 has 2 GB in each), waits for the device to count the pairs, and its
+sums are torch's, whose order may change from run to run.
+
 No counterpart in the reference, which ends at the neighbor list.
 """
 

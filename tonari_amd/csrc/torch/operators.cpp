@@ -185,8 +185,9 @@ Tensor species_embedding(const Tensor& species, const Tensor& weight, double sca
 // ------------------------------------------------- attention, as an expression
 
 // Attention over pairs (source, target) at distances r, in 32-bit torch
-// operations: what a graph of the gradient is built from.
-Tensor pair_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& r,
+// operations: what a graph of the gradient is built from.  It holds the rows of q, k and
+// v of every pair and head.
+Tensor pair_expression(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& r,
                       const Tensor& slopes, const Tensor& source, const Tensor& target,
                       double scale, double softcap) {
     const int64_t n = q.size(0), heads = q.size(1), dim = q.size(2), group = heads / k.size(1);
@@ -208,6 +209,21 @@ Tensor pair_attention(const Tensor& q, const Tensor& k, const Tensor& v, const T
     return at::zeros({n, heads, dim}, e.options())
         .index_add(0, source, p.unsqueeze(-1) * wide(v))
         .to(q.scalar_type());
+}
+
+Tensor pair_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& r,
+                      const Tensor& slopes, const Tensor& source, const Tensor& target,
+                      double scale, double softcap) {
+    try {
+        return pair_expression(q, k, v, r, slopes, source, target, scale, softcap);
+    } catch (const c10::OutOfMemoryError& e) {
+        const double gib = 4.0 * (double)source.numel() * q.size(1) * q.size(2) / (1 << 30);
+        TORCH_CHECK_WITH(OutOfMemoryError, false,
+                         "create_graph holds several tensors of pairs x heads x dim floats (",
+                         source.numel(), " x ", q.size(1), " x ", q.size(2), ": ", gib,
+                         " GiB each); take the gradient of fewer structures at a time.  ",
+                         e.what_without_backtrace());
+    }
 }
 
 // 1 or, where `ok` (a truth value on the device) does not hold, NaN: inputs are
