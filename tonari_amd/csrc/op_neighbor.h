@@ -12,11 +12,11 @@
 //
 // What bounds it: where the rows of all atoms outgrow the 4 MB L2 of an XCD and
 // the list is not in spatial order, the rate behind the L2 (100,000 atoms, 9 M
-// pairs, 8 heads of 16 bfloat16: 4.6 GB in 574 us, 8.0 TB/s); else what is done
-// for each score (256 crystals, 1.3 M pairs, 8 capped heads of 16 floats: 51 us
-// forward, 73 and 67 back).  Fewer registers and more waves lost: 32,768 atoms
-// with 4 query heads to a key head took 181 us at five waves to a SIMD and 137
-// at four.
+// pairs, 8 heads of 16 bfloat16: 4.6 GB in 593 us, 7.8 TB/s); else what is done
+// for each score (256 crystals, 1.3 M pairs, 8 capped heads of 16 floats: 48 us
+// forward, 70 and 63 back, vector instructions in 74 to 80 % of the busy cycles).
+// Fewer registers and more waves lose: 32,768 atoms with 4 query heads to a key head
+// take 179 us at five waves to a SIMD and 131 at four.
 //
 // Backward: by sources (grad_q, and grad_d, which needs the sum over heads of
 // one pair), then by targets in the list's transposed order (grad_k, grad_v),

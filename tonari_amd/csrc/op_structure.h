@@ -29,14 +29,16 @@
 // the largest keep digits down to 2^-31 of it.
 //
 // What bounds it: vector instructions, not the matrix cores.  A tile of 32 x 32
-// and one head takes about 25 instructions for each of a lane's 16 products
-// (distance 7, cap 10, the rest softmax) besides three that run at a quarter of
-// the rate, and 8 matrix products of 32 cycles for 64 channels.  Measured: 4,001
-// atoms, 8 capped heads of 64 on 2 key heads, bfloat16, 141 us (0.23 PFLOP/s,
-// vector units 70 % busy); 1,024 molecules of 20 to 120 atoms, 8 heads of 32,
-// 60 us, where a wave has two or three tiles and waits for their rows; float32
-// is bound by its matrix products, a sixteenth of the rate (48 structures of 1
-// to 509 atoms, 4 heads of 48: 89 us).
+// and one head takes about 29 instructions for each of a lane's 16 products
+// (distance 7, cap 10, the weights' two pieces 4, the rest softmax) besides three
+// that run at a quarter of the rate, and 12 matrix products of 32 cycles for 64
+// channels.  Measured: 4,001 atoms, 8 capped heads of 64 on 2 key heads, bfloat16,
+// 145 us (0.23 PFLOP/s, vector instructions in 79 % of the busy cycles, matrix
+// products in 15 %); 1,024 molecules of 20 to 120 atoms, 8 heads of 32, 71 us
+// (vector instructions in 94 %); one query in each of 64 structures of 2,000 to 20,000
+// atoms, 8 heads of 64 on 2, 123 us (the keys' and values' rows); float32 is bound by
+// its matrix products, a sixteenth of the rate (48 structures of 1 to 509 atoms, 4
+// heads of 48: 85 us).
 #pragma once
 
 #include "op_common.h"

@@ -14,9 +14,9 @@
 //
 // Both recompute a tile's scores, which costs seven products of matrices in place
 // of five but needs no sums across workgroups.  As the forward they are bound by
-// vector instructions: 4,001 atoms, 8 capped heads of 64 on 2, bfloat16: 251 us by
-// queries (726 instructions a tile) and 244 by keys, at two waves to a SIMD, whose
-// accumulators and rows fill its registers.
+// vector instructions: 4,001 atoms, 8 capped heads of 64 on 2, bfloat16: 222 us by
+// queries (751 instructions a tile, 16 of them matrix products) and 247 by keys (701,
+// 24), at two waves to a SIMD, whose accumulators and rows fill its registers.
 //
 // 16-bit types: dx and p go through two products, rounded and rest, so that each
 // gradient is rounded once, at the end.

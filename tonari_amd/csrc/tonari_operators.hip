@@ -251,8 +251,8 @@ NeighborArgs neighbor_args(const tnr_neighbor_attention& r) {
 // head's channels (a power of two), GH query heads to a lane where they share a
 // key head.  What is done once for each score is done by every lane of a head,
 // so one query head takes two pieces where the channels allow: 256 crystals (1.3 M
-// pairs) of 8 capped heads of 16 floats take 51 + 74 + 67 us, forward and both
-// passes back, and 53 + 96 + 82 at one piece.
+// pairs) of 8 capped heads of 16 floats take 48 + 70 + 63 us, forward and both
+// passes back, and 51 + 89 + 75 at one piece.
 template <typename T, typename F>
 void with_lanes(int32_t dim, int group, bool cap, F&& f) {
     const auto capped = [&](auto lanes, auto of, auto pieces) {

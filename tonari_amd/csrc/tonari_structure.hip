@@ -9,10 +9,11 @@ namespace {
 
 // ------------------------------------------------------- structure attention
 
-// Waves of 32 rows in a workgroup, which share the staged keys.  With long
-// structures four; with short ones two, of which fewer lie beyond a structure's
-// end: 1,024 molecules of 20 to 120 atoms take 73 us at two and 84 at four, a
-// cluster of 4,001 atoms 246 us at four and 286 at two (its queries' gradients).
+// Waves of 32 rows in a workgroup, which share the staged keys, by the batch's mean
+// structure.  Four for long ones; for short ones two, of which fewer lie beyond a
+// structure's end: 1,024 molecules of 20 to 120 atoms take 70 us at two and 73 at
+// four (a training step over 256 of them 122 and 127), a cluster of 4,001 atoms 222
+// us at four and 235 at two by queries, 247 and 254 by keys.
 int waves_for(int64_t rows, int64_t structures) {
     const int64_t mean = structures > 0 ? rows / structures : 0;
     return mean <= 512 ? 2 : 4;
@@ -35,9 +36,10 @@ StructurePlan structure_plan(const tnr_structure_attention& r) {
     p.q_tiles = tile_start(r.n_queries, p.group, p.q_waves * kTile, r.n_structures);
     p.k_tiles = tile_start(r.n_keys, 1, p.k_waves * kTile, r.n_structures);
     // Few rows: the keys (or, for the keys' gradients, the rows) are split over
-    // workgroups, at least 8 tiles each, into as many waves as the device holds of
-    // the kernel at once (`held` to a SIMD): a cluster of 4,001 atoms at three
-    // waves for all kernels took a second round of half the workgroups back.
+    // workgroups, at least 8 tiles each of the batch's mean structure, into as many
+    // waves as the device holds of the kernel at once (`held` to a SIMD): a cluster of
+    // 4,001 atoms split for three waves in all kernels takes 231 + 16 and 263 + 11 us
+    // back, queries and keys with their joins, in place of 222 + 13 and 247 + 9.
     const auto split = [&](int64_t rows, int64_t others, int held) {
         const int64_t waves = (rows / kTile + r.n_structures) * r.kv_heads;
         const int64_t most = r.n_structures > 0 ? others / r.n_structures / (8 * kTile) : 0;
