@@ -516,3 +516,17 @@ def test_graph_beyond_the_memory():
     finally:
         torch.cuda.set_per_process_memory_fraction(1.0)
     assert bool(torch.isfinite(torch.autograd.grad(out, c["positions"], c["upstream"])[0]).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("softcap", [None, 4.0])
+@pytest.mark.parametrize("queries", [None, [3] * 50])
+def test_one_key_is_its_value(dtype, softcap, queries):
+    # the weight is 1 whatever the score, and nothing moves it: exact, to the bit
+    c = make([1] * 50, 4, 2, 24, dtype, queries=queries, seed=35)
+    out = call(c, softcap)
+    of = torch.arange(50, device=DEV) if queries is None else torch.arange(50, device=DEV).repeat_interleave(3)
+    assert torch.equal(out, c["v"][of].repeat_interleave(2, 1))
+    names = [n for n in LEAVES if c[n] is not None and n != "v"]
+    for n, t in zip(names, torch.autograd.grad(out, [c[n] for n in names], c["upstream"])):
+        assert bool((t == 0).all()), n

@@ -528,6 +528,10 @@ constexpr int waves_held(int dp) {
 // float16 has small values down to 2^-24 and large ones below 2^16.
 template <typename T>
 constexpr bool kNarrow = std::is_same_v<T, f16>;
+// The exponent that a row's largest weight has in the forward: reached exactly, so that
+// a row of one key is that key's value to the bit.
+template <typename T>
+constexpr float kWeightLift = kNarrow<T> ? 7.f : 0.f;
 
 // grid: (tiles * kv_heads, splits); NW waves of 32 query rows each.
 template <typename T, int DP, int NW, bool CAP>
@@ -627,13 +631,12 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP)) void k_structure_forw
     // Weights are taken relative to `top`, the maximum when it was last set: it
     // is set anew only where a score passes it by more than 2^8 (the row's sums
     // then change their unit), so that most tiles neither subtract nor rescale.
-    // A lift lowers `top` below that maximum: weights reach up to 2^(8 + kLift).
-    constexpr float kLift = kNarrow<T> ? 7.f : 0.f;
+    constexpr float kLift = kWeightLift<T>;
     const auto weigh = [&](int sub, int left) {
         f32x16 dot{};
         M::template rows<DP>(dot, k_rows + sub * Pair::kRows, qr, a.dim);
         float s[16], unused[4];
-        const float ref = top == -inf_of() ? 0.f : top;
+        const float ref = top == -inf_of() ? 0.f : top - kLift;
         const bool near = all_near<CAP>(dot, a.rule);
         float high = -inf_of();
 #pragma unroll
@@ -663,15 +666,15 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP)) void k_structure_forw
         high = max_halves(high);
         const bool anew = high > 8.f + kLift || (top == -inf_of() && high > -inf_of());
         if (__builtin_amdgcn_ballot_w64(anew) != 0) {
-            const float up = anew ? high - kLift : 0.f;
+            const float up = anew ? high : 0.f, lift = anew ? kLift : 0.f;
             // (the first maximum has no sums to fade, and may lie far below 0)
-            const float fade = exp2_of(fminf(-up, 0.f));
-            top = anew ? ref + up : top;
+            const float fade = exp2_of(fminf(lift - up, 0.f));
+            top = anew ? ref + high : top;
             sum *= fade;
 #pragma unroll
             for (int d = 0; d < DP / 32; ++d) acc[d] *= fade;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] -= up;
+            for (int i = 0; i < 16; ++i) s[i] = kNarrow<T> ? (s[i] - up) + lift : s[i] - up;
         }
         float part[4] = {};
         typename M::Weights p, rest;
@@ -718,7 +721,7 @@ __global__ __launch_bounds__(NW* kWave, waves_held<T>(DP)) void k_structure_forw
     if (a.out32) store_channels<float, DP>(a.out32 + flat, a.dim, acc, by);
     if (a.lse && half == 0)
         a.lse[(int64_t)head * a.n_queries + query] =
-            sum == 0.f ? -inf_of() : top + __builtin_amdgcn_logf(sum);
+            sum == 0.f ? -inf_of() : top + (__builtin_amdgcn_logf(sum) - kLift);
 }
 
 // Joins the splits of a row: one wave each, lanes over channels.
@@ -756,7 +759,8 @@ __global__ __launch_bounds__(256) void k_structure_join(const StructureArgs a) {
         if (lane + kWave < a.dim) a.out32[flat + lane + kWave] = x1 * by;
     }
     if (a.lse && lane == 0)
-        a.lse[at] = sum == 0.f ? -inf_of() : top + __builtin_amdgcn_logf(sum);
+        a.lse[at] = sum == 0.f ? -inf_of()
+                               : top + (__builtin_amdgcn_logf(sum) - kWeightLift<T>);
 }
 
 }  // namespace op
