@@ -23,9 +23,10 @@
 //
 // The distance is computed in the tile from the positions, 32 bits.  Scores,
 // statistics and sums are 32 bits.  The matrix products with 16-bit values take
-// 16-bit weights: these go in two pieces, rounded and rest, so that the output
-// is rounded once, at the end.  (One piece adds as much error as the output's own
-// rounding.)  float16 weights are lifted by 2^7, so that those of keys far below
+// 16-bit weights: these go in two pieces, rounded and rest, which hold 16 bits of a
+// bfloat16 weight and 22 of a float16 one.  Against the output's own rounding at the
+// end that is nothing (2 values in 1,000 round to their neighbour); one piece alone
+// adds as much error as it.  float16 weights are lifted by 2^7, so that those of keys far below
 // the largest keep digits down to 2^-31 of it.
 //
 // What bounds it: vector instructions, not the matrix cores.  A tile of 32 x 32
