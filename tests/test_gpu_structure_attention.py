@@ -10,8 +10,8 @@ from __future__ import annotations
 import pytest
 import torch
 
-from tests._operators import (HALF_SPACING, assert_near, attend, distances, double, pointer,
-                              structure_pairs, tolerance)
+from tests._operators import HALF_SPACING, assert_near, attend, distances, double, pointer, structure_pairs
+from tests._operators import tolerance
 from tonari_amd.attention import structure_attention
 
 pytestmark = pytest.mark.gpu
